@@ -572,6 +572,112 @@ int ihip_prompt_cache_stats(ihip_prompt_cache* pc, int64_t* requests, int64_t* h
                             int64_t* idle);
 
 /* ======================================================================
+ * several sequences decoded together over one paged cache (no counterpart in
+ * the reference, whose device decodes one sequence at a time): a layer's keys
+ * and values live in a pool of pages of page_size tokens, a block table lists
+ * each sequence's pages, and one call serves every sequence of the batch. A
+ * step is _paged_slots once, then per layer _paged_qkrope and
+ * _paged_attention between its Linears, then _logprobs beside the argmax.
+ * Every array is on the device and lengths are read there, so the calls can
+ * be captured once and replayed as the sequences grow; none allocates. What
+ * a table, a slot or a length holds is checked on the device: an entry
+ * outside the pool is read as "not there", never followed.
+ * ==================================================================== */
+
+/* the pool of one layer. A slot is page * page_size + token: the values of a
+ * token's KV head h start at page * page_stride + token * slot_stride + h *
+ * head_stride. Strides in values, 0 for those of [pages, page_size, kv_heads,
+ * head_dim]; [pages, kv_heads, page_size, head_dim] has head_stride
+ * page_size * head_dim and slot_stride head_dim. head_dim is a multiple of 8,
+ * up to 512; the addresses and strides are multiples of 16 bytes. */
+typedef struct {
+  uint64_t k, v;           /* device addresses of the keys and the values */
+  int64_t pages;
+  int64_t page_stride, slot_stride, head_stride;
+  int32_t page_size, kv_heads, head_dim;
+  int32_t dtype;           /* IHIP_F32, IHIP_F16 or IHIP_BF16 */
+} ihip_pages;
+
+/* rotary positions of q and k: value pairs (i, i + dims / 2) of a head's
+ * first dims values, or (2 i, 2 i + 1) when interleaved, turned by the angle
+ * freq[i] * position (formed in double) and scaled by `scale` */
+typedef struct {
+  uint64_t freq;           /* device address of [dims / 2] floats (ihip_model_frequencies) */
+  int32_t dims;            /* even, up to head_dim; 0: the whole head */
+  int32_t interleaved;
+  double scale;            /* YaRN's attention factor; 0: 1 */
+} ihip_rope;
+
+/* the frequencies that ihip_model_rotary's table is formed with (on the host):
+ * freq [rope_dims / 2], YaRN applied when rope_factor is set, and the factor of
+ * cos and sin (scale may be NULL) */
+int ihip_model_frequencies(const ihip_model_desc* desc, float* freq, double* scale);
+
+/* the plan of a step, from the sequences' lengths. Sequence s of the batch
+ * (at most IHIP_PAGED_SEQS) holds past[s] tokens and brings count[s] new ones
+ * (count 0: one each), or ends with count[s] < 0, its pages back to the free
+ * ones; past[s] < 0 is an empty place of the batch. All arrays are int32 but
+ * `ends`:
+ * - table [seqs, max_pages]: each sequence's pages in order; the pages that its
+ *   new tokens need are taken from the free ones, in the sequences' order, and
+ *   written behind those it has;
+ * - ring [pages] and ends (int64[2]): the free pages are ring[i mod pages] for
+ *   ends[0] <= i < ends[1]; ends_out receives the ends after the call. Pages
+ *   that ended sequences give back are there from the next call on;
+ * - offsets [seqs + 1]: the rows of sequence s are offsets[s] .. offsets[s + 1];
+ * - lengths [seqs]: past + count, -1 of an ended sequence or an empty place;
+ * - positions, slots [rows]: of every new token; -1 in the rows behind the last;
+ * - failed [1] (or 0): the sequences that got none of their new tokens, because
+ *   the free pages, max_pages or rows do not hold them: their slots are -1 and
+ *   their length stays past[s] (positions are given). Free pages too few for a
+ *   sequence leave none for those behind it that need one.
+ * ends_out may be ends, and lengths may be past. */
+#define IHIP_PAGED_SEQS 4096
+int ihip_enqueue_paged_slots(ihip_ctx* ctx, uint64_t past, uint64_t count, int64_t seqs,
+                             uint64_t table, int64_t max_pages, int64_t page_size, uint64_t ring,
+                             int64_t pages, uint64_t ends, uint64_t ends_out, uint64_t offsets,
+                             uint64_t lengths, uint64_t positions, uint64_t slots, int64_t rows,
+                             uint64_t failed);
+/* the new rows' q, k and v between the q/k/v Linear and the attention: per row
+ * and head the RMSNorm of q and k heads (qn, kn device [head_dim] or 0), rotary
+ * positions (rope, NULL: none), q written to q_out ([rows, heads, head_dim], or 0:
+ * in place), k and v stored into the cache at the row's slot. Strides: floats
+ * from a row to the next (0: the rows are contiguous). A row with position < 0
+ * is left as it was; a slot outside the pool stores nothing. The rows of one
+ * call have slots of their own. (ihip_enqueue_qkrope over a paged cache) */
+int ihip_enqueue_paged_qkrope(ihip_ctx* ctx, uint64_t q, int64_t q_stride, uint64_t k,
+                              int64_t k_stride, uint64_t v, int64_t v_stride, int64_t rows,
+                              int64_t heads, uint64_t qn, uint64_t kn, double eps,
+                              const ihip_rope* rope, uint64_t positions, uint64_t slots,
+                              const ihip_pages* cache, uint64_t q_out);
+/* attention of one new token of each sequence over its pages: y [seqs, heads,
+ * head_dim] = softmax(scale q k) v over the keys 0 .. lengths[s] - 1 (window > 0:
+ * the last `window` of them; sinks: device [heads] or 0; scale 0: 1 / sqrt(
+ * head_dim)); table [seqs, max_pages], q rows of q_stride floats (0: heads *
+ * head_dim). A key whose table entry is outside the pool is not there, one whose
+ * score is -infinity has weight 0. A sequence with no key (length 0) gives
+ * zeros, one with lengths[s] < 0 leaves its row of y as it was. (ihip_enqueue_attention over a paged cache) */
+int ihip_enqueue_paged_attention(ihip_ctx* ctx, uint64_t q, int64_t q_stride,
+                                 const ihip_pages* cache, uint64_t table, int64_t max_pages,
+                                 uint64_t lengths, uint64_t y, int64_t seqs, int64_t heads,
+                                 int64_t window, uint64_t sinks, double scale);
+/* what a row of logits says of its tokens: logits [rows, vocab], `stride` floats
+ * from a row to the next (0: vocab);
+ * - logprobs [rows] (or 0): log softmax of token ids[r] (int32), NaN for an id
+ *   outside the vocabulary;
+ * - entropy [rows] (or 0): of the softmax, in nats;
+ * - top_ids, top_logprobs [rows, k] (k up to IHIP_LOGPROBS_TOP, 0: none): the
+ *   largest logits first, the lowest id on a tie, NaN behind all others; where
+ *   the vocabulary is smaller than k, id -1 and -infinity.
+ * A logit of -infinity is a token of probability 0; a row of nothing else has
+ * log probabilities of -infinity and entropy 0. A NaN or +infinity makes the
+ * row's results NaN (its top ids stay in order). */
+#define IHIP_LOGPROBS_TOP 64
+int ihip_enqueue_logprobs(ihip_ctx* ctx, uint64_t logits, int64_t rows, int64_t vocab,
+                          int64_t stride, uint64_t ids, uint64_t logprobs, uint64_t entropy,
+                          int64_t k, uint64_t top_ids, uint64_t top_logprobs);
+
+/* ======================================================================
  * GGUF v3 files (TGgufFile, src/infer/mormot.ai.infer.loader.gguf.pas:94-170)
  * and the decoder description of a llama.cpp file
  * (NewDecoderModelFromGguf, decoder.pas:3491-3510)

@@ -22,10 +22,11 @@ HIPCC = os.path.join(ROCM, "bin", "hipcc")
 LINEAR_FMTS = ["q8_0", "q4_0", "mxfp4", "q5_0", "q5_1", "q4_k", "q6_k", "f32", "bf16", "f16"]
 # gemm.hip (the MFMA prefill GEMM) once per quantized weight type
 GEMM_FMTS = ["q8_0", "q4_0", "mxfp4", "q5_0", "q5_1", "q4_k", "q6_k", "f32", "bf16", "f16"]
-KERNELS = ([("ops", "ops", []), ("deltanet", "deltanet", [])] +
+KERNELS = ([("ops", "ops", []), ("deltanet", "deltanet", []), ("paged", "paged", []),
+            ("logprobs", "logprobs", [])] +
            [("linear_" + f, "linear", ["-DIHIP_ONLY_FMT_" + f.upper()]) for f in LINEAR_FMTS] +
            [("gemm_" + f, "gemm", ["-DIHIP_ONLY_FMT_" + f.upper()]) for f in GEMM_FMTS])
-HOST = ["runtime", "backend", "model", "synth", "gguf"]
+HOST = ["runtime", "backend", "model", "synth", "gguf", "paged"]
 # host sources compiled as HIP (a device array registered with the runtime)
 HOST_HIP = ["static_scratch"]
 HIP_FLAGS = ["--genco", "--offload-arch=gfx950", "-O3", "-std=c++17", "-ffp-contract=off",

@@ -2086,6 +2086,18 @@ using namespace ihip;
 
 extern "C" {
 
+int ihip_model_frequencies(const ihip_model_desc* d, float* freq, double* scale)
+{
+  if (!d || !freq || rope_dims(*d) < 2 || rope_dims(*d) & 1 || !(d->rope_theta > 0))
+    return fail(IHIP_E_ARG, "ihip_model_frequencies: rotary dims or theta");
+  std::vector<float> f;
+  float rs;
+  inv_freq(*d, f, rs);
+  std::copy(f.begin(), f.end(), freq);
+  if (scale) *scale = rs;
+  return 0;
+}
+
 int ihip_model_rotary(const ihip_model_desc* d, int64_t first, int64_t rows, float* cs)
 {
   if (!d || !cs || rows < 1 || d->head_dim < 2) return fail(IHIP_E_ARG, "ihip_model_rotary");

@@ -1,0 +1,233 @@
+// paged.cpp - several sequences decoded together over one paged cache: the
+// plan of a step, q/k/v into the pages, attention over them, and the log
+// probabilities of a row of logits. Arguments are checked before the context,
+// so that a host without a device can check a call.
+#include <algorithm>
+#include <climits>
+#include <cmath>
+#include <cstdio>
+#include <string>
+
+#include "internal.h"
+
+using namespace ihip;
+
+namespace {
+
+// the context's device made the caller's for the launches of one call
+struct OnDevice {
+  int before = -1;
+  explicit OnDevice(const ihip_ctx* c)
+  {
+    int now = 0;
+    if (hipGetDevice(&now) != hipSuccess || now == c->device) return;
+    if (hipSetDevice(c->device) == hipSuccess) before = now;
+  }
+  ~OnDevice()
+  {
+    if (before >= 0) (void)hipSetDevice(before);
+  }
+};
+
+int no_context(const char* who) { return fail(IHIP_E_ARG, std::string(who) + ": no context"); }
+
+int refuse(const char* who, const char* why, int code = IHIP_E_ARG)
+{
+  return fail(code, std::string(who) + ": " + why);
+}
+
+// a pool with its strides filled in
+struct Pool {
+  int64_t page_stride = 0, slot_stride = 0, head_stride = 0;
+  const char* type = "";
+};
+
+const char* type_name(int t) { return t == IHIP_F32 ? "f32" : t == IHIP_F16 ? "f16" : t == IHIP_BF16 ? "bf16" : nullptr; }
+
+int check_pool(const char* who, const ihip_pages* p, Pool* out)
+{
+  if (!p || !p->k || !p->v) return refuse(who, "no cache");
+  out->type = type_name(p->dtype);
+  if (!out->type) return refuse(who, "a cache that is not F32, F16 or BF16", IHIP_E_UNSUPPORTED);
+  if (p->head_dim < 8 || p->head_dim > 512 || p->head_dim % 8)
+    return refuse(who, "head_dim is a multiple of 8 up to 512", IHIP_E_UNSUPPORTED);
+  if (p->kv_heads < 1 || p->kv_heads > 65535 || p->page_size < 1 || p->pages < 1 ||
+      p->pages > INT32_MAX / p->page_size)
+    return refuse(who, "kv_heads, page_size or pages out of range");
+  const int64_t row = (int64_t)p->kv_heads * p->head_dim, es = p->dtype == IHIP_F32 ? 4 : 2;
+  out->head_stride = p->head_stride ? p->head_stride : p->head_dim;
+  out->slot_stride = p->slot_stride ? p->slot_stride : row;
+  out->page_stride = p->page_stride ? p->page_stride : row * p->page_size;
+  for (int64_t s : {out->head_stride, out->slot_stride, out->page_stride})
+    if (s < p->head_dim || s > (int64_t)1 << 40 || s * es % 16)
+      return refuse(who, "a stride below head_dim or not of 16 bytes");
+  // within a page 32 bits hold every offset
+  if (out->slot_stride * (p->page_size - 1) + out->head_stride * (p->kv_heads - 1) + p->head_dim > INT32_MAX)
+    return refuse(who, "a page of more than 2^31 values");
+  if (p->k % 16 || p->v % 16) return refuse(who, "a cache that is not aligned to 16 bytes");
+  return 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+int ihip_enqueue_paged_slots(ihip_ctx* c, uint64_t past, uint64_t count, int64_t seqs, uint64_t table,
+                             int64_t max_pages, int64_t page_size, uint64_t ring, int64_t pages,
+                             uint64_t ends, uint64_t ends_out, uint64_t offsets, uint64_t lengths,
+                             uint64_t positions, uint64_t slots, int64_t rows, uint64_t failed)
+{
+  const char* who = "ihip_enqueue_paged_slots";
+  if (!past || !table || !ring || !ends || !ends_out || !offsets || !lengths || !positions || !slots)
+    return refuse(who, "a missing array");
+  if (seqs > IHIP_PAGED_SEQS) return refuse(who, "more sequences than IHIP_PAGED_SEQS", IHIP_E_NOMEM);
+  if (seqs < 1 || rows < 1 || rows > INT32_MAX || page_size < 1 || page_size > INT32_MAX || pages < 1 ||
+      pages > INT32_MAX / page_size || max_pages < 1 || max_pages > INT32_MAX / page_size)
+    return refuse(who, "seqs, rows, page_size, pages or max_pages out of range");
+  if (ends % 8 || ends_out % 8) return refuse(who, "ends are int64, aligned to 8 bytes");
+  if (!c) return no_context(who);
+  OnDevice on(c);
+  struct {
+    const int *past, *count;
+    int *table, *ring;
+    const int64_t* ends;
+    int64_t* ends_out;
+    int *offsets, *lengths, *positions, *slots, *failed;
+    int* plan;
+    int32_t seqs, max_pages, page_size, pages, rows, here;
+  } a = {(const int*)past, (const int*)count, (int*)table, (int*)ring, (const int64_t*)ends,
+         (int64_t*)ends_out, (int*)offsets, (int*)lengths, (int*)positions, (int*)slots, (int*)failed,
+         (int*)c->paged_plan, (int32_t)seqs, (int32_t)max_pages, (int32_t)page_size, (int32_t)pages,
+         (int32_t)rows, rows <= PAGED_ROWS_HERE};
+  const size_t shmem = (size_t)seqs * 5 * 4 + 64;
+  int rc = launch(c, "paged_slots", dim3(1), dim3(1024), &a, shmem);
+  if (rc || a.here) return rc;
+  return launch(c, "paged_slots_rows", dim3((unsigned)std::min<int64_t>(4 * c->cus, (rows + 1023) / 1024)),
+                dim3(256), &a, shmem);
+}
+
+int ihip_enqueue_paged_qkrope(ihip_ctx* c, uint64_t q, int64_t q_stride, uint64_t k, int64_t k_stride,
+                              uint64_t v, int64_t v_stride, int64_t rows, int64_t heads, uint64_t qn,
+                              uint64_t kn, double eps, const ihip_rope* rope, uint64_t positions,
+                              uint64_t slots, const ihip_pages* cache, uint64_t q_out)
+{
+  const char* who = "ihip_enqueue_paged_qkrope";
+  Pool p;
+  if (int rc = check_pool(who, cache, &p)) return rc;
+  const int64_t hd = cache->head_dim, kvh = cache->kv_heads, qw = heads * hd, kw = kvh * hd;
+  if (!q || !k || !v || !positions || !slots) return refuse(who, "a missing array");
+  if (rows < 1 || rows > INT32_MAX || heads < 1 || heads > 65535 || heads % kvh)
+    return refuse(who, "rows or heads out of range");
+  q_stride = q_stride ? q_stride : qw;
+  k_stride = k_stride ? k_stride : kw;
+  v_stride = v_stride ? v_stride : kw;
+  if (q_stride < qw || k_stride < kw || v_stride < kw) return refuse(who, "a stride below a row");
+  const uint64_t aligned = q | k | v | q_out | qn | kn;
+  if (aligned % 4) return refuse(who, "floats aligned to 4 bytes");
+  if (!(eps >= 0) || !std::isfinite(eps)) return refuse(who, "eps");
+  int64_t dims = 0;
+  if (rope) {
+    dims = rope->dims ? rope->dims : hd;
+    if (!rope->freq || rope->freq % 4 || dims < 2 || dims > hd || dims & 1)
+      return refuse(who, "rope: freq, or dims odd or beyond head_dim");
+    if (!std::isfinite(rope->scale)) return refuse(who, "rope: scale");
+  }
+  if (!c) return no_context(who);
+  OnDevice on(c);
+  struct {
+    const float *q, *k, *v;
+    float* q_out;
+    const float *qn, *kn, *freq;
+    const int *positions, *slots;
+    char *kc, *vc;
+    int64_t q_stride, k_stride, v_stride, out_stride;
+    int64_t pages, page_stride, slot_stride, head_stride;
+    double eps, scale;
+    int32_t rows, heads, kvh, hd, page_size, half, interleaved, wide, seg, parts;
+  } a = {(const float*)q, (const float*)k, (const float*)v, (float*)(q_out ? q_out : q), (const float*)qn,
+         (const float*)kn, (const float*)(rope ? rope->freq : 0), (const int*)positions, (const int*)slots,
+         (char*)cache->k, (char*)cache->v, q_stride, k_stride, v_stride, q_out ? qw : q_stride,
+         cache->pages, p.page_stride, p.slot_stride, p.head_stride, eps,
+         rope && rope->scale != 0 ? rope->scale : 1.0, (int32_t)rows, (int32_t)heads, (int32_t)kvh,
+         (int32_t)hd, cache->page_size, (int32_t)(dims / 2), rope ? rope->interleaved != 0 : 0,
+         // 16-byte loads: rows aligned, and no unit of 4 pairs that only half turns
+         aligned % 16 == 0 && (q_stride | k_stride | v_stride) % 4 == 0 &&
+             (!rope || rope->interleaved || dims % 8 == 0),
+         1, 1};
+  while (a.seg * 8 < hd) a.seg *= 2;  // lanes of a head: 8 values each
+  const int64_t lanes = (heads + 2 * kvh) * a.seg;
+  // a block per row; where the rows leave the chip empty, more blocks share a row's heads
+  a.parts = (int32_t)std::max<int64_t>(1, std::min<int64_t>((lanes + 255) / 256, 2 * c->cus / rows));
+  char name[32];
+  snprintf(name, sizeof name, "paged_qkrope_%s", p.type);
+  return launch(c, name, dim3((unsigned)rows, (unsigned)a.parts), dim3(256), &a);
+}
+
+int ihip_enqueue_paged_attention(ihip_ctx* c, uint64_t q, int64_t q_stride, const ihip_pages* cache,
+                                 uint64_t table, int64_t max_pages, uint64_t lengths, uint64_t y,
+                                 int64_t seqs, int64_t heads, int64_t window, uint64_t sinks, double scale)
+{
+  const char* who = "ihip_enqueue_paged_attention";
+  Pool p;
+  if (int rc = check_pool(who, cache, &p)) return rc;
+  const int64_t hd = cache->head_dim, kvh = cache->kv_heads;
+  if (!q || !table || !lengths || !y) return refuse(who, "a missing array");
+  if (seqs > IHIP_PAGED_SEQS) return refuse(who, "more sequences than IHIP_PAGED_SEQS", IHIP_E_NOMEM);
+  if (seqs < 1 || heads < 1 || heads > 65535 || heads % kvh || window < 0 || max_pages < 1 ||
+      max_pages > INT32_MAX / cache->page_size)
+    return refuse(who, "seqs, heads, window or max_pages out of range");
+  q_stride = q_stride ? q_stride : heads * hd;
+  if (q_stride < heads * hd) return refuse(who, "a stride below a row");
+  if ((q | y | sinks | lengths | table) % 4) return refuse(who, "arrays aligned to 4 bytes");
+  if (std::isnan(scale) || std::isinf(scale)) return refuse(who, "scale");
+  if (!c) return no_context(who);
+  OnDevice on(c);
+  struct {
+    const float* q;
+    const char *kc, *vc;
+    const int *table, *lengths;
+    float* y;
+    const float* sinks;
+    int64_t q_stride, pages, page_stride, slot_stride, head_stride, window;
+    float scale;
+    int32_t seqs, heads, kvh, hd, page_size, max_pages;
+  } a = {(const float*)q, (const char*)cache->k, (const char*)cache->v, (const int*)table,
+         (const int*)lengths, (float*)y, (const float*)sinks, q_stride, cache->pages, p.page_stride,
+         p.slot_stride, p.head_stride, window,
+         (float)(scale > 0 ? scale : 1.0 / std::sqrt((double)hd)), (int32_t)seqs, (int32_t)heads,
+         (int32_t)kvh, (int32_t)hd, cache->page_size, (int32_t)max_pages};
+  char name[40];
+  snprintf(name, sizeof name, "paged_attention_%s", p.type);
+  return launch(c, name, dim3((unsigned)heads, (unsigned)seqs), dim3(256), &a);
+}
+
+int ihip_enqueue_logprobs(ihip_ctx* c, uint64_t logits, int64_t rows, int64_t vocab, int64_t stride,
+                          uint64_t ids, uint64_t logprobs, uint64_t entropy, int64_t k,
+                          uint64_t top_ids, uint64_t top_logprobs)
+{
+  const char* who = "ihip_enqueue_logprobs";
+  if (k < 0 || k > IHIP_LOGPROBS_TOP) return refuse(who, "more alternatives than IHIP_LOGPROBS_TOP", IHIP_E_NOMEM);
+  if (!logits || (logprobs && !ids) || (k && (!top_ids || !top_logprobs)) || (!logprobs && !entropy && !k))
+    return refuse(who, "a missing array");
+  if (rows < 1 || rows > INT32_MAX || vocab < 1 || vocab > 1 << 22)
+    return refuse(who, "rows or vocab out of range");
+  stride = stride ? stride : vocab;
+  if (stride < vocab) return refuse(who, "a stride below a row");
+  if ((logits | ids | logprobs | entropy | top_ids | top_logprobs) % 4)
+    return refuse(who, "arrays aligned to 4 bytes");
+  if (!c) return no_context(who);
+  OnDevice on(c);
+  struct {
+    const float* x;
+    int64_t stride;
+    const int* ids;
+    float *logprobs, *entropy;
+    int* top_ids;
+    float* top_logprobs;
+    int32_t rows, vocab, k, pad;
+  } a = {(const float*)logits, stride, (const int*)ids, (float*)logprobs, (float*)entropy,
+         (int*)top_ids, (float*)top_logprobs, (int32_t)rows, (int32_t)vocab, (int32_t)k, 0};
+  return launch(c, "logprobs", dim3((unsigned)rows), dim3(256), &a);
+}
+
+}  // extern "C"

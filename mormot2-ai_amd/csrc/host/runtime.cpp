@@ -47,8 +47,9 @@ hipFunction_t kernel(ihip_ctx* c, const char* name)
       c->kernels.emplace(name, f);
       return f;
     }
+    // a module without it: not an error that a later call may report
+    (void)hipGetLastError();
   }
-  (void)hipGetLastError();
   return nullptr;
 }
 
@@ -214,6 +215,12 @@ int ihip_create(int device, ihip_ctx** out)
     return fail(IHIP_E_NOMEM, "hipMalloc");
   }
   c->scratch_argmax = (uint64_t)am;
+  void* plan = nullptr;
+  if (hipMalloc(&plan, PAGED_PLAN_BYTES) != hipSuccess) {
+    ihip_destroy(c);
+    return fail(IHIP_E_NOMEM, "hipMalloc");
+  }
+  c->paged_plan = (uint64_t)plan;
   if (int rc = static_scratch_init(c)) {
     ihip_destroy(c);
     return rc;
@@ -235,7 +242,7 @@ void ihip_destroy(ihip_ctx* c)
   for (auto& w : c->weights) (void)hipFree((void*)w.dev);
   for (auto a : c->allocations) (void)hipFree((void*)a);
   for (uint64_t b : {c->scratch_x, c->scratch_y, c->scratch_q, c->scratch_bad, c->scratch_attn,
-                     c->scratch_argmax, c->scratch_split, c->scratch_planes})
+                     c->scratch_argmax, c->scratch_split, c->scratch_planes, c->paged_plan})
     if (b) (void)hipFree((void*)b);
   for (auto ev : c->events)
     if (ev) (void)hipEventDestroy(ev);

@@ -55,6 +55,23 @@ class GgufTensor(C.Structure):
                 ("data", C.c_void_p)]
 
 
+class Pages(C.Structure):
+    """The paged cache of one layer (ihip_pages)."""
+    _fields_ = [("k", C.c_uint64), ("v", C.c_uint64), ("pages", C.c_int64),
+                ("page_stride", C.c_int64), ("slot_stride", C.c_int64), ("head_stride", C.c_int64),
+                ("page_size", C.c_int32), ("kv_heads", C.c_int32), ("head_dim", C.c_int32),
+                ("dtype", C.c_int32)]
+
+
+class Rope(C.Structure):
+    """Rotary positions of q and k (ihip_rope)."""
+    _fields_ = [("freq", C.c_uint64), ("dims", C.c_int32), ("interleaved", C.c_int32),
+                ("scale", C.c_double)]
+
+
+PAGED_SEQS, LOGPROBS_TOP = 4096, 64
+
+
 def row_bytes(dtype, cols):
     bv, bs = BLOCK[dtype]
     return cols // bv * bs
@@ -158,6 +175,15 @@ def lib():
             "ihip_prompt_cache_stats": (i32, [vp, C.POINTER(i64), C.POINTER(i64), C.POINTER(i64),
                                               C.POINTER(i64)]),
             "ihip_model_timing": (i32, [vp, C.POINTER(C.c_double), C.POINTER(C.c_double)]),
+            "ihip_model_frequencies": (i32, [vp, vp, C.POINTER(C.c_double)]),
+            "ihip_enqueue_paged_slots": (i32, [vp, u64, u64, i64, u64, i64, i64, u64, i64, u64, u64,
+                                               u64, u64, u64, u64, i64, u64]),
+            "ihip_enqueue_paged_qkrope": (i32, [vp, u64, i64, u64, i64, u64, i64, i64, i64, u64,
+                                                u64, C.c_double, C.POINTER(Rope), u64, u64,
+                                                C.POINTER(Pages), u64]),
+            "ihip_enqueue_paged_attention": (i32, [vp, u64, i64, C.POINTER(Pages), u64, i64, u64,
+                                                   u64, i64, i64, i64, u64, C.c_double]),
+            "ihip_enqueue_logprobs": (i32, [vp, u64, i64, i64, i64, u64, u64, u64, i64, u64, u64]),
             "ihip_synth_blocks": (i32, [vp, i32, i64, i64, u64, i32, i32, i32]),
             "ihip_synth_normal": (i32, [vp, i32, i64, i64, u64, C.c_float, i32]),
             "ihip_gguf_open": (i32, [C.c_char_p, C.POINTER(vp)]),
