@@ -104,6 +104,7 @@ struct ihip_ctx {
   uint64_t scratch_argmax = 0;  // [ARGMAX_PARTS] block results of argmax_part
   uint64_t scratch_attn = 0, scratch_attn_bytes = 0;
   uint64_t paged_plan = 0;  // the step plan between ihip_enqueue_paged_slots' two launches
+  uint64_t paged_part = 0;  // paged_attention's shared pieces and counters (zero between launches)
   uint64_t scratch_planes = 0, scratch_planes_bytes = 0;  // e4m3 activation planes (gemm_mxfp4_f8)
   // the device address of static_scratch.hip's array on this device
   // (ihip_enqueue_linear_at_static), read once at ihip_create
@@ -151,6 +152,11 @@ void unpack(const void* src, void* dst, int dtype, int64_t out, int64_t in, int6
 constexpr int ARGMAX_PARTS = 1024;
 // rows of a step that paged_slots' one block writes itself
 constexpr int64_t PAGED_ROWS_HERE = 4096;
+// paged_attention: blocks of a launch at most, the pieces of sequences that they
+// share (the resident blocks' two each, whatever the lengths), and a counter of
+// 128 bytes a block behind them
+constexpr int64_t PAGED_BLOCKS = 1024;
+constexpr uint64_t PAGED_PART_BYTES = 17u << 20;
 constexpr uint64_t PAGED_PLAN_BYTES = (5 * IHIP_PAGED_SEQS + 4) * 4;
 
 struct LinearCall {

@@ -180,6 +180,11 @@ int ihip_enqueue_paged_attention(ihip_ctx* c, uint64_t q, int64_t q_stride, cons
   if (q_stride < heads * hd) return refuse(who, "a stride below a row");
   if ((q | y | sinks | lengths | table) % 4) return refuse(who, "arrays aligned to 4 bytes");
   if (std::isnan(scale) || std::isinf(scale)) return refuse(who, "scale");
+  // the kernels take tiles of 128 keys of 16-bit caches, 64 of single ones
+  const int64_t group = heads / kvh, tiles = (group + 15) / 16, tk = cache->dtype == IHIP_F32 ? 64 : 128;
+  const int64_t keys = window > 0 ? std::min(window, max_pages * cache->page_size) : max_pages * cache->page_size;
+  const int64_t units = (keys + tk - 1) / tk * kvh * tiles;
+  if (units > INT32_MAX / seqs) return refuse(who, "more than 2^31 tiles of keys", IHIP_E_NOMEM);
   if (!c) return no_context(who);
   OnDevice on(c);
   struct {
@@ -188,17 +193,25 @@ int ihip_enqueue_paged_attention(ihip_ctx* c, uint64_t q, int64_t q_stride, cons
     const int *table, *lengths;
     float* y;
     const float* sinks;
+    float* part;
+    int* done;
     int64_t q_stride, pages, page_stride, slot_stride, head_stride, window;
     float scale;
-    int32_t seqs, heads, kvh, hd, page_size, max_pages;
+    int32_t seqs, heads, kvh, hd, page_size, max_pages, group, tiles;
   } a = {(const float*)q, (const char*)cache->k, (const char*)cache->v, (const int*)table,
-         (const int*)lengths, (float*)y, (const float*)sinks, q_stride, cache->pages, p.page_stride,
+         (const int*)lengths, (float*)y, (const float*)sinks, (float*)c->paged_part,
+         (int*)(c->paged_part + PAGED_PART_BYTES), q_stride, cache->pages, p.page_stride,
          p.slot_stride, p.head_stride, window,
-         (float)(scale > 0 ? scale : 1.0 / std::sqrt((double)hd)), (int32_t)seqs, (int32_t)heads,
-         (int32_t)kvh, (int32_t)hd, cache->page_size, (int32_t)max_pages};
+         (float)((scale > 0 ? scale : 1.0 / std::sqrt((double)hd)) * 1.4426950408889634), (int32_t)seqs,
+         (int32_t)heads, (int32_t)kvh, (int32_t)hd, cache->page_size, (int32_t)max_pages, (int32_t)group,
+         (int32_t)tiles};
+  const int d = hd <= 64 ? 64 : hd <= 128 ? 128 : hd <= 256 ? 256 : 512;
   char name[40];
-  snprintf(name, sizeof name, "paged_attention_%s", p.type);
-  return launch(c, name, dim3((unsigned)heads, (unsigned)seqs), dim3(256), &a);
+  snprintf(name, sizeof name, "paged_attention_%s_%d%s", p.type, d, hd == d ? "" : "_part");
+  // as many blocks as reside at once, and as there are tiles and pieces for them
+  int64_t blocks = (int64_t)c->cus * resident_blocks(c, name, 256);
+  blocks = std::min<int64_t>({blocks, PAGED_BLOCKS, (int64_t)(PAGED_PART_BYTES / (2 * (16 * hd + 32) * 4)), units * seqs});
+  return launch(c, name, dim3((unsigned)blocks), dim3(256), &a);
 }
 
 int ihip_enqueue_logprobs(ihip_ctx* c, uint64_t logits, int64_t rows, int64_t vocab, int64_t stride,

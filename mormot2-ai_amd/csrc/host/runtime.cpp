@@ -221,6 +221,17 @@ int ihip_create(int device, ihip_ctx** out)
     return fail(IHIP_E_NOMEM, "hipMalloc");
   }
   c->paged_plan = (uint64_t)plan;
+  // fixed, so that a captured call holds an address that stays
+  void* part = nullptr;
+  if (hipMalloc(&part, PAGED_PART_BYTES + PAGED_BLOCKS * 128) != hipSuccess) {
+    ihip_destroy(c);
+    return fail(IHIP_E_NOMEM, "hipMalloc");
+  }
+  c->paged_part = (uint64_t)part;
+  if ((e = hipMemsetAsync((char*)part + PAGED_PART_BYTES, 0, PAGED_BLOCKS * 128, c->stream)) != hipSuccess) {
+    ihip_destroy(c);
+    return hip_fail(e, "hipMemsetAsync");
+  }
   if (int rc = static_scratch_init(c)) {
     ihip_destroy(c);
     return rc;
@@ -242,7 +253,7 @@ void ihip_destroy(ihip_ctx* c)
   for (auto& w : c->weights) (void)hipFree((void*)w.dev);
   for (auto a : c->allocations) (void)hipFree((void*)a);
   for (uint64_t b : {c->scratch_x, c->scratch_y, c->scratch_q, c->scratch_bad, c->scratch_attn,
-                     c->scratch_argmax, c->scratch_split, c->scratch_planes, c->paged_plan})
+                     c->scratch_argmax, c->scratch_split, c->scratch_planes, c->paged_plan, c->paged_part})
     if (b) (void)hipFree((void*)b);
   for (auto ev : c->events)
     if (ev) (void)hipEventDestroy(ev);

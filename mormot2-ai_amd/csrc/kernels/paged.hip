@@ -35,6 +35,7 @@ __device__ __forceinline__ int64_t scan_block(int64_t v, int64_t& total)
   __syncthreads();
   int64_t before = 0;
   total = 0;
+#pragma unroll 1
   for (int i = 0; i < SLOT_THREADS / 64; i++) {
     if (i < w) before += part[i];
     total += part[i];
@@ -115,15 +116,15 @@ extern "C" __global__ __launch_bounds__(SLOT_THREADS) void paged_slots(SlotArgs 
   extern __shared__ int slot_lds[];
   SlotPlan p = slot_plan(slot_lds, a.seqs);
   const int t = threadIdx.x, ps = a.page_size;
-  const int64_t width = a.max_pages, cap = width * ps;
+  const int64_t cap = (int64_t)a.max_pages * ps;
   const int64_t first = a.ends[0], last = a.ends[1];
   int64_t free_pages = first >= 0 && last > first ? last - first : 0;
   if (free_pages > a.pages) free_pages = a.pages;
   p.first = first >= 0 ? (int)(first % a.pages) : 0;
   p.last = last >= 0 ? (int)(last % a.pages) : 0;
 
-  int past[SLOT_PER], live[SLOT_PER];
-  int64_t fresh[SLOT_PER], have[SLOT_PER], rows = 0, back = 0;
+  int past[SLOT_PER], live[SLOT_PER], fresh[SLOT_PER], have[SLOT_PER];
+  int64_t rows = 0, back = 0;
 #pragma unroll
   for (int i = 0; i < SLOT_PER; i++) {
     const int s = t * SLOT_PER + i;
@@ -131,16 +132,16 @@ extern "C" __global__ __launch_bounds__(SLOT_THREADS) void paged_slots(SlotArgs 
     const int n = s < a.seqs && a.count ? a.count[s] : 1;
     live[i] = past[i] < 0 ? 0 : n < 0 ? 2 : 1;
     fresh[i] = live[i] == 1 ? n : 0;
-    have[i] = live[i] ? ((int64_t)past[i] + ps - 1) / ps : 0;
+    have[i] = live[i] ? (int)(((uint32_t)past[i] + ps - 1) / (uint32_t)ps) : 0;
     if (live[i] == 2) {  // no more than the table holds
-      if (have[i] > width) have[i] = width;
+      have[i] = min(have[i], a.max_pages);
       back += have[i];
     }
     rows += fresh[i];
   }
   int64_t all_rows, all_back, all_want, want = 0;
   int64_t row = scan_block(rows, all_rows), put = scan_block(back, all_back);
-  int64_t need[SLOT_PER];
+  int need[SLOT_PER];
   {
     int64_t r = row;
 #pragma unroll
@@ -148,9 +149,9 @@ extern "C" __global__ __launch_bounds__(SLOT_THREADS) void paged_slots(SlotArgs 
       r += fresh[i];
       need[i] = 0;
       if (live[i] == 1) {
-        const int64_t upto = past[i] + fresh[i];
+        const int64_t upto = (int64_t)past[i] + fresh[i];
         if (upto > cap || r > a.rows) live[i] = 3;  // has no place
-        else need[i] = (upto + ps - 1) / ps - have[i];
+        else need[i] = (int)(((uint32_t)upto + ps - 1) / (uint32_t)ps) - have[i];
       }
       want += need[i];
     }
@@ -436,10 +437,23 @@ struct PagedAttnArgs {
   const int *table, *lengths;
   float* y;
   const float* sinks;
+  float* part;  // [blocks][2][16 * hd + 32]: a block's pieces of sequences that other blocks share
+  int* done;    // [blocks] counters, 32 ints apart, zero between launches
   int64_t q_stride, pages, page_stride, slot_stride, head_stride, window;
-  float scale;
+  float scale;  // of the scores, times log2 e
   int32_t seqs, heads, kvh, hd, page_size, max_pages;
+  int32_t group, tiles;  // query heads of a KV head, in tiles of 16
 };
+
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef uint32_t uintx4 __attribute__((ext_vector_type(4)));
+typedef uint32_t uintx2 __attribute__((ext_vector_type(2)));
+
+constexpr float LOG2E = 1.44269504088896340736f;
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ bool finite(float x) { return (float_bits(x) & 0x7f800000u) != 0x7f800000u; }
 
 template <int T>
 __device__ __forceinline__ float load1(const char* p)
@@ -449,68 +463,605 @@ __device__ __forceinline__ float load1(const char* p)
   else return bits_float((uint32_t)*(const uint16_t*)p << 16);
 }
 
-// one block per (head, sequence): wave w takes keys w, w + 4, ..., its lanes the
-// dimensions, with a running maximum, sum and values; the waves meet at the end
 template <int T>
-__device__ __forceinline__ void paged_attention_t(const PagedAttnArgs& a)
+__device__ __forceinline__ floatx4 mfma16(uintx4 a, uintx4 b, floatx4 c)
 {
-  constexpr int ES = T == 0 ? 4 : 2, NV = 8;
-  __shared__ float acc_s[4][512];
-  __shared__ float ml[4][2];
-  const int h = blockIdx.x, s = blockIdx.y, t = threadIdx.x, lane = t & 63, w = t >> 6;
-  const int len = a.lengths[s], hd = a.hd;
-  if (len < 0) return;
-  int64_t lo, hi;
-  paged_range(len, a.window, a.max_pages, a.page_size, &lo, &hi);
-  const int64_t hoff = (int64_t)(h / (a.heads / a.kvh)) * a.head_stride;
-  float q[NV], acc[NV];
+  if constexpr (T == 1)
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+// two singles as NP parts of the cache's type that add up to them: halves (the
+// first towards zero, the second to nearest: 22 bits, of values scaled into a
+// half's normal range) or bf16 (towards zero: all 24 bits)
+template <int T>
+__device__ __forceinline__ void split2(float x, float y, uint32_t* part)
+{
+  if constexpr (T == 1) {
+    const auto hi = __builtin_amdgcn_cvt_pkrtz(x, y);
+    part[0] = __builtin_bit_cast(uint32_t, hi);
+    const _Float16 lx = (_Float16)(x - (float)hi[0]), ly = (_Float16)(y - (float)hi[1]);
+    part[1] = (uint32_t)__builtin_bit_cast(uint16_t, lx) | (uint32_t)__builtin_bit_cast(uint16_t, ly) << 16;
+  } else {
 #pragma unroll
-  for (int i = 0; i < NV; i++) {
-    const int d = lane + 64 * i;
-    q[i] = d < hd ? a.q[s * a.q_stride + (int64_t)h * hd + d] : 0.f;
-    acc[i] = 0.f;
-  }
-  float m = -__builtin_inff(), l = 0.f;
-  for (int64_t j = lo + w; j < hi; j += 4) {
-    const uint32_t pg = (uint32_t)j / (uint32_t)a.page_size;
-    const int64_t at = paged_value(a.table[(int64_t)s * a.max_pages + pg], (int)((uint32_t)j % (uint32_t)a.page_size),
-                                   a.pages, a.page_stride, a.slot_stride);
-    if (at < 0) continue;
-    float x = 0.f;
-#pragma unroll
-    for (int i = 0; i < NV; i++)
-      if (lane + 64 * i < hd) x = __builtin_fmaf(q[i], load1<T>(a.kc + (at + hoff + lane + 64 * i) * ES), x);
-    x = wave_sum(x, 64) * a.scale;
-    const float m2 = x > m || x != x ? x : m;
-    const float f = m == -__builtin_inff() ? 0.f : expf(m - m2), p = x == -__builtin_inff() ? 0.f : expf(x - m2);
-    l = l * f + p;
-    m = m2;
-#pragma unroll
-    for (int i = 0; i < NV; i++)
-      if (lane + 64 * i < hd) acc[i] = __builtin_fmaf(p, load1<T>(a.vc + (at + hoff + lane + 64 * i) * ES), acc[i] * f);
-  }
-#pragma unroll
-  for (int i = 0; i < NV; i++) acc_s[w][lane + 64 * i] = acc[i];
-  if (lane == 0) {
-    ml[w][0] = m;
-    ml[w][1] = l;
-  }
-  __syncthreads();
-  float M = a.sinks ? a.sinks[h] : -__builtin_inff();
-  for (int i = 0; i < 4; i++) M = ml[i][0] > M || ml[i][0] != ml[i][0] ? ml[i][0] : M;
-  float den = a.sinks && lo < hi ? expf(a.sinks[h] - M) : 0.f, f[4];
-  for (int i = 0; i < 4; i++) {
-    f[i] = ml[i][1] == 0.f ? 0.f : expf(ml[i][0] - M);
-    den += f[i] * ml[i][1];
-  }
-  for (int d = t; d < hd; d += 256) {
-    float v = 0;
-    for (int i = 0; i < 4; i++)
-      if (ml[i][1] != 0.f) v += f[i] * acc_s[i][d];
-    a.y[((int64_t)s * a.heads + h) * hd + d] = den != 0.f ? v / den : 0.f;
+    for (int i = 0; i < 3; i++) {
+      const uint32_t hx = float_bits(x), hy = float_bits(y);
+      part[i] = __builtin_amdgcn_perm(hy, hx, 0x07060302u);
+      x = x - bits_float(hx & 0xffff0000u);
+      y = y - bits_float(hy & 0xffff0000u);
+    }
   }
 }
 
-extern "C" __global__ __launch_bounds__(256) void paged_attention_f32(PagedAttnArgs a) { paged_attention_t<0>(a); }
-extern "C" __global__ __launch_bounds__(256) void paged_attention_f16(PagedAttnArgs a) { paged_attention_t<1>(a); }
-extern "C" __global__ __launch_bounds__(256) void paged_attention_bf16(PagedAttnArgs a) { paged_attention_t<2>(a); }
+// the maximum and the sum over the four lanes of a head (lanes c, c + 16, c + 32,
+// c + 48)
+__device__ __forceinline__ float quad_max(float v)
+{
+  v = fmaxf(v, xpart<16>(v));
+  return fmaxf(v, xpart<32>(v));
+}
+__device__ __forceinline__ float quad_sum(float v)
+{
+  v = v + xpart<16>(v);
+  return v + xpart<32>(v);
+}
+
+// what a block works on: keys [lo, hi) of a sequence, one KV head, 16 of its
+// query heads
+struct AttnItem {
+  int s, kv, tile;  // sequence, KV head, tile of its group
+  int heads;        // query heads of the tile
+  int head0;        // the first of them
+  int64_t lo, hi;   // the keys
+};
+
+template <int T, int D>
+struct AttnShape {
+  static constexpr int ES = T == 0 ? 4 : 2;            // bytes of a value
+  static constexpr int KS = T == 0 ? 16 : 32;          // keys of a wave's step
+  static constexpr int TK = 4 * KS;                    // keys of a block's tile
+  static constexpr int NT = KS / 16;                   // score tiles of a step
+  static constexpr int QL = 16 / ES;                   // values of a key load
+  static constexpr int NQ = D / (4 * QL);              // key loads of a lane and key
+  static constexpr int NP = T == 0 ? 1 : T == 1 ? 2 : 3;  // parts of a single value
+  static constexpr int VL = T != 0 && D > 64 ? 8 : 4;  // values of a value load
+  static constexpr int NJ = D / (16 * VL);             // value loads of a lane and key
+  static constexpr int OS = D + 4;                     // a head's row in o_s
+  static constexpr float P0 = T == 1 ? 15.f : 0.f;     // weights times 2^P0: halves' normal range
+};
+
+template <int T, int D>
+struct AttnLds {
+  using S = AttnShape<T, D>;
+  uintx4 q[S::NP * S::NQ * 64];  // the query tile as the matrix cores take it, by lane
+  float o[16 * S::OS];           // a piece's values
+  float m[16], l[16];            // its maxima and sums
+  float wm[4][16], wl[4][16];    // the waves'
+  float qs[16];                  // powers of two that the queries were divided by
+  int64_t off[4][2][S::KS];      // byte offsets of the steps' keys
+};
+
+// The heads of a piece whose sums are not all finite, again by the formula's own
+// steps in single: the matrix cores' parts turn an infinity into NaN (0 times it
+// is added), and a key of score -infinity has weight 0. Waves take keys in turn,
+// lanes dimensions. Slow, and only for such data.
+template <int T, int D>
+__device__ __forceinline__ void paged_walk(const PagedAttnArgs& a, const AttnItem& it, int64_t j0, int64_t j1,
+                                           AttnLds<T, D>& s)
+{
+  using S = AttnShape<T, D>;
+  constexpr int NV = D / 64;
+  float* const tmp = (float*)s.q;
+  const int t = threadIdx.x, lane = t & 63, w = t >> 6;
+  for (int h = 0; h < it.heads; h++) {
+    float q[NV], acc[NV];
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+      const int d = lane + 64 * i;
+      q[i] = d < a.hd ? a.q[it.s * a.q_stride + (int64_t)(it.head0 + h) * a.hd + d] * a.scale : 0.f;
+      acc[i] = 0.f;
+    }
+    float m = -__builtin_inff(), l = 0.f;
+    for (int64_t j = j0 + w; j < j1; j += 4) {
+      const uint32_t pg = (uint32_t)j / (uint32_t)a.page_size;
+      const int64_t at = paged_value(a.table[(int64_t)it.s * a.max_pages + pg], (int)((uint32_t)j % (uint32_t)a.page_size),
+                                     a.pages, a.page_stride, a.slot_stride);
+      if (at < 0) continue;
+      const int64_t row = (at + it.kv * a.head_stride) * S::ES;
+      float x = 0.f;
+#pragma unroll
+      for (int i = 0; i < NV; i++)
+        if (lane + 64 * i < a.hd) x = __builtin_fmaf(q[i], load1<T>(a.kc + row + (lane + 64 * i) * S::ES), x);
+      x = wave_sum(x, 64);
+      if (x == -__builtin_inff()) continue;
+      const float m2 = x > m || x != x ? x : m;
+      const float f = m == -__builtin_inff() ? 0.f : exp2_fast(m - m2), p = exp2_fast(x - m2);
+      l = l * f + p;
+      m = m2;
+#pragma unroll
+      for (int i = 0; i < NV; i++)
+        if (lane + 64 * i < a.hd)
+          acc[i] = __builtin_fmaf(p, load1<T>(a.vc + row + (lane + 64 * i) * S::ES), acc[i] * f);
+    }
+#pragma unroll
+    for (int i = 0; i < NV; i++) tmp[w * D + lane + 64 * i] = acc[i];
+    if (lane == 0) {
+      s.wm[w][0] = m;
+      s.wl[w][0] = l;
+    }
+    __syncthreads();
+    float M = -__builtin_inff(), L = 0.f, f[4];
+    for (int i = 0; i < 4; i++) M = s.wm[i][0] > M || s.wm[i][0] != s.wm[i][0] ? s.wm[i][0] : M;
+    for (int i = 0; i < 4; i++) {
+      f[i] = s.wl[i][0] == 0.f ? 0.f : exp2_fast(s.wm[i][0] - M);
+      L += f[i] * s.wl[i][0];
+    }
+    for (int d = t; d < a.hd; d += 256) {
+      float v = 0.f;
+      for (int i = 0; i < 4; i++)
+        if (s.wl[i][0] != 0.f) v += f[i] * tmp[i * D + d];
+      s.o[h * S::OS + d] = v;
+    }
+    if (t == 0) {
+      s.m[h] = M;
+      s.l[h] = L;
+    }
+    __syncthreads();
+  }
+}
+
+// the query tile into LDS in the lanes' order: lane (c, g) = (l & 15, l >> 4) holds
+// head c, values 4 QL i + QL g .. of load i; heads past the tile and values past
+// head_dim are 0. Halves: a head's values times a power of two, so that the
+// largest is below 2^14 and the second parts stay normal.
+template <int T, int D>
+__device__ __forceinline__ void stage_query(const PagedAttnArgs& a, const AttnItem& it, AttnLds<T, D>& s)
+{
+  using S = AttnShape<T, D>;
+  const int t = threadIdx.x;
+  const float* const q = a.q + it.s * a.q_stride + (int64_t)it.head0 * a.hd;
+  if constexpr (T == 1) {
+    const int c = t >> 4;
+    float top = 0.f;
+    if (c < it.heads)
+      for (int d = t & 15; d < a.hd; d += 16) top = fmaxf(top, fabsf(q[c * a.hd + d] * a.scale));
+    top = fmaxf(top, xpart<1>(top));
+    top = fmaxf(top, xpart<2>(top));
+    top = fmaxf(top, xpart<4>(top));
+    top = fmaxf(top, xpart<8>(top));
+    if ((t & 15) == 0) {
+      int e = (int)(float_bits(top) >> 23) - 126;  // top < 2^e
+      if (top == 0.f || !finite(top)) e = 14;
+      s.qs[c] = ldexpf(1.f, max(e - 14, -120));
+    }
+    __syncthreads();
+  }
+  for (int i = t; i < S::NQ * 64; i += 256) {
+    const int c = i & 15, d0 = (i >> 6) * 4 * S::QL + ((i >> 4) & 3) * S::QL;
+    float v[S::QL];
+    const bool in = c < it.heads && d0 < a.hd;
+    float f = a.scale;
+    if constexpr (T == 1) f = 1.f / s.qs[c];
+#pragma unroll
+    for (int j = 0; j < S::QL; j++) {
+      v[j] = in ? q[c * a.hd + d0 + j] : 0.f;
+      v[j] = T == 1 ? v[j] * a.scale * f : v[j] * f;
+    }
+    if constexpr (T == 0) {
+      s.q[i] = uintx4{float_bits(v[0]), float_bits(v[1]), float_bits(v[2]), float_bits(v[3])};
+    } else {
+      uint32_t part[4][S::NP];
+#pragma unroll
+      for (int j = 0; j < 4; j++) split2<T>(v[2 * j], v[2 * j + 1], part[j]);
+#pragma unroll
+      for (int n = 0; n < S::NP; n++) s.q[n * S::NQ * 64 + i] = uintx4{part[0][n], part[1][n], part[2][n], part[3][n]};
+    }
+  }
+  __syncthreads();
+}
+
+// Attention of one token of each sequence. The work of all sequences and KV heads
+// is one row of tiles of TK keys, shared out evenly over the grid's blocks
+// (ragged lengths leave no block idle, and a captured grid fits the lengths of
+// every replay); a block walks its tiles in pieces of one (sequence, KV head). A
+// piece that is the whole of its item is written at once; the others go to
+// `part`, and the last block of an item to arrive joins them in order.
+//
+// A wave takes KS keys a step. Scores are K q^T with the keys as the matrix
+// cores' rows and the group's heads as columns (16 of them, zeros past the
+// group), so that lane (c, g) holds head c's scores of keys 4 g .. 4 g + 3 of each
+// 16 - which is how the value product takes its weights: values V^T with
+// dimensions as rows, keys as the inner index, each lane loading 8 dimensions of
+// the 8 keys that it has the weights of and turning them by byte permutes in its
+// registers. No key, value or weight goes through LDS, and the running maximum, sum
+// and rescale are a lane's own. Queries and weights enter as 2 half or 3 bf16
+// parts (f32 caches: the f32 matrix cores), so the sums are those of single.
+// HBM bound: the cache is read once.
+template <int T, int D, bool FULL>
+__device__ __forceinline__ void paged_attention_t(const PagedAttnArgs& a)
+{
+  using S = AttnShape<T, D>;
+  __shared__ AttnLds<T, D> s;
+  const int t = threadIdx.x, lane = t & 63, c = lane & 15, g = lane >> 4;
+  const int w = __builtin_amdgcn_readfirstlane(t >> 6);
+  const uint32_t grid = gridDim.x, b = blockIdx.x, per = a.kvh * a.tiles;
+  const int hd = FULL ? D : a.hd, row_out = a.heads * a.hd;
+
+  auto tiles_of = [&](int seq, int64_t& lo, int64_t& hi) {
+    paged_range(a.lengths[seq], a.window, a.max_pages, a.page_size, &lo, &hi);
+    return (uint32_t)((hi - lo + S::TK - 1) / S::TK);
+  };
+  // all tiles (each wave for itself); rows without a key are zeros
+  uint32_t all = 0;
+  for (int s0 = 0; s0 < a.seqs; s0 += 64) {
+    const int seq = s0 + lane;
+    uint32_t n = 0;
+    bool zero = false;
+    if (seq < a.seqs) {
+      int64_t lo, hi;
+      n = tiles_of(seq, lo, hi);
+      zero = n == 0 && a.lengths[seq] >= 0 && (uint32_t)seq % grid == b;
+    }
+    all += n * per;
+    for (uint64_t z = __ballot(zero); z; z &= z - 1) {
+      float* const y = a.y + (int64_t)(s0 + __builtin_ctzll(z)) * row_out;
+      for (int i = t; i < row_out; i += 256) y[i] = 0.f;
+    }
+  }
+  all = __builtin_amdgcn_readfirstlane(wave_sum(all, 64));
+  // block i of those with a tile takes tiles first(i) .. first(i + 1) - 1
+  const uint32_t B = min(grid, all);
+  if (b >= B) return;
+  const uint32_t quot = all / B, rem = all % B;
+  auto first = [&](uint32_t i) { return i * quot + i * rem / B; };
+  uint32_t u = first(b);
+  const uint32_t end = first(b + 1);
+  // the sequence of tile u
+  int seq = 0;
+  uint32_t before = 0, n = 0;  // tiles before the sequence, tiles of a KV head's item
+  int64_t lo = 0, hi = 0;
+  for (int s0 = 0;; s0 += 64) {
+    uint32_t m = 0;
+    int64_t l2, h2;
+    if (s0 + lane < a.seqs) m = tiles_of(s0 + lane, l2, h2) * per;
+    uint32_t upto = m;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      const uint32_t o = __shfl_up(upto, d, 64);
+      if (lane >= d) upto += o;
+    }
+    const uint64_t there = __ballot(before + upto > u);
+    if (there) {
+      const int f = __builtin_ctzll(there);
+      seq = __builtin_amdgcn_readfirstlane(s0 + f);
+      before = __builtin_amdgcn_readfirstlane(before + __shfl(upto - m, f, 64));
+      break;
+    }
+    before = __builtin_amdgcn_readfirstlane(before + __shfl(upto, 63, 64));
+  }
+  n = tiles_of(seq, lo, hi);
+
+  for (;;) {
+    const uint32_t item = (u - before) / n, tile0 = (u - before) - item * n;
+    const uint32_t tile1 = min(n, tile0 + (end - u));
+    AttnItem it;
+    it.s = seq;
+    it.kv = item / a.tiles;
+    it.tile = item - it.kv * a.tiles;
+    it.heads = min(16, a.group - 16 * it.tile);
+    it.head0 = it.kv * a.group + 16 * it.tile;
+    it.lo = lo;
+    it.hi = hi;
+    stage_query<T, D>(a, it, s);
+
+    const float sscale = T == 1 ? s.qs[c] : 1.f;
+    const char* const kb = a.kc + (int64_t)it.kv * a.head_stride * S::ES;
+    const char* const vb = a.vc + (int64_t)it.kv * a.head_stride * S::ES;
+    const int* const table = a.table + (int64_t)seq * a.max_pages;
+    const int64_t wlo = lo + w * S::KS;
+    // a step's key of this lane: its page's table entry
+    auto entry = [&](uint32_t tile) {
+      const int64_t j = wlo + (int64_t)tile * S::TK + (lane & (S::KS - 1));
+      return j < hi ? table[(uint32_t)j / (uint32_t)a.page_size] : -1;
+    };
+    // the offsets of a step's keys into LDS, the keys that are there as bits
+    auto locate = [&](uint32_t tile, int page) {
+      const int64_t j = wlo + (int64_t)tile * S::TK + (lane & (S::KS - 1));
+      const int64_t at = paged_value(page, (int)((uint32_t)j % (uint32_t)a.page_size), a.pages, a.page_stride, a.slot_stride);
+      if (lane < S::KS) s.off[w][tile & 1][lane] = at < 0 ? 0 : at * S::ES;
+      // other lanes read it: no instruction, but no reordering or forwarding past here
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      return (uint32_t)__ballot(at >= 0) & (uint32_t)((1ull << S::KS) - 1);
+    };
+    uintx4 kr[S::NT][S::NQ];
+    auto load_keys = [&](uint32_t tile) {
+#pragma unroll
+      for (int i = 0; i < S::NT; i++) {
+        const char* const p = kb + s.off[w][tile & 1][16 * i + c];
+#pragma unroll
+        for (int j = 0; j < S::NQ; j++) {
+          const int d0 = j * 4 * S::QL + g * S::QL;
+          const bool in = FULL || d0 < hd;
+          kr[i][j] = *(const uintx4*)(p + (in ? d0 : 0) * S::ES);
+          if (!in) kr[i][j] = uintx4{0, 0, 0, 0};
+        }
+      }
+    };
+
+    floatx4 o[S::NJ][S::VL];
+#pragma unroll
+    for (int i = 0; i < S::NJ; i++)
+#pragma unroll
+      for (int j = 0; j < S::VL; j++) o[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+    float m = -__builtin_inff(), l = 0.f;
+    uint32_t tile = tile0;
+    uint32_t steps = 0;  // of this wave: up to the last tile with a key of its own
+    if (wlo + (int64_t)tile0 * S::TK < hi) {
+      const uint32_t mine = (uint32_t)((hi - wlo + S::TK - 1) / S::TK);
+      steps = min(tile1, mine) - tile0;
+    }
+    // The loop has no branch between a product and what reads it, so keys are
+    // located and loaded one step past the last too: entry() has no page there and
+    // the loads read the pool's first row.
+    uint32_t there = locate(tile, entry(tile));
+    int page = entry(tile + 1);
+    if (steps) load_keys(tile);
+    for (uint32_t i = 0; i < steps; i++, tile++) {
+      // the step's values, on their way while its scores are formed
+      constexpr int NV = 4 * S::NT;  // keys of a lane: 16 q + 4 g + r
+      uintx4 vr[NV][S::NJ];
+#pragma unroll
+      for (int k = 0; k < NV; k++) {
+        const char* const p = vb + s.off[w][tile & 1][16 * (k >> 2) + 4 * g + (k & 3)];
+#pragma unroll
+        for (int j = 0; j < S::NJ; j++) {
+          const int d0 = j * 16 * S::VL + c * S::VL;
+          const char* const v = p + (FULL || d0 < hd ? d0 : 0) * S::ES;
+          if constexpr (S::VL * S::ES == 16) {
+            vr[k][j] = *(const uintx4*)v;
+          } else {
+            const uintx2 h = *(const uintx2*)v;
+            vr[k][j] = uintx4{h[0], h[1], 0, 0};
+          }
+        }
+      }
+      const uint32_t now = there;
+      there = locate(tile + 1, page);
+      page = entry(tile + 2);
+      floatx4 x[S::NT];
+#pragma unroll
+      for (int k = 0; k < S::NT; k++) x[k] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int j = 0; j < S::NQ; j++) {
+#pragma unroll
+        for (int n2 = 0; n2 < S::NP; n2++) {
+          const uintx4 q = s.q[(n2 * S::NQ + j) * 64 + lane];
+#pragma unroll
+          for (int k = 0; k < S::NT; k++) {
+            if constexpr (T == 0) {
+#pragma unroll
+              for (int e = 0; e < 4; e++)
+                x[k] = __builtin_amdgcn_mfma_f32_16x16x4f32(bits_float(kr[k][j][e]), bits_float(q[e]), x[k], 0, 0, 0);
+            } else {
+              x[k] = mfma16<T>(kr[k][j], q, x[k]);
+            }
+          }
+        }
+      }
+      load_keys(tile + 1);
+      // masked keys: no weight, and values of zero (0 times NaN is NaN)
+      float top = -__builtin_inff();
+      if (now == (uint32_t)((1ull << S::KS) - 1)) {
+#pragma unroll
+        for (int k = 0; k < S::NT; k++)
+#pragma unroll
+          for (int r = 0; r < 4; r++) {
+            x[k][r] = x[k][r] * sscale;
+            top = fmaxf(top, x[k][r]);
+          }
+      } else {
+#pragma unroll
+        for (int k = 0; k < NV; k++) {
+          const bool in = now >> (16 * (k >> 2) + 4 * g + (k & 3)) & 1;
+          x[k >> 2][k & 3] = in ? x[k >> 2][k & 3] * sscale : -__builtin_inff();
+          top = fmaxf(top, x[k >> 2][k & 3]);
+#pragma unroll
+          for (int j = 0; j < S::NJ; j++)
+            if (!in) vr[k][j] = uintx4{0, 0, 0, 0};
+        }
+      }
+      top = quad_max(top);
+      if (__any(top > m)) {
+        const float m2 = fmaxf(top, m), f = m == -__builtin_inff() ? 0.f : exp2_fast(m - m2);
+        m = m2;
+        l *= f;
+#pragma unroll
+        for (int j = 0; j < S::NJ; j++)
+#pragma unroll
+          for (int e = 0; e < S::VL; e++) o[j][e] *= f;
+      }
+      const float shift = (m == -__builtin_inff() ? 0.f : m) - S::P0;
+      float p[NV];
+#pragma unroll
+      for (int k = 0; k < NV; k++) {
+        p[k] = exp2_fast(x[k >> 2][k & 3] - shift);
+        l += p[k];
+      }
+      if constexpr (T == 0) {
+#pragma unroll
+        for (int k = 0; k < NV; k++)
+#pragma unroll
+          for (int j = 0; j < S::NJ; j++)
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+              o[j][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(bits_float(vr[k][j][e]), p[k], o[j][e], 0, 0, 0);
+      } else {
+        uint32_t part[4][S::NP];
+#pragma unroll
+        for (int k = 0; k < 4; k++) split2<T>(p[2 * k], p[2 * k + 1], part[k]);
+#pragma unroll
+        for (int j = 0; j < S::NJ; j++)
+#pragma unroll
+          for (int e = 0; e < S::VL; e++) {
+            uintx4 v;
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+              v[k] = __builtin_amdgcn_perm(vr[2 * k + 1][j][e / 2], vr[2 * k][j][e / 2], e & 1 ? 0x07060302u : 0x05040100u);
+#pragma unroll
+            for (int n2 = 0; n2 < S::NP; n2++)
+              o[j][e] = mfma16<T>(v, uintx4{part[0][n2], part[1][n2], part[2][n2], part[3][n2]}, o[j][e]);
+          }
+      }
+    }
+
+    // the waves' sums meet
+    l = quad_sum(l);
+    if (g == 0) {
+      s.wm[w][c] = m;
+      s.wl[w][c] = l;
+    }
+    __syncthreads();
+    float M = fmaxf(fmaxf(s.wm[0][c], s.wm[1][c]), fmaxf(s.wm[2][c], s.wm[3][c]));
+    const float Ms = M == -__builtin_inff() ? 0.f : M;
+    const float f = exp2_fast(m - Ms - S::P0);
+    bool odd = false;
+    if (w == 0 && g == 0) {
+      float L = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; i++) L += s.wl[i][c] * exp2_fast(s.wm[i][c] - Ms - S::P0);
+      s.m[c] = M;
+      s.l[c] = L;
+      odd = c < it.heads && !finite(L);
+    }
+    for (int r4 = 0; r4 < 4; r4++) {
+      if (w == r4) {
+#pragma unroll
+        for (int j = 0; j < S::NJ; j++)
+#pragma unroll
+          for (int r = 0; r < 4; r++)
+#pragma unroll
+            for (int e = 0; e < S::VL; e += 4) {
+              floatx4* const d = (floatx4*)&s.o[c * S::OS + j * 16 * S::VL + S::VL * (4 * g + r) + e];
+              floatx4 v = {o[j][e][r] * f, o[j][e + 1][r] * f, o[j][e + 2][r] * f, o[j][e + 3][r] * f};
+              if (r4) v += *d;
+              *d = v;
+            }
+      }
+      __syncthreads();
+    }
+    for (int h = w; h < it.heads; h += 4)
+      for (int d = lane; d < hd; d += 64) odd |= !finite(s.o[h * S::OS + d]);
+    if (__syncthreads_or(odd))
+      paged_walk<T, D>(a, it, lo + (int64_t)tile0 * S::TK, min(hi, lo + (int64_t)tile1 * S::TK), s);
+
+    float* const y = a.y + (int64_t)seq * row_out + (int64_t)it.head0 * a.hd;
+    // with the sink: its weight beside the sum's, both against the larger maximum
+    auto finish = [&](int h, float m2, float l2, float& f2) {
+      f2 = 1.f;
+      if (a.sinks) {
+        const float sk = a.sinks[it.head0 + h] * LOG2E;
+        if (sk > m2) {
+          f2 = exp2_fast(m2 - sk);
+          l2 = l2 * f2 + 1.f;
+        } else {
+          l2 += exp2_fast(sk - m2);
+        }
+      }
+      f2 = l2 != 0.f ? f2 / l2 : 0.f;
+    };
+    if (tile0 == 0 && tile1 == n) {
+      for (int h = w; h < it.heads; h += 4) {
+        float f2;
+        finish(h, s.m[h], s.l[h], f2);
+        for (int d = lane; d < hd; d += 64) y[h * a.hd + d] = f2 == 0.f ? 0.f : s.o[h * S::OS + d] * f2;
+      }
+      __syncthreads();
+    } else {
+      const int ps = 16 * a.hd + 32;  // floats of a piece
+      float* const pc = a.part + (int64_t)(2 * b + (tile0 ? 0 : 1)) * ps;
+      for (int h = w; h < it.heads; h += 4)
+        for (int d = lane; d < hd; d += 64) store_agent(pc + h * a.hd + d, s.o[h * S::OS + d]);
+      if (t < 16) {
+        store_agent(pc + 16 * a.hd + t, s.m[t]);
+        store_agent(pc + 16 * a.hd + 16 + t, s.l[t]);
+      }
+      // the blocks of the item's first and last tile
+      auto block_of = [&](uint32_t i) {
+        uint32_t k = (uint32_t)((double)i * B / all);
+        while (k > 0 && first(k) > i) k--;
+        while (first(k + 1) <= i) k++;
+        return k;
+      };
+      const uint32_t u0 = before + item * n, b0 = block_of(u0), np = block_of(u0 + n - 1) - b0 + 1;
+      if (last_block(a.done + 32 * b0, (int)np)) {
+        auto piece = [&](uint32_t i) { return a.part + (int64_t)(2 * (b0 + i) + (i == 0)) * ps; };
+        {
+          const int h = t >> 4;
+          float M2 = -__builtin_inff(), L = 0.f;
+          for (uint32_t i = t & 15; i < np; i += 16) M2 = fmaxf(M2, load_agent(piece(i) + 16 * a.hd + h));
+          M2 = fmaxf(M2, xpart<1>(M2));
+          M2 = fmaxf(M2, xpart<2>(M2));
+          M2 = fmaxf(M2, xpart<4>(M2));
+          M2 = fmaxf(M2, xpart<8>(M2));
+          const float s2 = M2 == -__builtin_inff() ? 0.f : M2;
+          for (uint32_t i = t & 15; i < np; i += 16)
+            L += exp2_fast(load_agent(piece(i) + 16 * a.hd + h) - s2) * load_agent(piece(i) + 16 * a.hd + 16 + h);
+          L = wave_sum(L, 16);
+          if ((t & 15) == 0) {
+            s.m[h] = M2;
+            s.l[h] = L;
+          }
+        }
+        __syncthreads();
+        for (int h = w; h < it.heads; h += 4) {
+          const float m2 = s.m[h], s2 = m2 == -__builtin_inff() ? 0.f : m2;
+          float f2;
+          finish(h, m2, s.l[h], f2);
+          for (int d = lane; d < hd; d += 64) {
+            float v = 0.f;
+#pragma unroll 4
+            for (uint32_t i = 0; i < np; i++) {
+              const float wt = exp2_fast(load_agent(piece(i) + 16 * a.hd + h) - s2);
+              const float x = load_agent(piece(i) + h * a.hd + d);
+              v += wt == 0.f ? 0.f : wt * x;
+            }
+            y[h * a.hd + d] = f2 == 0.f ? 0.f : v * f2;
+          }
+        }
+        if (t == 0) __hip_atomic_store(a.done + 32 * b0, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __syncthreads();
+      }
+    }
+    u += tile1 - tile0;
+    if (u >= end) return;
+    if (tile1 == n && item + 1 == per) {  // the next sequence with a key
+      before = u;
+      do n = tiles_of(++seq, lo, hi);
+      while (n == 0);
+    }
+  }
+}
+
+#define PAGED_ATTENTION(NAME, T, D)                                                                     \
+  extern "C" __global__ __launch_bounds__(256) void paged_attention_##NAME##_##D(PagedAttnArgs a)       \
+  {                                                                                                     \
+    paged_attention_t<T, D, true>(a);                                                                   \
+  }                                                                                                     \
+  extern "C" __global__ __launch_bounds__(256) void paged_attention_##NAME##_##D##_part(PagedAttnArgs a) \
+  {                                                                                                     \
+    paged_attention_t<T, D, false>(a);                                                                  \
+  }
+PAGED_ATTENTION(f32, 0, 64)
+PAGED_ATTENTION(f32, 0, 128)
+PAGED_ATTENTION(f32, 0, 256)
+PAGED_ATTENTION(f32, 0, 512)
+PAGED_ATTENTION(f16, 1, 64)
+PAGED_ATTENTION(f16, 1, 128)
+PAGED_ATTENTION(f16, 1, 256)
+PAGED_ATTENTION(f16, 1, 512)
+PAGED_ATTENTION(bf16, 2, 64)
+PAGED_ATTENTION(bf16, 2, 128)
+PAGED_ATTENTION(bf16, 2, 256)
+PAGED_ATTENTION(bf16, 2, 512)
