@@ -105,6 +105,7 @@ struct ihip_ctx {
   uint64_t scratch_attn = 0, scratch_attn_bytes = 0;
   uint64_t paged_plan = 0;  // the step plan between ihip_enqueue_paged_slots' two launches
   uint64_t paged_part = 0;  // paged_attention's shared pieces and counters (zero between launches)
+  uint64_t logprobs_part = 0;  // the same of ihip_enqueue_logprobs
   uint64_t scratch_planes = 0, scratch_planes_bytes = 0;  // e4m3 activation planes (gemm_mxfp4_f8)
   // the device address of static_scratch.hip's array on this device
   // (ihip_enqueue_linear_at_static), read once at ihip_create
@@ -157,6 +158,10 @@ constexpr int64_t PAGED_ROWS_HERE = 4096;
 // 128 bytes a block behind them
 constexpr int64_t PAGED_BLOCKS = 1024;
 constexpr uint64_t PAGED_PART_BYTES = 17u << 20;
+// logprobs: blocks up to which rows are split into parts, the parts' results (3
+// doubles and IHIP_LOGPROBS_TOP alternatives each), and a counter of 32 bytes a row
+constexpr int64_t LOGPROBS_BLOCKS = 1024;
+constexpr uint64_t LOGPROBS_PART_BYTES = LOGPROBS_BLOCKS * (3 + IHIP_LOGPROBS_TOP) * 8;
 constexpr uint64_t PAGED_PLAN_BYTES = (5 * IHIP_PAGED_SEQS + 4) * 4;
 
 struct LinearCall {

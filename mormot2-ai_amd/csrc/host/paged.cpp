@@ -230,6 +230,10 @@ int ihip_enqueue_logprobs(ihip_ctx* c, uint64_t logits, int64_t rows, int64_t vo
     return refuse(who, "arrays aligned to 4 bytes");
   if (!c) return no_context(who);
   OnDevice on(c);
+  // the rows' parts: blocks for the whole chip, of no less than 4 tiles of 1024 logits (one a wave)
+  int64_t parts = 1;
+  if (rows < LOGPROBS_BLOCKS)
+    parts = std::max<int64_t>(1, std::min<int64_t>((vocab + 4095) / 4096, LOGPROBS_BLOCKS / rows));
   struct {
     const float* x;
     int64_t stride;
@@ -237,10 +241,28 @@ int ihip_enqueue_logprobs(ihip_ctx* c, uint64_t logits, int64_t rows, int64_t vo
     float *logprobs, *entropy;
     int* top_ids;
     float* top_logprobs;
-    int32_t rows, vocab, k, pad;
+    double* part;
+    int* done;
+    int32_t rows, vocab, k, parts;
   } a = {(const float*)logits, stride, (const int*)ids, (float*)logprobs, (float*)entropy,
-         (int*)top_ids, (float*)top_logprobs, (int32_t)rows, (int32_t)vocab, (int32_t)k, 0};
-  return launch(c, "logprobs", dim3((unsigned)rows), dim3(256), &a);
+         (int*)top_ids, (float*)top_logprobs, (double*)c->logprobs_part,
+         (int*)(c->logprobs_part + LOGPROBS_PART_BYTES), (int32_t)rows, (int32_t)vocab, (int32_t)k,
+         (int32_t)parts};
+  // rows in a grid's y, 65535 a launch
+  for (int64_t r = 0; r < rows; r += 65535) {
+    const int64_t n = std::min<int64_t>(rows - r, 65535);
+    auto b = a;
+    b.x += r * stride;
+    if (ids) b.ids += r;
+    if (logprobs) b.logprobs += r;
+    if (entropy) b.entropy += r;
+    if (k) {
+      b.top_ids += r * k;
+      b.top_logprobs += r * k;
+    }
+    if (int rc = launch(c, "logprobs", dim3((unsigned)parts, (unsigned)n), dim3(256), &b)) return rc;
+  }
+  return 0;
 }
 
 }  // extern "C"

@@ -4,6 +4,7 @@
 // copies, events and stream capture into graphs.
 #include <cstdio>
 #include <cstring>
+#include <tuple>
 
 #include "internal.h"
 
@@ -221,16 +222,19 @@ int ihip_create(int device, ihip_ctx** out)
     return fail(IHIP_E_NOMEM, "hipMalloc");
   }
   c->paged_plan = (uint64_t)plan;
-  // fixed, so that a captured call holds an address that stays
-  void* part = nullptr;
-  if (hipMalloc(&part, PAGED_PART_BYTES + PAGED_BLOCKS * 128) != hipSuccess) {
-    ihip_destroy(c);
-    return fail(IHIP_E_NOMEM, "hipMalloc");
-  }
-  c->paged_part = (uint64_t)part;
-  if ((e = hipMemsetAsync((char*)part + PAGED_PART_BYTES, 0, PAGED_BLOCKS * 128, c->stream)) != hipSuccess) {
-    ihip_destroy(c);
-    return hip_fail(e, "hipMemsetAsync");
+  // fixed, so that a captured call holds an address that stays; the counters behind zeroed
+  for (auto [to, bytes, counters] : {std::tuple(&c->paged_part, PAGED_PART_BYTES, PAGED_BLOCKS * 128),
+                                     std::tuple(&c->logprobs_part, LOGPROBS_PART_BYTES, LOGPROBS_BLOCKS * 32)}) {
+    void* q = nullptr;
+    if (hipMalloc(&q, bytes + counters) != hipSuccess) {
+      ihip_destroy(c);
+      return fail(IHIP_E_NOMEM, "hipMalloc");
+    }
+    *to = (uint64_t)q;
+    if ((e = hipMemsetAsync((char*)q + bytes, 0, counters, c->stream)) != hipSuccess) {
+      ihip_destroy(c);
+      return hip_fail(e, "hipMemsetAsync");
+    }
   }
   if (int rc = static_scratch_init(c)) {
     ihip_destroy(c);
@@ -253,7 +257,8 @@ void ihip_destroy(ihip_ctx* c)
   for (auto& w : c->weights) (void)hipFree((void*)w.dev);
   for (auto a : c->allocations) (void)hipFree((void*)a);
   for (uint64_t b : {c->scratch_x, c->scratch_y, c->scratch_q, c->scratch_bad, c->scratch_attn,
-                     c->scratch_argmax, c->scratch_split, c->scratch_planes, c->paged_plan, c->paged_part})
+                     c->scratch_argmax, c->scratch_split, c->scratch_planes, c->paged_plan, c->paged_part,
+                     c->logprobs_part})
     if (b) (void)hipFree((void*)b);
   for (auto ev : c->events)
     if (ev) (void)hipEventDestroy(ev);
