@@ -45,7 +45,9 @@ struct TopList {
   __device__ __forceinline__ void insert(uint64_t c)  // c the same in every lane
   {
     const int at = __popcll(__ballot(v > c));  // descending: the first `at` stay
-    const uint32_t lo = __shfl_up((uint32_t)v, 1, 64), hi = __shfl_up((uint32_t)(v >> 32), 1, 64);
+    // the lane before: DPP shifts over the whole wave
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0u, (uint32_t)v, 0x138, 0xF, 0xF, false);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0u, (uint32_t)(v >> 32), 0x138, 0xF, 0xF, false);
     const int lane = threadIdx.x & 63;
     if (lane == at) v = c;
     else if (lane > at) v = (uint64_t)hi << 32 | lo;

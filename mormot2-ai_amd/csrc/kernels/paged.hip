@@ -494,6 +494,12 @@ __device__ __forceinline__ void split2(float x, float y, uint32_t* part)
   }
 }
 
+__device__ __forceinline__ uint64_t lane_value(uint64_t v, int lane)
+{
+  return (uint64_t)__builtin_amdgcn_readlane((uint32_t)(v >> 32), lane) << 32 |
+         (uint32_t)__builtin_amdgcn_readlane((uint32_t)v, lane);
+}
+
 // the maximum and the sum over the four lanes of a head (lanes c, c + 16, c + 32,
 // c + 48)
 __device__ __forceinline__ float quad_max(float v)
@@ -524,6 +530,7 @@ struct AttnShape {
   static constexpr int NT = KS / 16;                   // score tiles of a step
   static constexpr int QL = 16 / ES;                   // values of a key load
   static constexpr int NQ = D / (4 * QL);              // key loads of a lane and key
+  static constexpr int KH = D == 512 ? 2 : 1;          // chunks that a step's keys are loaded in (registers)
   static constexpr int NP = T == 0 ? 1 : T == 1 ? 2 : 3;  // parts of a single value
   static constexpr int VL = T != 0 && D > 64 ? 8 : 4;  // values of a value load
   static constexpr int NJ = D / (16 * VL);             // value loads of a lane and key
@@ -693,7 +700,8 @@ __device__ __forceinline__ void paged_attention_t(const PagedAttnArgs& a)
     return (uint32_t)((hi - lo + S::TK - 1) / S::TK);
   };
   // all tiles (each wave for itself); rows without a key are zeros
-  uint32_t all = 0;
+  uint32_t all = 0, n0 = 0;
+  int64_t lo0 = 0, hi0 = 0;  // of the first 64 sequences, a lane each
   for (int s0 = 0; s0 < a.seqs; s0 += 64) {
     const int seq = s0 + lane;
     uint32_t n = 0;
@@ -701,6 +709,7 @@ __device__ __forceinline__ void paged_attention_t(const PagedAttnArgs& a)
     if (seq < a.seqs) {
       int64_t lo, hi;
       n = tiles_of(seq, lo, hi);
+      if (s0 == 0) n0 = n, lo0 = lo, hi0 = hi;
       zero = n == 0 && a.lengths[seq] >= 0 && (uint32_t)seq % grid == b;
     }
     all += n * per;
@@ -722,9 +731,10 @@ __device__ __forceinline__ void paged_attention_t(const PagedAttnArgs& a)
   uint32_t before = 0, n = 0;  // tiles before the sequence, tiles of a KV head's item
   int64_t lo = 0, hi = 0;
   for (int s0 = 0;; s0 += 64) {
-    uint32_t m = 0;
-    int64_t l2, h2;
-    if (s0 + lane < a.seqs) m = tiles_of(s0 + lane, l2, h2) * per;
+    uint32_t m = s0 == 0 ? n0 : 0;
+    if (s0 > 0 && s0 + lane < a.seqs) m = tiles_of(s0 + lane, lo0, hi0);
+    const uint32_t items = m;
+    m *= per;
     uint32_t upto = m;
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) {
@@ -735,12 +745,14 @@ __device__ __forceinline__ void paged_attention_t(const PagedAttnArgs& a)
     if (there) {
       const int f = __builtin_ctzll(there);
       seq = __builtin_amdgcn_readfirstlane(s0 + f);
-      before = __builtin_amdgcn_readfirstlane(before + __shfl(upto - m, f, 64));
+      before += __builtin_amdgcn_readlane(upto - m, f);
+      n = __builtin_amdgcn_readlane(items, f);
+      lo = (int64_t)lane_value((uint64_t)lo0, f);
+      hi = (int64_t)lane_value((uint64_t)hi0, f);
       break;
     }
-    before = __builtin_amdgcn_readfirstlane(before + __shfl(upto, 63, 64));
+    before += __builtin_amdgcn_readlane(upto, 63);
   }
-  n = tiles_of(seq, lo, hi);
 
   for (;;) {
     const uint32_t item = (u - before) / n, tile0 = (u - before) - item * n;
@@ -753,9 +765,6 @@ __device__ __forceinline__ void paged_attention_t(const PagedAttnArgs& a)
     it.head0 = it.kv * a.group + 16 * it.tile;
     it.lo = lo;
     it.hi = hi;
-    stage_query<T, D>(a, it, s);
-
-    const float sscale = T == 1 ? s.qs[c] : 1.f;
     const char* const kb = a.kc + (int64_t)it.kv * a.head_stride * S::ES;
     const char* const vb = a.vc + (int64_t)it.kv * a.head_stride * S::ES;
     const int* const table = a.table + (int64_t)seq * a.max_pages;
@@ -775,14 +784,21 @@ __device__ __forceinline__ void paged_attention_t(const PagedAttnArgs& a)
       __builtin_amdgcn_wave_barrier();
       return (uint32_t)__ballot(at >= 0) & (uint32_t)((1ull << S::KS) - 1);
     };
-    uintx4 kr[S::NT][S::NQ];
-    auto load_keys = [&](uint32_t tile) {
+    uint32_t tile = tile0;
+    const int page0 = entry(tile);
+    int page = entry(tile + 1);
+    stage_query<T, D>(a, it, s);
+    const float sscale = T == 1 ? s.qs[c] : 1.f;
+
+    constexpr int KC = S::NQ / S::KH;
+    uintx4 kr[S::NT][KC];
+    auto load_keys = [&](uint32_t tile, int chunk) {
 #pragma unroll
       for (int i = 0; i < S::NT; i++) {
         const char* const p = kb + s.off[w][tile & 1][16 * i + c];
 #pragma unroll
-        for (int j = 0; j < S::NQ; j++) {
-          const int d0 = j * 4 * S::QL + g * S::QL;
+        for (int j = 0; j < KC; j++) {
+          const int d0 = (chunk * KC + j) * 4 * S::QL + g * S::QL;
           const bool in = FULL || d0 < hd;
           kr[i][j] = *(const uintx4*)(p + (in ? d0 : 0) * S::ES);
           if (!in) kr[i][j] = uintx4{0, 0, 0, 0};
@@ -796,7 +812,6 @@ __device__ __forceinline__ void paged_attention_t(const PagedAttnArgs& a)
 #pragma unroll
       for (int j = 0; j < S::VL; j++) o[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
     float m = -__builtin_inff(), l = 0.f;
-    uint32_t tile = tile0;
     uint32_t steps = 0;  // of this wave: up to the last tile with a key of its own
     if (wlo + (int64_t)tile0 * S::TK < hi) {
       const uint32_t mine = (uint32_t)((hi - wlo + S::TK - 1) / S::TK);
@@ -805,9 +820,8 @@ __device__ __forceinline__ void paged_attention_t(const PagedAttnArgs& a)
     // The loop has no branch between a product and what reads it, so keys are
     // located and loaded one step past the last too: entry() has no page there and
     // the loads read the pool's first row.
-    uint32_t there = locate(tile, entry(tile));
-    int page = entry(tile + 1);
-    if (steps) load_keys(tile);
+    uint32_t there = locate(tile, page0);
+    if (steps) load_keys(tile, 0);
     for (uint32_t i = 0; i < steps; i++, tile++) {
       // the step's values, on their way while its scores are formed
       constexpr int NV = 4 * S::NT;  // keys of a lane: 16 q + 4 g + r
@@ -834,23 +848,27 @@ __device__ __forceinline__ void paged_attention_t(const PagedAttnArgs& a)
 #pragma unroll
       for (int k = 0; k < S::NT; k++) x[k] = floatx4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int j = 0; j < S::NQ; j++) {
+      for (int h = 0; h < S::KH; h++) {
+        if (h) load_keys(tile, h);
 #pragma unroll
-        for (int n2 = 0; n2 < S::NP; n2++) {
-          const uintx4 q = s.q[(n2 * S::NQ + j) * 64 + lane];
+        for (int j = 0; j < KC; j++) {
 #pragma unroll
-          for (int k = 0; k < S::NT; k++) {
-            if constexpr (T == 0) {
+          for (int n2 = 0; n2 < S::NP; n2++) {
+            const uintx4 q = s.q[(n2 * S::NQ + h * KC + j) * 64 + lane];
 #pragma unroll
-              for (int e = 0; e < 4; e++)
-                x[k] = __builtin_amdgcn_mfma_f32_16x16x4f32(bits_float(kr[k][j][e]), bits_float(q[e]), x[k], 0, 0, 0);
-            } else {
-              x[k] = mfma16<T>(kr[k][j], q, x[k]);
+            for (int k = 0; k < S::NT; k++) {
+              if constexpr (T == 0) {
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                  x[k] = __builtin_amdgcn_mfma_f32_16x16x4f32(bits_float(kr[k][j][e]), bits_float(q[e]), x[k], 0, 0, 0);
+              } else {
+                x[k] = mfma16<T>(kr[k][j], q, x[k]);
+              }
             }
           }
         }
       }
-      load_keys(tile + 1);
+      load_keys(tile + 1, 0);
       // masked keys: no weight, and values of zero (0 times NaN is NaN)
       float top = -__builtin_inff();
       if (now == (uint32_t)((1ull << S::KS) - 1)) {
@@ -995,44 +1013,80 @@ __device__ __forceinline__ void paged_attention_t(const PagedAttnArgs& a)
         return k;
       };
       const uint32_t u0 = before + item * n, b0 = block_of(u0), np = block_of(u0 + n - 1) - b0 + 1;
-      if (last_block(a.done + 32 * b0, (int)np)) {
-        auto piece = [&](uint32_t i) { return a.part + (int64_t)(2 * (b0 + i) + (i == 0)) * ps; };
+      auto piece = [&](uint32_t i) { return a.part + (int64_t)(2 * (b0 + i) + (i == 0)) * ps; };
+      // pieces i0, i0 + step, .. (cnt of them, at most 64) joined in that order: into
+      // the output, or into the first of them
+      auto join = [&](uint32_t i0, uint32_t step, uint32_t cnt, bool out) {
+        float* const wt = s.o;  // [64][16]: a piece's weight for each head
         {
           const int h = t >> 4;
-          float M2 = -__builtin_inff(), L = 0.f;
-          for (uint32_t i = t & 15; i < np; i += 16) M2 = fmaxf(M2, load_agent(piece(i) + 16 * a.hd + h));
+          float pm[4], pl[4], M2 = -__builtin_inff(), L = 0.f;
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            const uint32_t j = (t & 15) + 16 * i;
+            const float* const e = piece(i0 + step * min(j, cnt - 1)) + 16 * a.hd + h;
+            pm[i] = j < cnt ? load_agent(e) : -__builtin_inff();
+            pl[i] = j < cnt ? load_agent(e + 16) : 0.f;
+            M2 = fmaxf(M2, pm[i]);
+          }
           M2 = fmaxf(M2, xpart<1>(M2));
           M2 = fmaxf(M2, xpart<2>(M2));
           M2 = fmaxf(M2, xpart<4>(M2));
           M2 = fmaxf(M2, xpart<8>(M2));
           const float s2 = M2 == -__builtin_inff() ? 0.f : M2;
-          for (uint32_t i = t & 15; i < np; i += 16)
-            L += exp2_fast(load_agent(piece(i) + 16 * a.hd + h) - s2) * load_agent(piece(i) + 16 * a.hd + 16 + h);
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            const float f2 = exp2_fast(pm[i] - s2);
+            L += f2 * pl[i];
+            wt[((t & 15) + 16 * i) * 16 + h] = f2;
+          }
           L = wave_sum(L, 16);
+          __syncthreads();
           if ((t & 15) == 0) {
             s.m[h] = M2;
             s.l[h] = L;
-          }
-        }
-        __syncthreads();
-        for (int h = w; h < it.heads; h += 4) {
-          const float m2 = s.m[h], s2 = m2 == -__builtin_inff() ? 0.f : m2;
-          float f2;
-          finish(h, m2, s.l[h], f2);
-          for (int d = lane; d < hd; d += 64) {
-            float v = 0.f;
-#pragma unroll 4
-            for (uint32_t i = 0; i < np; i++) {
-              const float wt = exp2_fast(load_agent(piece(i) + 16 * a.hd + h) - s2);
-              const float x = load_agent(piece(i) + h * a.hd + d);
-              v += wt == 0.f ? 0.f : wt * x;
+            if (!out) {
+              store_agent(piece(i0) + 16 * a.hd + h, M2);
+              store_agent(piece(i0) + 16 * a.hd + 16 + h, L);
             }
-            y[h * a.hd + d] = f2 == 0.f ? 0.f : v * f2;
           }
         }
-        if (t == 0) __hip_atomic_store(a.done + 32 * b0, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         __syncthreads();
+        for (int i = 2 * t; i < it.heads * a.hd; i += 512) {
+          const int h = i / a.hd;
+          float v0 = 0.f, v1 = 0.f;
+#pragma unroll 8
+          for (uint32_t j = 0; j < cnt; j++) {
+            const uint64_t x = __builtin_bit_cast(uint64_t, load_agent((const double*)(piece(i0 + step * j) + i)));
+            const float f2 = wt[j * 16 + h];
+            // (a part of no weight may hold an infinity)
+            v0 = __builtin_fmaf(f2, f2 != 0.f ? bits_float((uint32_t)x) : 0.f, v0);
+            v1 = __builtin_fmaf(f2, f2 != 0.f ? bits_float((uint32_t)(x >> 32)) : 0.f, v1);
+          }
+          if (out) {
+            float f2;
+            finish(h, s.m[h], s.l[h], f2);
+            y[i] = f2 == 0.f ? 0.f : v0 * f2;
+            y[i + 1] = f2 == 0.f ? 0.f : v1 * f2;
+          } else {
+            store_agent(piece(i0) + i, v0);
+            store_agent(piece(i0) + i + 1, v1);
+          }
+        }
+      };
+      // 16 pieces are joined by the last of their blocks, then those by the last of all
+      const uint32_t mine = b - b0, i0 = mine & ~15u, cnt = min(16u, np - i0);
+      int* const group = a.done + 32 * (b0 + i0) + (i0 == 0);
+      if (last_block(group, (int)cnt)) {
+        const uint32_t groups = (np + 15) / 16;
+        join(i0, 1, cnt, groups == 1);
+        if (t == 0) __hip_atomic_store(group, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (groups > 1 && last_block(a.done + 32 * b0 + 2, (int)groups)) {
+          join(0, 16, groups, true);
+          if (t == 0) __hip_atomic_store(a.done + 32 * b0 + 2, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
       }
+      __syncthreads();
     }
     u += tile1 - tile0;
     if (u >= end) return;
