@@ -16,6 +16,7 @@ struct LogprobArgs {
   int32_t rows, vocab, k, parts;
 };
 
+typedef uint32_t uintx4 __attribute__((ext_vector_type(4)));
 typedef float floatx4u __attribute__((ext_vector_type(4), aligned(4)));
 
 // a logit's place in the order of the alternatives: larger values first (both
@@ -38,44 +39,95 @@ __device__ __forceinline__ uint64_t lane_value(uint64_t v, int lane)
          (uint32_t)__builtin_amdgcn_readlane((uint32_t)v, lane);
 }
 
-// the alternatives of a wave: lane i holds the i-th best so far as (order, ~id),
-// 0 where there is none yet, so that a larger number is a better alternative
+// The alternatives of a wave: lane i holds the i-th best so far as (order, ~id), 0
+// where there is none yet, so that a larger number is a better alternative; a
+// tile's candidates meet in LDS first. The code is kept small: a block of one row
+// runs it once, from a cold instruction cache (sorting networks written out took
+// 18 us for one row of 151936 logits where these loops take 11).
 struct TopList {
   uint64_t v;
-  __device__ __forceinline__ void insert(uint64_t c)  // c the same in every lane
+  uint64_t* buf;   // [64 + 256]
+  uint64_t* list;  // [64]
+  int n;           // waiting in buf (the same in every lane)
+
+  // between a lane's LDS write and another's read: no instruction, but no
+  // reordering or forwarding past it
+  __device__ __forceinline__ void lanes_meet()
   {
-    const int at = __popcll(__ballot(v > c));  // descending: the first `at` stay
-    // the lane before: DPP shifts over the whole wave
-    const uint32_t lo = __builtin_amdgcn_update_dpp(0u, (uint32_t)v, 0x138, 0xF, 0xF, false);
-    const uint32_t hi = __builtin_amdgcn_update_dpp(0u, (uint32_t)(v >> 32), 0x138, 0xF, 0xF, false);
-    const int lane = threadIdx.x & 63;
-    if (lane == at) v = c;
-    else if (lane > at) v = (uint64_t)hi << 32 | lo;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
   }
-  // every lane's c (0: none) that is better than the list's k-th
-  __device__ __forceinline__ void insert_lanes(uint64_t c, int k)
+  // the lanes' numbers c where `in` (b: those lanes)
+  __device__ __forceinline__ void add(uint64_t b, bool in, uint64_t c)
   {
-    for (;;) {
-      const uint64_t b = __ballot(c > lane_value(v, k - 1));
-      if (!b) return;
-      const int l = __builtin_ctzll(b);
-      insert(lane_value(c, l));
-      if ((int)(threadIdx.x & 63) == l) c = 0;
+    if (in) buf[n + __builtin_amdgcn_mbcnt_hi((uint32_t)(b >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)b, 0u))] = c;
+    n += __popcll(b);
+  }
+  // the waiting ones into the list, 64 at a time: few one by one, more by counting
+  // for each, and for each of the list, how many are better
+  __device__ __forceinline__ void flush(int k)
+  {
+    const int lane = threadIdx.x & 63;
+    lanes_meet();
+#pragma unroll 1
+    for (int i = 0; i < n; i += 64) {
+      const int m = min(n - i, 64);
+      uint64_t c = lane < m ? buf[i + lane] : 0;
+      uint64_t b = __ballot(c > lane_value(v, k - 1));
+      if (__popcll(b) > 12) {
+        int cr = 0, vr = lane;
+        list[lane] = v;
+        lanes_meet();
+#pragma unroll 4
+        for (int j = 0; j < m; j++) {
+          const uint64_t x = buf[i + j];
+          cr += x > c;
+          vr += x > v;
+        }
+        if (lane_value(v, 0))
+#pragma unroll 4
+          for (int j = 0; j < k; j++) cr += list[j] > c;
+        lanes_meet();
+        list[lane] = 0;
+        lanes_meet();
+        if (v && vr < k) list[vr] = v;
+        if (c && cr < k) list[cr] = c;
+        lanes_meet();
+        v = list[lane];
+        continue;
+      }
+      while (b) {
+        const int l = __builtin_ctzll(b);
+        const uint64_t best = lane_value(c, l);
+        // descending: the first `at` stay, the others move by a lane (DPP over the wave)
+        const int at = __popcll(__ballot(v > best));
+        const uint32_t lo = __builtin_amdgcn_update_dpp(0u, (uint32_t)v, 0x138, 0xF, 0xF, false);
+        const uint32_t hi = __builtin_amdgcn_update_dpp(0u, (uint32_t)(v >> 32), 0x138, 0xF, 0xF, false);
+        if (lane == at) v = best;
+        else if (lane > at) v = (uint64_t)hi << 32 | lo;
+        if (lane == l) c = 0;
+        b = __ballot(c > lane_value(v, k - 1));
+      }
     }
+    lanes_meet();
+    n = 0;
   }
 };
 
-// the k-th largest of the lanes' values, at least: the largest t with k lanes >= t
+constexpr uint32_t ORDER_LEAST = 0x007fffffu;  // of -infinity
+
+// a bound that k lanes reach: the largest number of 20 high bits that k lanes'
+// values are no smaller than (a 2^-11 below the k-th largest at most)
 __device__ __forceinline__ uint32_t kth_of_lanes(uint32_t v, int k)
 {
   uint32_t t = 0;
 #pragma unroll 1
-  for (uint32_t bit = 0x80000000u; bit; bit >>= 1)
+  for (uint32_t bit = 0x80000000u; bit >= 0x1000u; bit >>= 1)
     if (__popcll(__ballot(v >= (t | bit))) >= k) t |= bit;
-  return t;
+  return t ? max(t, ORDER_LEAST) : 0;
 }
 
-// a thread's sums: sum of e^(x - m) and of (x - m) e^(x - m)
+// a thread's sums (m their maximum): sum of e^(x - m) and of (x - m) e^(x - m)
 struct Sums {
   float m;
   double s, w;
@@ -87,11 +139,10 @@ struct Sums {
     s = f * s;
     m = m2;
   }
+  // o's sums against the same maximum or a smaller one
   __device__ __forceinline__ void add(Sums o)
   {
-    const float m2 = fmaxf(m, o.m);
-    rescale(m2);
-    o.rescale(m2);
+    o.rescale(m);
     s += o.s;
     w += o.w;
   }
@@ -105,14 +156,14 @@ constexpr int TILE = 1024;  // a wave's logits of one step, 16 a lane
 // chip; its waves take tiles of 1024 logits in turn, so that a wave sees ids in
 // ascending order. One pass: a lane adds 16 logits in single against its own
 // running maximum (their sums go on in double) and compares their maximum with
-// the wave's k-th best so far; few tiles after the first have a better one, and
-// those are inserted one by one into a list held across the lanes. The first
+// the wave's k-th best so far; few tiles after the first have a better one. The first
 // tile's bound is the k-th largest of the lanes' maxima, found by bits with
 // ballots. HBM bound: 4 bytes a logit.
 extern "C" __global__ __launch_bounds__(256) void logprobs(LogprobArgs a)
 {
   __shared__ Sums sums_s[4];
-  __shared__ uint64_t list_s[4][64];
+  __shared__ alignas(16) uint32_t quarter_s[4], kth_s[4];  // bounds of the waves' lists
+  __shared__ uint64_t list_s[4][64], buf_s[4][64 + 256];
   const int r = blockIdx.y, part = blockIdx.x, t = threadIdx.x, lane = t & 63;
   const int w = __builtin_amdgcn_readfirstlane(t >> 6);
   const float* const x = a.x + (int64_t)r * a.stride;
@@ -121,7 +172,9 @@ extern "C" __global__ __launch_bounds__(256) void logprobs(LogprobArgs a)
   const int t0 = (int)((int64_t)part * tiles / a.parts), t1 = (int)((int64_t)(part + 1) * tiles / a.parts);
 
   Sums sum = {LOWEST, 0.0, 0.0};
-  TopList top = {0};
+  TopList top = {0, buf_s[w], list_s[w], 0};
+  if (t < 4) quarter_s[t] = kth_s[t] = 0;
+  __syncthreads();
   floatx4u v[4], nv[4];
   auto load = [&](int tile, floatx4u* d) {
     const int base = tile * TILE + 4 * lane;
@@ -164,96 +217,122 @@ extern "C" __global__ __launch_bounds__(256) void logprobs(LogprobArgs a)
     sum.s += (double)((s[0] + s[1]) + (s[2] + s[3]));
     sum.w += (double)((wsum[0] + wsum[1]) + (wsum[2] + wsum[3]));
     if (a.k) {
-      const uint64_t kth = lane_value(top.v, a.k - 1);
-      const int base = tile * TILE + 4 * lane;
-      uint32_t least = (uint32_t)(kth >> 32) + 1;  // ids ascend: only what is larger
-      bool look = true;
-      if (kth >> 32) look = __any(m > order_value((uint32_t)(kth >> 32)));
-      else least = (tile + 1) * TILE <= a.vocab ? kth_of_lanes(order_of(m), a.k) : 0;
-      if (look) {
-#pragma unroll
-        for (int j = 0; j < 4; j++)
+      const bool start = tile == t0 + w;
+      uint32_t least;
+      if (start) {
+        // as large as the k-th of the lanes' maxima (equal ones only until there are k)
+        least = (tile + 1) * TILE <= a.vocab ? kth_of_lanes(order_of(m), a.k) : 0;
+      } else {
+        // larger than the wave's own k-th, as ids ascend; no smaller than another
+        // wave's k-th, or than what each wave has a quarter of k of (what the waves
+        // last wrote: an older bound holds too)
+        const uintx4 q = *(const volatile uintx4*)quarter_s, f = *(const volatile uintx4*)kth_s;
+        least = max(max(min(min(q[0], q[1]), min(q[2], q[3])), max(max(f[0], f[1]), max(f[2], f[3]))),
+                    (uint32_t)(lane_value(top.v, a.k - 1) >> 32) + 1);
+      }
+      float bound = order_value(max(least, ORDER_LEAST));  // (NaN above infinity)
+      if (start || __any(m >= bound)) {
+        const int base = tile * TILE + 4 * lane;
+        const uint32_t first = least;
+        int equal = 0;
+#pragma unroll 1
+        for (int j = 0; j < 4; j++) {
 #pragma unroll
           for (int e = 0; e < 4; e++) {
-            const int i = base + 256 * j + e;
-            const uint32_t o = order_of(v[j][e]);
-            const bool in = o >= least && i < a.vocab;
-            if (__any(in)) top.insert_lanes(in ? (uint64_t)o << 32 | (uint32_t)~i : 0, a.k);
+            if (__ballot(v[0][e] >= bound || least == 0)) {
+              const int i = base + 256 * j + e;
+              const uint32_t o = order_of(v[0][e]);
+              const bool in = o >= least && i < a.vocab;
+              if (start) equal += __popcll(__ballot(in && o == first));
+              top.add(__ballot(in), in, (uint64_t)o << 32 | (uint32_t)~i);
+            }
           }
+          if (start && equal >= a.k) {
+            least = first + 1;
+            bound = order_value(max(least, ORDER_LEAST));
+          }
+          if (top.n > 64 || j == 3) top.flush(a.k);
+          v[0] = v[1];
+          v[1] = v[2];
+          v[2] = v[3];
+        }
+        if (lane == 0) {
+          quarter_s[w] = (uint32_t)(lane_value(top.v, (a.k + 3) / 4 - 1) >> 32);
+          kth_s[w] = (uint32_t)(lane_value(top.v, a.k - 1) >> 32);
+        }
       }
     }
   }
 
-  // the lanes' sums, then the waves'; the waves' lists
-  auto lanes_meet = [&](Sums z) {
-    const float m = wave_max(z.m);
-    z.rescale(m);
+  // the lanes' sums and the waves' meet, then, of a row in parts, the parts' in its
+  // last block
+  Sums z = sum;
+#pragma unroll 1
+  for (int parts = a.parts;; parts = 1) {
+    const float wm = wave_max(z.m);
+    z.rescale(wm);
     z.s = wave_sum(z.s, 64);
     z.w = wave_sum(z.w, 64);
-    return z;
-  };
-  auto block_meets = [&](Sums z) {  // sums of the waves (in every lane), lists of the waves
     if (lane == 0) sums_s[w] = z;
     list_s[w][lane] = top.v;
     __syncthreads();
-    z = sums_s[0];
-    for (int i = 1; i < 4; i++) z.add(sums_s[i]);
-    // an alternative's place among all: those before it in its own list, and the
-    // better ones of the others'
-    const uint64_t mine = top.v;
-    int rank = lane;
-    for (int i = 0; i < 4; i++) {
-      if (i == w) continue;
-      int n = 0;
-#pragma unroll
-      for (int step = 32; step; step >>= 1)
-        if (list_s[i][n + step - 1] > mine) n += step;
-      n += n == 63 && list_s[i][63] > mine;
-      rank += n;
+    z = sums_s[lane & 3];
+    z.rescale(fmaxf(fmaxf(sums_s[0].m, sums_s[1].m), fmaxf(sums_s[2].m, sums_s[3].m)));
+    z.s = wave_sum(z.s, 4);
+    z.w = wave_sum(z.w, 4);
+    if (a.k) {
+      // an alternative's place among all: behind its own list's, and the others' better ones
+      const uint64_t mine = top.v;
+      int rank = lane;
+      for (int i = 1; i < 4; i++) {
+        const uint64_t* const o = list_s[(w + i) & 3];
+#pragma unroll 4
+        for (int j = 0; j < a.k; j++) rank += o[j] > mine;
+      }
+      buf_s[0][t < a.k ? t : 64] = 0;
+      __syncthreads();
+      if (lane < a.k && mine && rank < a.k) buf_s[0][rank] = mine;
+      __syncthreads();
+      top.v = lane < a.k ? buf_s[0][lane] : 0;
     }
-    __syncthreads();
-    if (t < 64) list_s[0][t] = 0;
-    __syncthreads();
-    if (mine && rank < a.k) list_s[0][rank] = mine;
-    __syncthreads();
-    return z;
-  };
-  Sums z = block_meets(lanes_meet(sum));
-
-  if (a.parts > 1) {
+    if (parts == 1) break;
     double* const p = a.part + ((int64_t)r * a.parts + part) * (3 + a.k);
-    if (t < a.k) store_agent(p + 3 + t, __builtin_bit_cast(double, list_s[0][t]));
+    if (t < a.k) store_agent(p + 3 + t, __builtin_bit_cast(double, top.v));
     if (t == 0) {
       store_agent(p, (double)z.m);
       store_agent(p + 1, z.s);
       store_agent(p + 2, z.w);
     }
     if (!last_block(a.done + 8 * r, a.parts)) return;
+    if (t == 0) __hip_atomic_store(a.done + 8 * r, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     const double* const q = a.part + (int64_t)r * a.parts * (3 + a.k);
     z = {LOWEST, 0.0, 0.0};
     top.v = 0;
-    uint64_t bound = 0;  // the best of the parts' k-th: no worse one is among the k
-    for (int i = lane; i < a.parts; i += 64) {
+    for (int i = t; i < a.parts; i += 256) {
       const double* const e = q + (int64_t)i * (3 + a.k);
-      if (w == 0) z.add({(float)load_agent(e), load_agent(e + 1), load_agent(e + 2)});
-      if (a.k) {
-        const uint64_t b = __builtin_bit_cast(uint64_t, load_agent(e + 2 + a.k));
-        bound = b > bound ? b : bound;
-      }
+      const Sums o = {(float)load_agent(e), load_agent(e + 1), load_agent(e + 2)};
+      const float m2 = fmaxf(z.m, o.m);
+      z.rescale(m2);
+      z.add(o);
     }
     if (a.k) {
-      bound = wave_max(bound);
+      // a bound that k of them reach: some lanes' parts have their j-th that good
+      const int lanes = min(a.parts, 64), j = (a.k + lanes - 1) / lanes;
+      uint32_t best = 0;
+      for (int i = lane; i < a.parts; i += 64)
+        best = max(best, (uint32_t)(__builtin_bit_cast(uint64_t, load_agent(q + (int64_t)i * (3 + a.k) + 2 + j)) >> 32));
+      const uint64_t bound = (uint64_t)kth_of_lanes(best, (a.k + j - 1) / j) << 32;
       const int all = a.parts * a.k;
+#pragma unroll 4
       for (int i0 = 64 * w; i0 < all; i0 += 256) {
-        const int i = i0 + lane;
-        uint64_t c = 0;
-        if (i < all) c = __builtin_bit_cast(uint64_t, load_agent(q + (int64_t)(i / a.k) * (3 + a.k) + 3 + i % a.k));
-        top.insert_lanes(c >= bound ? c : 0, a.k);
+        const int i = min(i0 + lane, all - 1), of = i / a.k;
+        const uint64_t c = __builtin_bit_cast(uint64_t, load_agent(q + (int64_t)of * (3 + a.k) + 3 + i - of * a.k));
+        const bool in = i0 + lane < all && c >= bound && c;
+        top.add(__ballot(in), in, c);
+        if (top.n > 64) top.flush(a.k);
       }
+      top.flush(a.k);
     }
-    __syncthreads();
-    z = block_meets(lanes_meet(z));
-    if (t == 0) __hip_atomic_store(a.done + 8 * r, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
 
   // s is NaN where a logit is NaN or +infinity, 0 where all are -infinity
@@ -268,7 +347,7 @@ extern "C" __global__ __launch_bounds__(256) void logprobs(LogprobArgs a)
     if (a.entropy) a.entropy[r] = none ? 0.f : (float)(ls - z.w / z.s);
   }
   if (t < a.k) {
-    const uint64_t c = list_s[0][t];
+    const uint64_t c = top.v;
     a.top_ids[(int64_t)r * a.k + t] = c ? (int)~(uint32_t)c : -1;
     a.top_logprobs[(int64_t)r * a.k + t] = c ? lp(order_value((uint32_t)(c >> 32))) : -__builtin_inff();
   }
