@@ -99,8 +99,11 @@ int ihip_enqueue_paged_slots(ihip_ctx* c, uint64_t past, uint64_t count, int64_t
          (int64_t*)ends_out, (int*)offsets, (int*)lengths, (int*)positions, (int*)slots, (int*)failed,
          (int*)c->paged_plan, (int32_t)seqs, (int32_t)max_pages, (int32_t)page_size, (int32_t)pages,
          (int32_t)rows, rows <= PAGED_ROWS_HERE};
-  const size_t shmem = (size_t)seqs * 5 * 4 + 64;
-  int rc = launch(c, "paged_slots", dim3(1), dim3(1024), &a, shmem);
+  const size_t shmem = (size_t)seqs * 5 * 4;
+  // a thread for 4 sequences, and where this block writes the rows one for a row
+  // and a wave beside them for the pages that move
+  const int64_t threads = std::max<int64_t>((seqs + 3) / 4, a.here ? std::min<int64_t>(rows + 64, 1024) : 256);
+  int rc = launch(c, "paged_slots", dim3(1), dim3((unsigned)((threads + 63) / 64 * 64)), &a, shmem);
   if (rc || a.here) return rc;
   return launch(c, "paged_slots_rows", dim3((unsigned)std::min<int64_t>(4 * c->cus, (rows + 1023) / 1024)),
                 dim3(256), &a, shmem);
@@ -180,8 +183,10 @@ int ihip_enqueue_paged_attention(ihip_ctx* c, uint64_t q, int64_t q_stride, cons
   if (q_stride < heads * hd) return refuse(who, "a stride below a row");
   if ((q | y | sinks | lengths | table) % 4) return refuse(who, "arrays aligned to 4 bytes");
   if (std::isnan(scale) || std::isinf(scale)) return refuse(who, "scale");
-  // the kernels take tiles of 128 keys of 16-bit caches, 64 of single ones
-  const int64_t group = heads / kvh, tiles = (group + 15) / 16, tk = cache->dtype == IHIP_F32 ? 64 : 128;
+  // the kernels take tiles of 128 keys of 16-bit caches, 64 of single ones, half as
+  // many of heads beyond 256
+  const int64_t group = heads / kvh, tiles = (group + 15) / 16;
+  const int64_t tk = (cache->dtype == IHIP_F32 ? 64 : 128) / (hd > 256 ? 2 : 1);
   const int64_t keys = window > 0 ? std::min(window, max_pages * cache->page_size) : max_pages * cache->page_size;
   const int64_t units = (keys + tk - 1) / tk * kvh * tiles;
   if (units > INT32_MAX / seqs) return refuse(who, "more than 2^31 tiles of keys", IHIP_E_NOMEM);
@@ -230,10 +235,16 @@ int ihip_enqueue_logprobs(ihip_ctx* c, uint64_t logits, int64_t rows, int64_t vo
     return refuse(who, "arrays aligned to 4 bytes");
   if (!c) return no_context(who);
   OnDevice on(c);
-  // the rows' parts: blocks for the whole chip, of no less than 4 tiles of 1024 logits (one a wave)
+  // The rows' parts: blocks for the whole chip (2048 instead of 1024: 61 rows of
+  // 201088 35.9 us, 26.1), but no part so short that its first tile and its list cost
+  // more than the blocks gain: 4096 logits for a few rows, 8192 from 16 rows (16 of
+  // 151936 in 37 parts 16.9 us, in 18 16.5), 24576 from 256 (512 of 32000 in two parts
+  // 29.5, in one 25.6; 300 of 151936 in one 57.3, in three 47.6)
   int64_t parts = 1;
-  if (rows < LOGPROBS_BLOCKS)
-    parts = std::max<int64_t>(1, std::min<int64_t>((vocab + 4095) / 4096, LOGPROBS_BLOCKS / rows));
+  if (rows < LOGPROBS_BLOCKS) {
+    const int64_t least = rows < 16 ? 4096 : rows < 256 ? 8192 : 24576;
+    parts = std::max<int64_t>(1, std::min<int64_t>(vocab / least, LOGPROBS_BLOCKS / rows));
+  }
   struct {
     const float* x;
     int64_t stride;

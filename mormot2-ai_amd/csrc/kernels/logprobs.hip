@@ -162,7 +162,7 @@ constexpr int TILE = 1024;  // a wave's logits of one step, 16 a lane
 extern "C" __global__ __launch_bounds__(256) void logprobs(LogprobArgs a)
 {
   __shared__ Sums sums_s[4];
-  __shared__ alignas(16) uint32_t quarter_s[4], kth_s[4];  // bounds of the waves' lists
+  __shared__ alignas(16) uint32_t share_s[4], kth_s[4];  // bounds: of a share of k, of k
   __shared__ uint64_t list_s[4][64], buf_s[4][64 + 256];
   const int r = blockIdx.y, part = blockIdx.x, t = threadIdx.x, lane = t & 63;
   const int w = __builtin_amdgcn_readfirstlane(t >> 6);
@@ -171,10 +171,10 @@ extern "C" __global__ __launch_bounds__(256) void logprobs(LogprobArgs a)
   const int tiles = (a.vocab + TILE - 1) / TILE;
   const int t0 = (int)((int64_t)part * tiles / a.parts), t1 = (int)((int64_t)(part + 1) * tiles / a.parts);
 
+  IHIP_STAMP_SCOPE;
+  IHIP_STAMP(0);
   Sums sum = {LOWEST, 0.0, 0.0};
   TopList top = {0, buf_s[w], list_s[w], 0};
-  if (t < 4) quarter_s[t] = kth_s[t] = 0;
-  __syncthreads();
   floatx4u v[4], nv[4];
   auto load = [&](int tile, floatx4u* d) {
     const int base = tile * TILE + 4 * lane;
@@ -192,6 +192,24 @@ extern "C" __global__ __launch_bounds__(256) void logprobs(LogprobArgs a)
     }
   };
   if (t0 + w < t1) load(t0 + w, nv);
+  // a first bound of the block: each of its waves has a share of k as large, among
+  // the lanes' maxima of its first tile
+  const int active = min(4, t1 - t0), share = (a.k + active - 1) / active;
+  if (a.k) {
+    float m = nv[0][0];
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) m = fmaxf(m, nv[j][e]);
+    uint32_t q = 0;
+    if (w < active && (t0 + w + 1) * TILE <= a.vocab) q = kth_of_lanes(order_of(m), share);
+    if (lane == 0) {
+      share_s[w] = w < active ? q : 0xffffffffu;
+      kth_s[w] = 0;
+    }
+    __syncthreads();
+  }
+  IHIP_STAMP(1);
   for (int tile = t0 + w; tile < t1; tile += 4) {
 #pragma unroll
     for (int j = 0; j < 4; j++) v[j] = nv[j];
@@ -201,7 +219,8 @@ extern "C" __global__ __launch_bounds__(256) void logprobs(LogprobArgs a)
     for (int j = 0; j < 4; j++)
 #pragma unroll
       for (int e = 0; e < 4; e++) m = fmaxf(m, v[j][e]);
-    if (m > sum.m) sum.rescale(m);
+    // one maximum for the wave's lanes: it grows in few tiles
+    if (__any(m > sum.m)) sum.rescale(fmaxf(sum.m, wave_max(m)));
     float s[4], wsum[4];
 #pragma unroll
     for (int j = 0; j < 4; j++) {
@@ -219,16 +238,16 @@ extern "C" __global__ __launch_bounds__(256) void logprobs(LogprobArgs a)
     if (a.k) {
       const bool start = tile == t0 + w;
       uint32_t least;
+      const uintx4 q = *(const volatile uintx4*)share_s, f = *(const volatile uintx4*)kth_s;
+      least = min(min(q[0], q[1]), min(q[2], q[3]));
       if (start) {
-        // as large as the k-th of the lanes' maxima (equal ones only until there are k)
-        least = (tile + 1) * TILE <= a.vocab ? kth_of_lanes(order_of(m), a.k) : 0;
+        // equal ones only until there are k; a wave that knows no bound takes its own
+        if (!least && (tile + 1) * TILE <= a.vocab) least = kth_of_lanes(order_of(m), a.k);
       } else {
         // larger than the wave's own k-th, as ids ascend; no smaller than another
-        // wave's k-th, or than what each wave has a quarter of k of (what the waves
-        // last wrote: an older bound holds too)
-        const uintx4 q = *(const volatile uintx4*)quarter_s, f = *(const volatile uintx4*)kth_s;
-        least = max(max(min(min(q[0], q[1]), min(q[2], q[3])), max(max(f[0], f[1]), max(f[2], f[3]))),
-                    (uint32_t)(lane_value(top.v, a.k - 1) >> 32) + 1);
+        // wave's, or than what each wave has its share of (what the waves last wrote: an
+        // older bound holds too)
+        least = max(max(least, max(max(f[0], f[1]), max(f[2], f[3]))), (uint32_t)(lane_value(top.v, a.k - 1) >> 32) + 1);
       }
       float bound = order_value(max(least, ORDER_LEAST));  // (NaN above infinity)
       if (start || __any(m >= bound)) {
@@ -257,7 +276,7 @@ extern "C" __global__ __launch_bounds__(256) void logprobs(LogprobArgs a)
           v[2] = v[3];
         }
         if (lane == 0) {
-          quarter_s[w] = (uint32_t)(lane_value(top.v, (a.k + 3) / 4 - 1) >> 32);
+          share_s[w] = max(q[w], (uint32_t)(lane_value(top.v, share - 1) >> 32));
           kth_s[w] = (uint32_t)(lane_value(top.v, a.k - 1) >> 32);
         }
       }
@@ -266,17 +285,17 @@ extern "C" __global__ __launch_bounds__(256) void logprobs(LogprobArgs a)
 
   // the lanes' sums and the waves' meet, then, of a row in parts, the parts' in its
   // last block
+  IHIP_STAMP(2);
   Sums z = sum;
 #pragma unroll 1
   for (int parts = a.parts;; parts = 1) {
-    const float wm = wave_max(z.m);
-    z.rescale(wm);
     z.s = wave_sum(z.s, 64);
     z.w = wave_sum(z.w, 64);
     if (lane == 0) sums_s[w] = z;
     list_s[w][lane] = top.v;
     __syncthreads();
     z = sums_s[lane & 3];
+    // (a wave without a tile: no sums, the lowest maximum)
     z.rescale(fmaxf(fmaxf(sums_s[0].m, sums_s[1].m), fmaxf(sums_s[2].m, sums_s[3].m)));
     z.s = wave_sum(z.s, 4);
     z.w = wave_sum(z.w, 4);
@@ -295,6 +314,7 @@ extern "C" __global__ __launch_bounds__(256) void logprobs(LogprobArgs a)
       __syncthreads();
       top.v = lane < a.k ? buf_s[0][lane] : 0;
     }
+    IHIP_STAMP(3);
     if (parts == 1) break;
     double* const p = a.part + ((int64_t)r * a.parts + part) * (3 + a.k);
     if (t < a.k) store_agent(p + 3 + t, __builtin_bit_cast(double, top.v));
@@ -305,15 +325,26 @@ extern "C" __global__ __launch_bounds__(256) void logprobs(LogprobArgs a)
     }
     if (!last_block(a.done + 8 * r, a.parts)) return;
     if (t == 0) __hip_atomic_store(a.done + 8 * r, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    IHIP_STAMP(4);
     const double* const q = a.part + (int64_t)r * a.parts * (3 + a.k);
     z = {LOWEST, 0.0, 0.0};
     top.v = 0;
-    for (int i = t; i < a.parts; i += 256) {
-      const double* const e = q + (int64_t)i * (3 + a.k);
-      const Sums o = {(float)load_agent(e), load_agent(e + 1), load_agent(e + 2)};
-      const float m2 = fmaxf(z.m, o.m);
-      z.rescale(m2);
-      z.add(o);
+    uint64_t c[4];  // the wave's first alternatives, on their way meanwhile
+    const int all = a.parts * a.k;
+    auto alternative = [&](int i0) {
+      const int i = min(i0 + lane, all - 1), of = i / a.k;
+      return __builtin_bit_cast(uint64_t, load_agent(q + (int64_t)of * (3 + a.k) + 3 + i - of * a.k));
+    };
+    if (a.k)
+#pragma unroll
+      for (int j = 0; j < 4; j++) c[j] = alternative(64 * w + 256 * j);
+    for (int i0 = 64 * w; i0 < a.parts; i0 += 256) {
+      const double* const e = q + (int64_t)min(i0 + lane, a.parts - 1) * (3 + a.k);
+      const bool in = i0 + lane < a.parts;
+      const float em = (float)load_agent(e);
+      const double es = load_agent(e + 1), ew = load_agent(e + 2);
+      z.rescale(fmaxf(z.m, wave_max(em)));
+      z.add({em, in ? es : 0.0, in ? ew : 0.0});
     }
     if (a.k) {
       // a bound that k of them reach: some lanes' parts have their j-th that good
@@ -322,17 +353,19 @@ extern "C" __global__ __launch_bounds__(256) void logprobs(LogprobArgs a)
       for (int i = lane; i < a.parts; i += 64)
         best = max(best, (uint32_t)(__builtin_bit_cast(uint64_t, load_agent(q + (int64_t)i * (3 + a.k) + 2 + j)) >> 32));
       const uint64_t bound = (uint64_t)kth_of_lanes(best, (a.k + j - 1) / j) << 32;
-      const int all = a.parts * a.k;
-#pragma unroll 4
+#pragma unroll 1
       for (int i0 = 64 * w; i0 < all; i0 += 256) {
-        const int i = min(i0 + lane, all - 1), of = i / a.k;
-        const uint64_t c = __builtin_bit_cast(uint64_t, load_agent(q + (int64_t)of * (3 + a.k) + 3 + i - of * a.k));
-        const bool in = i0 + lane < all && c >= bound && c;
-        top.add(__ballot(in), in, c);
+        const bool in = i0 + lane < all && c[0] >= bound && c[0];
+        top.add(__ballot(in), in, c[0]);
         if (top.n > 64) top.flush(a.k);
+        c[0] = c[1];
+        c[1] = c[2];
+        c[2] = c[3];
+        if (i0 + 1024 < all) c[3] = alternative(i0 + 1024);
       }
       top.flush(a.k);
     }
+    IHIP_STAMP(5);
   }
 
   // s is NaN where a logit is NaN or +infinity, 0 where all are -infinity
@@ -351,4 +384,5 @@ extern "C" __global__ __launch_bounds__(256) void logprobs(LogprobArgs a)
     a.top_ids[(int64_t)r * a.k + t] = c ? (int)~(uint32_t)c : -1;
     a.top_logprobs[(int64_t)r * a.k + t] = c ? lp(order_value((uint32_t)(c >> 32))) : -__builtin_inff();
   }
+  IHIP_STAMP(6);
 }

@@ -20,27 +20,46 @@ struct SlotArgs {
 constexpr int SLOT_THREADS = 1024, SLOT_PER = 4;  // sequences: 4 a thread
 static_assert(SLOT_THREADS * SLOT_PER == 4096, "IHIP_PAGED_SEQS");
 
-// the sums of v over the threads before this one; total: over all of them
-__device__ __forceinline__ int64_t scan_block(int64_t v, int64_t& total)
+// one step of a scan over the wave: v and what lane - CTRL's shift holds (0 beyond
+// the row of 16; broadcasts of a row's last lane: to the rows of `rows`)
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int64_t scan_step(int64_t v)
 {
-  __shared__ int64_t part[SLOT_THREADS / 64];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  int64_t s = v;
-  for (int d = 1; d < 64; d *= 2) {
-    const int64_t o = __shfl_up(s, d, 64);
-    if (lane >= d) s += o;
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0u, (uint32_t)v, CTRL, ROWS, 0xF, false);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0u, (uint32_t)((uint64_t)v >> 32), CTRL, ROWS, 0xF, false);
+  return v + (int64_t)((uint64_t)hi << 32 | lo);
+}
+
+// N values: each one's sum over the threads before this one, and over all of them
+template <int N>
+__device__ __forceinline__ void scan_block(const int64_t (&v)[N], int64_t (&before)[N], int64_t (&all)[N])
+{
+  __shared__ int64_t part[SLOT_THREADS / 64][4];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, waves = blockDim.x >> 6;
+  int64_t s[N];
+#pragma unroll
+  for (int i = 0; i < N; i++) {
+    s[i] = scan_step<0x111, 0xF>(v[i]);     // row_shr 1, 2, 4, 8
+    s[i] = scan_step<0x112, 0xF>(s[i]);
+    s[i] = scan_step<0x114, 0xF>(s[i]);
+    s[i] = scan_step<0x118, 0xF>(s[i]);
+    s[i] = scan_step<0x142, 0xA>(s[i]);     // rows 0 and 2 into 1 and 3
+    s[i] = scan_step<0x143, 0xC>(s[i]);     // rows 0 and 1 into 2 and 3
+    before[i] = s[i] - v[i];
+    all[i] = 0;
   }
   __syncthreads();
-  if (lane == 63) part[w] = s;
+  if (lane == 63)
+#pragma unroll
+    for (int i = 0; i < N; i++) part[w][i] = s[i];
   __syncthreads();
-  int64_t before = 0;
-  total = 0;
 #pragma unroll 1
-  for (int i = 0; i < SLOT_THREADS / 64; i++) {
-    if (i < w) before += part[i];
-    total += part[i];
-  }
-  return before + s - v;
+  for (int k = 0; k < waves; k++)
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      if (k < w) before[i] += part[k][i];
+      all[i] += part[k][i];
+    }
 }
 
 // the plan of the sequences, in LDS: row[s] the first row, move[s] the first
@@ -79,7 +98,7 @@ __device__ __forceinline__ int ring_at(uint32_t base, uint32_t i, uint32_t pages
 __device__ __forceinline__ void slot_rows(const SlotArgs& a, const SlotPlan& p, int i0, int step)
 {
   const uint32_t ps = a.page_size;
-  for (int64_t i = i0; i < p.moves; i += step) {
+  for (int64_t i = step - 1 - i0; i < p.moves; i += step) {  // (other waves than the first rows')
     const int s = slot_find(p.move, a.seqs, (int)i), j = (int)i - p.move[s];
     int* const t = a.table + (int64_t)s * a.max_pages;
     const uint32_t at = (uint32_t)p.rank[s] + (uint32_t)j;
@@ -139,8 +158,10 @@ extern "C" __global__ __launch_bounds__(SLOT_THREADS) void paged_slots(SlotArgs 
     }
     rows += fresh[i];
   }
-  int64_t all_rows, all_back, all_want, want = 0;
-  int64_t row = scan_block(rows, all_rows), put = scan_block(back, all_back);
+  int64_t first2[2], all2[2], first1[1], all1[1], first4[4], all4[4], want = 0;
+  scan_block<2>({rows, back}, first2, all2);
+  int64_t row = first2[0], put = first2[1];
+  const int64_t all_rows = all2[0];
   int need[SLOT_PER];
   {
     int64_t r = row;
@@ -156,7 +177,8 @@ extern "C" __global__ __launch_bounds__(SLOT_THREADS) void paged_slots(SlotArgs 
       want += need[i];
     }
   }
-  int64_t take = scan_block(want, all_want);
+  scan_block<1>({want}, first1, all1);
+  int64_t take = first1[0];
   int64_t moved = 0, taken = 0, lost = 0;
   back = 0;
 #pragma unroll
@@ -185,11 +207,8 @@ extern "C" __global__ __launch_bounds__(SLOT_THREADS) void paged_slots(SlotArgs 
     }
     row += fresh[i];
   }
-  int64_t all_moved, all_taken, all_lost;
-  int64_t move = scan_block(moved, all_moved);
-  scan_block(back, all_back);
-  scan_block(taken, all_taken);
-  scan_block(lost, all_lost);
+  scan_block<4>({moved, back, taken, lost}, first4, all4);
+  int64_t move = first4[0];
 #pragma unroll
   for (int i = 0; i < SLOT_PER; i++) {
     const int s = t * SLOT_PER + i;
@@ -197,7 +216,7 @@ extern "C" __global__ __launch_bounds__(SLOT_THREADS) void paged_slots(SlotArgs 
     move += live[i] == 2 ? have[i] : need[i];
   }
   p.rows = (int)(all_rows < INT32_MAX ? all_rows : INT32_MAX);
-  p.moves = (int)all_moved;
+  p.moves = (int)all4[0];
   __syncthreads();  // the inputs are read, the plan is in LDS
 #pragma unroll
   for (int i = 0; i < SLOT_PER; i++) {
@@ -208,15 +227,15 @@ extern "C" __global__ __launch_bounds__(SLOT_THREADS) void paged_slots(SlotArgs 
   }
   if (t == 0) {
     a.offsets[a.seqs] = p.rows;
-    a.ends_out[0] = first + all_taken;
-    a.ends_out[1] = last + all_back;
-    if (a.failed) a.failed[0] = (int)all_lost;
+    a.ends_out[0] = first + all4[2];
+    a.ends_out[1] = last + all4[1];
+    if (a.failed) a.failed[0] = (int)all4[3];
   }
   if (a.here) {
-    slot_rows(a, p, t, SLOT_THREADS);
+    slot_rows(a, p, t, blockDim.x);
     return;
   }
-  for (int i = t; i < 5 * a.seqs; i += SLOT_THREADS) a.plan[i] = slot_lds[i];
+  for (int i = t; i < 5 * a.seqs; i += blockDim.x) a.plan[i] = slot_lds[i];
   if (t == 0) {
     int* const e = a.plan + 5 * a.seqs;
     e[0] = p.rows;
@@ -526,14 +545,16 @@ template <int T, int D>
 struct AttnShape {
   static constexpr int ES = T == 0 ? 4 : 2;            // bytes of a value
   static constexpr int KS = T == 0 ? 16 : 32;          // keys of a wave's step
-  static constexpr int TK = 4 * KS;                    // keys of a block's tile
+  static constexpr int DS = D == 512 ? 2 : 1;          // waves that share a head's dimensions (registers)
+  static constexpr int DW = D / DS;                    // dimensions of a wave
+  static constexpr int KG = 4 / DS;                    // groups of keys: the others' waves
+  static constexpr int TK = KG * KS;                   // keys of a block's tile
   static constexpr int NT = KS / 16;                   // score tiles of a step
   static constexpr int QL = 16 / ES;                   // values of a key load
-  static constexpr int NQ = D / (4 * QL);              // key loads of a lane and key
-  static constexpr int KH = D == 512 ? 2 : 1;          // chunks that a step's keys are loaded in (registers)
+  static constexpr int NQ = DW / (4 * QL);             // key loads of a lane and key
   static constexpr int NP = T == 0 ? 1 : T == 1 ? 2 : 3;  // parts of a single value
   static constexpr int VL = T != 0 && D > 64 ? 8 : 4;  // values of a value load
-  static constexpr int NJ = D / (16 * VL);             // value loads of a lane and key
+  static constexpr int NJ = DW / (16 * VL);            // value loads of a lane and key
   static constexpr int OS = D + 4;                     // a head's row in o_s
   static constexpr float P0 = T == 1 ? 15.f : 0.f;     // weights times 2^P0: halves' normal range
 };
@@ -541,12 +562,13 @@ struct AttnShape {
 template <int T, int D>
 struct AttnLds {
   using S = AttnShape<T, D>;
-  uintx4 q[S::NP * S::NQ * 64];  // the query tile as the matrix cores take it, by lane
+  uintx4 q[S::NP * S::DS * S::NQ * 64];  // the query tile as the matrix cores take it, by lane
   float o[16 * S::OS];           // a piece's values
   float m[16], l[16];            // its maxima and sums
   float wm[4][16], wl[4][16];    // the waves'
   float qs[16];                  // powers of two that the queries were divided by
   int64_t off[4][2][S::KS];      // byte offsets of the steps' keys
+  floatx4 x[S::DS > 1 ? 2 : 1][S::DS > 1 ? 4 : 1][S::NT][64];  // the waves' shares of the scores
 };
 
 // The heads of a piece whose sums are not all finite, again by the formula's own
@@ -644,7 +666,7 @@ __device__ __forceinline__ void stage_query(const PagedAttnArgs& a, const AttnIt
     }
     __syncthreads();
   }
-  for (int i = t; i < S::NQ * 64; i += 256) {
+  for (int i = t; i < S::DS * S::NQ * 64; i += 256) {
     const int c = i & 15, d0 = (i >> 6) * 4 * S::QL + ((i >> 4) & 3) * S::QL;
     float v[S::QL];
     const bool in = c < it.heads && d0 < a.hd;
@@ -662,7 +684,7 @@ __device__ __forceinline__ void stage_query(const PagedAttnArgs& a, const AttnIt
 #pragma unroll
       for (int j = 0; j < 4; j++) split2<T>(v[2 * j], v[2 * j + 1], part[j]);
 #pragma unroll
-      for (int n = 0; n < S::NP; n++) s.q[n * S::NQ * 64 + i] = uintx4{part[0][n], part[1][n], part[2][n], part[3][n]};
+      for (int n = 0; n < S::NP; n++) s.q[n * S::DS * S::NQ * 64 + i] = uintx4{part[0][n], part[1][n], part[2][n], part[3][n]};
     }
   }
   __syncthreads();
@@ -684,7 +706,10 @@ __device__ __forceinline__ void stage_query(const PagedAttnArgs& a, const AttnIt
 // registers. No key, value or weight goes through LDS, and the running maximum, sum
 // and rescale are a lane's own. Queries and weights enter as 2 half or 3 bf16
 // parts (f32 caches: the f32 matrix cores), so the sums are those of single.
-// HBM bound: the cache is read once.
+// HBM bound: the cache is read once. Heads beyond 256 give a wave half of the
+// dimensions, two waves adding their shares of the scores in LDS, as the values of
+// 512 do not fit the registers beside the keys (one wave each, spilling: 16
+// sequences of 8192, 2 KV heads 252 us).
 template <int T, int D, bool FULL>
 __device__ __forceinline__ void paged_attention_t(const PagedAttnArgs& a)
 {
@@ -768,7 +793,8 @@ __device__ __forceinline__ void paged_attention_t(const PagedAttnArgs& a)
     const char* const kb = a.kc + (int64_t)it.kv * a.head_stride * S::ES;
     const char* const vb = a.vc + (int64_t)it.kv * a.head_stride * S::ES;
     const int* const table = a.table + (int64_t)seq * a.max_pages;
-    const int64_t wlo = lo + w * S::KS;
+    const int kg = w / S::DS, dh = w % S::DS;  // the wave's keys of a tile, its dimensions
+    const int64_t wlo = lo + kg * S::KS;
     // a step's key of this lane: its page's table entry
     auto entry = [&](uint32_t tile) {
       const int64_t j = wlo + (int64_t)tile * S::TK + (lane & (S::KS - 1));
@@ -790,15 +816,14 @@ __device__ __forceinline__ void paged_attention_t(const PagedAttnArgs& a)
     stage_query<T, D>(a, it, s);
     const float sscale = T == 1 ? s.qs[c] : 1.f;
 
-    constexpr int KC = S::NQ / S::KH;
-    uintx4 kr[S::NT][KC];
-    auto load_keys = [&](uint32_t tile, int chunk) {
+    uintx4 kr[S::NT][S::NQ];
+    auto load_keys = [&](uint32_t tile) {
 #pragma unroll
       for (int i = 0; i < S::NT; i++) {
         const char* const p = kb + s.off[w][tile & 1][16 * i + c];
 #pragma unroll
-        for (int j = 0; j < KC; j++) {
-          const int d0 = (chunk * KC + j) * 4 * S::QL + g * S::QL;
+        for (int j = 0; j < S::NQ; j++) {
+          const int d0 = dh * S::DW + j * 4 * S::QL + g * S::QL;
           const bool in = FULL || d0 < hd;
           kr[i][j] = *(const uintx4*)(p + (in ? d0 : 0) * S::ES);
           if (!in) kr[i][j] = uintx4{0, 0, 0, 0};
@@ -813,7 +838,9 @@ __device__ __forceinline__ void paged_attention_t(const PagedAttnArgs& a)
       for (int j = 0; j < S::VL; j++) o[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
     float m = -__builtin_inff(), l = 0.f;
     uint32_t steps = 0;  // of this wave: up to the last tile with a key of its own
-    if (wlo + (int64_t)tile0 * S::TK < hi) {
+    if (S::DS > 1) {
+      steps = tile1 - tile0;  // the waves meet in each step
+    } else if (wlo + (int64_t)tile0 * S::TK < hi) {
       const uint32_t mine = (uint32_t)((hi - wlo + S::TK - 1) / S::TK);
       steps = min(tile1, mine) - tile0;
     }
@@ -821,7 +848,7 @@ __device__ __forceinline__ void paged_attention_t(const PagedAttnArgs& a)
     // located and loaded one step past the last too: entry() has no page there and
     // the loads read the pool's first row.
     uint32_t there = locate(tile, page0);
-    if (steps) load_keys(tile, 0);
+    if (steps) load_keys(tile);
     for (uint32_t i = 0; i < steps; i++, tile++) {
       // the step's values, on their way while its scores are formed
       constexpr int NV = 4 * S::NT;  // keys of a lane: 16 q + 4 g + r
@@ -831,7 +858,7 @@ __device__ __forceinline__ void paged_attention_t(const PagedAttnArgs& a)
         const char* const p = vb + s.off[w][tile & 1][16 * (k >> 2) + 4 * g + (k & 3)];
 #pragma unroll
         for (int j = 0; j < S::NJ; j++) {
-          const int d0 = j * 16 * S::VL + c * S::VL;
+          const int d0 = dh * S::DW + j * 16 * S::VL + c * S::VL;
           const char* const v = p + (FULL || d0 < hd ? d0 : 0) * S::ES;
           if constexpr (S::VL * S::ES == 16) {
             vr[k][j] = *(const uintx4*)v;
@@ -848,27 +875,31 @@ __device__ __forceinline__ void paged_attention_t(const PagedAttnArgs& a)
 #pragma unroll
       for (int k = 0; k < S::NT; k++) x[k] = floatx4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int h = 0; h < S::KH; h++) {
-        if (h) load_keys(tile, h);
+      for (int j = 0; j < S::NQ; j++) {
 #pragma unroll
-        for (int j = 0; j < KC; j++) {
+        for (int n2 = 0; n2 < S::NP; n2++) {
+          const uintx4 q = s.q[(n2 * S::DS * S::NQ + dh * S::NQ + j) * 64 + lane];
 #pragma unroll
-          for (int n2 = 0; n2 < S::NP; n2++) {
-            const uintx4 q = s.q[(n2 * S::NQ + h * KC + j) * 64 + lane];
+          for (int k = 0; k < S::NT; k++) {
+            if constexpr (T == 0) {
 #pragma unroll
-            for (int k = 0; k < S::NT; k++) {
-              if constexpr (T == 0) {
-#pragma unroll
-                for (int e = 0; e < 4; e++)
-                  x[k] = __builtin_amdgcn_mfma_f32_16x16x4f32(bits_float(kr[k][j][e]), bits_float(q[e]), x[k], 0, 0, 0);
-              } else {
-                x[k] = mfma16<T>(kr[k][j], q, x[k]);
-              }
+              for (int e = 0; e < 4; e++)
+                x[k] = __builtin_amdgcn_mfma_f32_16x16x4f32(bits_float(kr[k][j][e]), bits_float(q[e]), x[k], 0, 0, 0);
+            } else {
+              x[k] = mfma16<T>(kr[k][j], q, x[k]);
             }
           }
         }
       }
-      load_keys(tile + 1, 0);
+      load_keys(tile + 1);
+      if constexpr (S::DS > 1) {
+        // the scores of all dimensions: two waves' shares added, the same sum in both
+#pragma unroll
+        for (int k = 0; k < S::NT; k++) s.x[tile & 1][w][k][lane] = x[k];
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < S::NT; k++) x[k] += s.x[tile & 1][w ^ 1][k][lane];
+      }
       // masked keys: no weight, and values of zero (0 times NaN is NaN)
       float top = -__builtin_inff();
       if (now == (uint32_t)((1ull << S::KS) - 1)) {
@@ -936,32 +967,34 @@ __device__ __forceinline__ void paged_attention_t(const PagedAttnArgs& a)
 
     // the waves' sums meet
     l = quad_sum(l);
-    if (g == 0) {
-      s.wm[w][c] = m;
-      s.wl[w][c] = l;
+    if (g == 0 && dh == 0) {
+      s.wm[kg][c] = m;
+      s.wl[kg][c] = l;
     }
     __syncthreads();
-    float M = fmaxf(fmaxf(s.wm[0][c], s.wm[1][c]), fmaxf(s.wm[2][c], s.wm[3][c]));
+    float M = s.wm[0][c];
+#pragma unroll
+    for (int i = 1; i < S::KG; i++) M = fmaxf(M, s.wm[i][c]);
     const float Ms = M == -__builtin_inff() ? 0.f : M;
     const float f = exp2_fast(m - Ms - S::P0);
     bool odd = false;
     if (w == 0 && g == 0) {
       float L = 0.f;
 #pragma unroll
-      for (int i = 0; i < 4; i++) L += s.wl[i][c] * exp2_fast(s.wm[i][c] - Ms - S::P0);
+      for (int i = 0; i < S::KG; i++) L += s.wl[i][c] * exp2_fast(s.wm[i][c] - Ms - S::P0);
       s.m[c] = M;
       s.l[c] = L;
       odd = c < it.heads && !finite(L);
     }
-    for (int r4 = 0; r4 < 4; r4++) {
-      if (w == r4) {
+    for (int r4 = 0; r4 < S::KG; r4++) {
+      if (kg == r4) {
 #pragma unroll
         for (int j = 0; j < S::NJ; j++)
 #pragma unroll
           for (int r = 0; r < 4; r++)
 #pragma unroll
             for (int e = 0; e < S::VL; e += 4) {
-              floatx4* const d = (floatx4*)&s.o[c * S::OS + j * 16 * S::VL + S::VL * (4 * g + r) + e];
+              floatx4* const d = (floatx4*)&s.o[c * S::OS + dh * S::DW + j * 16 * S::VL + S::VL * (4 * g + r) + e];
               floatx4 v = {o[j][e][r] * f, o[j][e + 1][r] * f, o[j][e + 2][r] * f, o[j][e + 3][r] * f};
               if (r4) v += *d;
               *d = v;
@@ -1098,14 +1131,18 @@ __device__ __forceinline__ void paged_attention_t(const PagedAttnArgs& a)
   }
 }
 
-#define PAGED_ATTENTION(NAME, T, D)                                                                     \
-  extern "C" __global__ __launch_bounds__(256) void paged_attention_##NAME##_##D(PagedAttnArgs a)       \
-  {                                                                                                     \
-    paged_attention_t<T, D, true>(a);                                                                   \
-  }                                                                                                     \
-  extern "C" __global__ __launch_bounds__(256) void paged_attention_##NAME##_##D##_part(PagedAttnArgs a) \
-  {                                                                                                     \
-    paged_attention_t<T, D, false>(a);                                                                  \
+// heads between two sizes: two blocks a CU up to 128 (the bound costs the join of few
+// long sequences, 24 us became 32, so the others, which stay below 256 registers on
+// their own, have none)
+#define PAGED_ATTENTION(NAME, T, D)                                                                         \
+  extern "C" __global__ __launch_bounds__(256) void paged_attention_##NAME##_##D(PagedAttnArgs a)           \
+  {                                                                                                         \
+    paged_attention_t<T, D, true>(a);                                                                       \
+  }                                                                                                         \
+  extern "C" __global__ __launch_bounds__(256, D == 128 ? 2 : 1) void                                       \
+  paged_attention_##NAME##_##D##_part(PagedAttnArgs a)                                                      \
+  {                                                                                                         \
+    paged_attention_t<T, D, false>(a);                                                                      \
   }
 PAGED_ATTENTION(f32, 0, 64)
 PAGED_ATTENTION(f32, 0, 128)
