@@ -1050,7 +1050,19 @@ __device__ __forceinline__ void paged_attention_t(const PagedAttnArgs& a)
       // pieces i0, i0 + step, .. (cnt of them, at most 64) joined in that order: into
       // the output, or into the first of them
       auto join = [&](uint32_t i0, uint32_t step, uint32_t cnt, bool out) {
-        float* const wt = s.o;  // [64][16]: a piece's weight for each head
+        // 4 values of 16 pieces a thread, the first on their way while the weights are formed
+        const int total = it.heads * a.hd;
+        uint64_t x[16][2];
+        auto fetch = [&](int i, uint32_t j0) {
+#pragma unroll
+          for (uint32_t k = 0; k < 16; k++) {
+            const double* const e = (const double*)(piece(i0 + step * min(j0 + k, cnt - 1)) + i);
+            x[k][0] = __builtin_bit_cast(uint64_t, load_agent(e));
+            x[k][1] = __builtin_bit_cast(uint64_t, load_agent(e + 1));
+          }
+        };
+        if (4 * t < total) fetch(4 * t, 0);
+        float* const wt = s.o;  // [64][16]: a piece's weight for each head, 0 past the last
         {
           const int h = t >> 4;
           float pm[4], pl[4], M2 = -__builtin_inff(), L = 0.f;
@@ -1085,25 +1097,30 @@ __device__ __forceinline__ void paged_attention_t(const PagedAttnArgs& a)
           }
         }
         __syncthreads();
-        for (int i = 2 * t; i < it.heads * a.hd; i += 512) {
+        for (int i = 4 * t; i < total; i += 1024) {
           const int h = i / a.hd;
-          float v0 = 0.f, v1 = 0.f;
-#pragma unroll 8
-          for (uint32_t j = 0; j < cnt; j++) {
-            const uint64_t x = __builtin_bit_cast(uint64_t, load_agent((const double*)(piece(i0 + step * j) + i)));
-            const float f2 = wt[j * 16 + h];
-            // (a part of no weight may hold an infinity)
-            v0 = __builtin_fmaf(f2, f2 != 0.f ? bits_float((uint32_t)x) : 0.f, v0);
-            v1 = __builtin_fmaf(f2, f2 != 0.f ? bits_float((uint32_t)(x >> 32)) : 0.f, v1);
+          float v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+          for (uint32_t j0 = 0; j0 < cnt; j0 += 16) {
+            if (i != 4 * t || j0) fetch(i, j0);
+#pragma unroll
+            for (uint32_t k = 0; k < 16; k++) {
+              const float f2 = wt[(j0 + k) * 16 + h];
+#pragma unroll
+              for (int e = 0; e < 4; e++) {
+                const float p = bits_float((uint32_t)(x[k][e / 2] >> (32 * (e & 1))));
+                v[e] = __builtin_fmaf(f2, f2 != 0.f ? p : 0.f, v[e]);  // (a part of no weight may hold an infinity)
+              }
+            }
           }
           if (out) {
             float f2;
             finish(h, s.m[h], s.l[h], f2);
-            y[i] = f2 == 0.f ? 0.f : v0 * f2;
-            y[i + 1] = f2 == 0.f ? 0.f : v1 * f2;
+#pragma unroll
+            for (int e = 0; e < 4; e++) y[i + e] = f2 == 0.f ? 0.f : v[e] * f2;
           } else {
-            store_agent(piece(i0) + i, v0);
-            store_agent(piece(i0) + i + 1, v1);
+#pragma unroll
+            for (int e = 0; e < 4; e++) store_agent(piece(i0) + i + e, v[e]);
           }
         }
       };
