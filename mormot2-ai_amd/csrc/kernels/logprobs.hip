@@ -301,13 +301,17 @@ extern "C" __global__ __launch_bounds__(256) void logprobs(LogprobArgs a)
     z.w = wave_sum(z.w, 4);
     if (a.k) {
       // an alternative's place among all: behind its own list's, and the others' better ones
+      // (the lists descend, so a number's place in one is a search)
       const uint64_t mine = top.v;
+      int n[3] = {0, 0, 0};
+#pragma unroll 1
+      for (int step = 32; step; step >>= 1)
+#pragma unroll
+        for (int i = 0; i < 3; i++)
+          if (list_s[(w + i + 1) & 3][n[i] + step - 1] > mine) n[i] += step;
       int rank = lane;
-      for (int i = 1; i < 4; i++) {
-        const uint64_t* const o = list_s[(w + i) & 3];
-#pragma unroll 4
-        for (int j = 0; j < a.k; j++) rank += o[j] > mine;
-      }
+#pragma unroll
+      for (int i = 0; i < 3; i++) rank += n[i] + (n[i] == 63 && list_s[(w + i + 1) & 3][63] > mine);
       buf_s[0][t < a.k ? t : 64] = 0;
       __syncthreads();
       if (lane < a.k && mine && rank < a.k) buf_s[0][rank] = mine;

@@ -351,14 +351,14 @@ __device__ __forceinline__ void paged_qkrope_t(const PagedRopeArgs& a)
   const int pos = a.positions[row];
   if (pos < 0) return;  // (the block's threads alike)
   const int64_t base = paged_slot_value(a.slots[row], a.page_size, a.pages, a.page_stride, a.slot_stride);
-  if (t < a.half) {
+  for (int i = t; i < a.half; i += blockDim.x) {
     double c, s;
-    turn((double)a.freq[t] * (double)pos, c, s);
-    cs[t] = make_double2(c * a.scale, s * a.scale);
+    turn((double)a.freq[i] * (double)pos, c, s);
+    cs[i] = make_double2(c * a.scale, s * a.scale);
   }
   __syncthreads();
   const int seg = a.seg, all = (a.heads + 2 * a.kvh) * seg, hd = a.hd;
-  for (int i = blockIdx.y * 256 + t; i < all; i += a.parts * 256) {
+  for (int i = blockIdx.y * blockDim.x + t; i < all; i += a.parts * blockDim.x) {
     const int h = i / seg, u = i & (seg - 1);  // the head, the lane's unit of 8 values
     const int kind = h < a.heads ? 0 : h < a.heads + a.kvh ? 1 : 2;
     const int hh = kind == 0 ? h : kind == 1 ? h - a.heads : h - a.heads - a.kvh;
