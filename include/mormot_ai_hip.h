@@ -600,7 +600,7 @@ typedef struct {
 
 /* rotary positions of q and k: value pairs (i, i + dims / 2) of a head's
  * first dims values, or (2 i, 2 i + 1) when interleaved, turned by the angle
- * freq[i] * position (formed in double) and scaled by `scale` */
+ * freq[i] * position (formed in double, up to 2^31) and scaled by `scale` */
 typedef struct {
   uint64_t freq;           /* device address of [dims / 2] floats (ihip_model_frequencies) */
   int32_t dims;            /* even, up to head_dim; 0: the whole head */
@@ -641,10 +641,12 @@ int ihip_enqueue_paged_slots(ihip_ctx* ctx, uint64_t past, uint64_t count, int64
 /* the new rows' q, k and v between the q/k/v Linear and the attention: per row
  * and head the RMSNorm of q and k heads (qn, kn device [head_dim] or 0), rotary
  * positions (rope, NULL: none), q written to q_out ([rows, heads, head_dim], or 0:
- * in place), k and v stored into the cache at the row's slot. Strides: floats
- * from a row to the next (0: the rows are contiguous). A row with position < 0
- * is left as it was; a slot outside the pool stores nothing. The rows of one
- * call have slots of their own. (ihip_enqueue_qkrope over a paged cache) */
+ * in place; elsewhere it does not overlap q), k and v stored into the cache at
+ * the row's slot. Strides: floats from a row to the next (0: the rows are
+ * contiguous). A row with position < 0 is left as it was; a slot outside the
+ * pool stores nothing. The rows of one call have slots of their own: of two in
+ * one slot either may stay, value by value. (ihip_enqueue_qkrope over a paged
+ * cache) */
 int ihip_enqueue_paged_qkrope(ihip_ctx* ctx, uint64_t q, int64_t q_stride, uint64_t k,
                               int64_t k_stride, uint64_t v, int64_t v_stride, int64_t rows,
                               int64_t heads, uint64_t qn, uint64_t kn, double eps,

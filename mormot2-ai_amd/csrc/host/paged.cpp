@@ -36,6 +36,9 @@ int refuse(const char* who, const char* why, int code = IHIP_E_ARG)
   return fail(code, std::string(who) + ": " + why);
 }
 
+// floats from a row to the next: rows times it stay far from 64 bits
+constexpr int64_t STRIDE_MOST = (int64_t)1 << 36;
+
 // a pool with its strides filled in
 struct Pool {
   int64_t page_stride = 0, slot_stride = 0, head_stride = 0;
@@ -117,14 +120,17 @@ int ihip_enqueue_paged_qkrope(ihip_ctx* c, uint64_t q, int64_t q_stride, uint64_
   const char* who = "ihip_enqueue_paged_qkrope";
   Pool p;
   if (int rc = check_pool(who, cache, &p)) return rc;
-  const int64_t hd = cache->head_dim, kvh = cache->kv_heads, qw = heads * hd, kw = kvh * hd;
+  const int64_t hd = cache->head_dim, kvh = cache->kv_heads;
   if (!q || !k || !v || !positions || !slots) return refuse(who, "a missing array");
-  if (rows < 1 || rows > INT32_MAX || heads < 1 || heads > 65535 || heads % kvh)
+  // (a grid of 256 threads a row counts its threads in 32 bits)
+  if (rows < 1 || rows > 1 << 23 || heads < 1 || heads > 65535 || heads % kvh)
     return refuse(who, "rows or heads out of range");
+  const int64_t qw = heads * hd, kw = kvh * hd;
   q_stride = q_stride ? q_stride : qw;
   k_stride = k_stride ? k_stride : kw;
   v_stride = v_stride ? v_stride : kw;
   if (q_stride < qw || k_stride < kw || v_stride < kw) return refuse(who, "a stride below a row");
+  if (std::max({q_stride, k_stride, v_stride}) > STRIDE_MOST) return refuse(who, "a stride beyond 2^36");
   const uint64_t aligned = q | k | v | q_out | qn | kn;
   if (aligned % 4) return refuse(who, "floats aligned to 4 bytes");
   if (!(eps >= 0) || !std::isfinite(eps)) return refuse(who, "eps");
@@ -183,6 +189,7 @@ int ihip_enqueue_paged_attention(ihip_ctx* c, uint64_t q, int64_t q_stride, cons
     return refuse(who, "seqs, heads, window or max_pages out of range");
   q_stride = q_stride ? q_stride : heads * hd;
   if (q_stride < heads * hd) return refuse(who, "a stride below a row");
+  if (q_stride > STRIDE_MOST) return refuse(who, "a stride beyond 2^36");
   if ((q | y | sinks | lengths | table) % 4) return refuse(who, "arrays aligned to 4 bytes");
   if (std::isnan(scale) || std::isinf(scale)) return refuse(who, "scale");
   // the kernels take tiles of 128 keys of 16-bit caches, 64 of single ones, half as
@@ -233,6 +240,7 @@ int ihip_enqueue_logprobs(ihip_ctx* c, uint64_t logits, int64_t rows, int64_t vo
     return refuse(who, "rows or vocab out of range");
   stride = stride ? stride : vocab;
   if (stride < vocab) return refuse(who, "a stride below a row");
+  if (stride > STRIDE_MOST || rows > (int64_t)1 << 24) return refuse(who, "rows beyond 2^24 or a stride beyond 2^36");
   if ((logits | ids | logprobs | entropy | top_ids | top_logprobs) % 4)
     return refuse(who, "arrays aligned to 4 bytes");
   if (!c) return no_context(who);

@@ -551,3 +551,67 @@ def test_two_contexts(dev, ctx):
         for i in range(3):
             assert_close(*attention_case(ctx, dev, rng, "f16", 128, 16, 2, 16, [1500, 3, 700])[:3])
             assert_close(*attention_case(other, dev2, rng, "f16", 128, 16, 2, 16, [900, 2500])[:3])
+
+
+def test_first_calls_captured():
+    """The first calls of a context, captured before any kernel of theirs has run; two graphs of
+    one context share its workspaces, replayed in turn over other lengths."""
+    rng = np.random.default_rng(51)
+    n, heads, kvh, hd, ps, pages = 6, 16, 2, 128, 16, 400
+    with H.Context(0) as c:
+        k, v = (R.pack(rng.standard_normal((pages, ps, kvh, hd)), "f16") for _ in range(2))
+        dk, dv = c.array(k), c.array(v)
+        pool = pages_struct(dk.ptr, dv.ptr, pages, ps, kvh, hd, "f16")
+        table = rng.permutation(pages)[:n * 60].reshape(n, 60).astype(np.int32)
+        q = rng.standard_normal((n, heads, hd)).astype(np.float32)
+        x = rng.standard_normal((3, 40000)).astype(np.float32)
+        dt, dq, dx = c.array(table), c.array(q), c.array(x)
+        lens = [c.array(np.zeros(n, np.int32)) for _ in range(2)]
+        ys = [c.alloc(q.nbytes) for _ in range(2)]
+        top = [[c.alloc(4 * 3 * 8) for _ in range(2)] for _ in range(2)]
+        for g in range(2):
+            H.check(H.lib().ihip_capture_begin(c.h))
+            H.check(H.lib().ihip_enqueue_paged_attention(
+                c.h, dq.ptr, 0, C.byref(pool), dt.ptr, 60, lens[g].ptr, ys[g].ptr, n, heads, 0, 0, 0.0))
+            H.check(H.lib().ihip_enqueue_logprobs(c.h, dx.ptr, 3, 40000, 0, 0, 0, 0, 8, top[g][0].ptr, top[g][1].ptr))
+            H.check(H.lib().ihip_capture_end(c.h, g))
+        for i in range(5):
+            ln = [rng.integers(0, 960, n).astype(np.int32) for _ in range(2)]
+            for g in range(2):
+                lens[g].upload(ln[g])
+            for g in range(2):
+                H.check(H.lib().ihip_graph_launch(c.h, g))
+            for g in range(2):
+                got = ys[g].download(np.float32, q.size).reshape(q.shape)
+                want, tol = R.attention(q.astype(np.float64), R.unpack(k, "f16"), R.unpack(v, "f16"), table, ln[g], ps)
+                assert_close(got, want, tol)
+                ids = top[g][0].download(np.int32, 24).reshape(3, 8)
+                assert np.array_equal(ids, np.stack([R.order(r)[:8] for r in x]))
+            # an eager call between the replays
+            H.check(H.lib().ihip_enqueue_paged_attention(
+                c.h, dq.ptr, 0, C.byref(pool), dt.ptr, 60, lens[0].ptr, ys[1].ptr, n, heads, 0, 0, 0.0))
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+def test_attention_many_short_sequences(ctx, dev, dtype):
+    """More sequences than a wave scans at once, empty places and empty rows among them."""
+    rng = np.random.default_rng(61)
+    lengths = rng.integers(-1, 40, 700)
+    lengths[rng.random(700) < 0.3] = 0
+    assert_close(*attention_case(ctx, dev, rng, dtype, 64, 2, 1, 8, lengths.tolist()))
+
+
+def test_attention_of_nobody(ctx, dev):
+    """No sequence has a key: zeros and rows left alone, nothing else."""
+    rng = np.random.default_rng(62)
+    got, want, tol, lengths = attention_case(ctx, dev, rng, "bf16", 128, 8, 2, 16, [0, -1, 0, -5, 0])
+    assert (got == 0).all() and len(got) == 3
+
+
+def test_attention_shares_pages(ctx, dev):
+    """Two sequences over the same pages (a common prompt), unlike lengths."""
+    def change(q, k, v, table, lengths):
+        table[1, :4] = table[0, :4]
+
+    rng = np.random.default_rng(63)
+    assert_close(*attention_case(ctx, dev, rng, "f16", 128, 8, 2, 16, [90, 60], change=change))

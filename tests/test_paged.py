@@ -76,6 +76,10 @@ def test_attention_refused():
         refused(lambda: attention(pages(), **bad), -1, "out of range")
     refused(lambda: attention(pages(), seqs=H.PAGED_SEQS + 1), -6, "IHIP_PAGED_SEQS")
     refused(lambda: attention(pages(), q_stride=255), -1, "stride below")
+    refused(lambda: attention(pages(), q_stride=1 << 37), -1, "2^36")
+    # tables whose tiles of keys pass 32 bits
+    refused(lambda: attention(pages(page_size=1 << 20, pages=2, kv_heads=2, head_dim=8), max_pages=1 << 10,
+                              seqs=4096, heads=64), -6, "2^31 tiles")
     for bad in (float("nan"), float("inf")):
         refused(lambda: attention(pages(), scale=bad), -1, "scale")
     # everything in order but the context
@@ -91,6 +95,9 @@ def test_qkrope_refused():
         refused(lambda: qkrope(pages(), **bad), -1, "out of range")
     for bad in (dict(qs=255), dict(ks=127), dict(vs=100)):
         refused(lambda: qkrope(pages(), **bad), -1, "stride below")
+    refused(lambda: qkrope(pages(), qs=1 << 37), -1, "2^36")
+    refused(lambda: qkrope(pages(), rows=(1 << 23) + 1), -1, "out of range")
+    refused(lambda: qkrope(pages(), heads=1 << 60), -1, "out of range")
     refused(lambda: qkrope(pages(), q=A + 2), -1, "4 bytes")
     for bad in (-1.0, float("nan"), float("inf")):
         refused(lambda: qkrope(pages(), eps=bad), -1, "eps")
@@ -134,6 +141,7 @@ def test_logprobs_refused():
     for bad in (dict(k=-1), dict(k=H.LOGPROBS_TOP + 1)):
         refused(lambda: call(**bad), -6, "IHIP_LOGPROBS_TOP")
     refused(lambda: call(stride=999), -1, "stride below")
+    refused(lambda: call(stride=1 << 37), -1, "2^36")
     refused(lambda: call(entropy=A + 1), -1, "4 bytes")
     refused(lambda: call(ids=0, logprobs=0), -1, "no context")
 
