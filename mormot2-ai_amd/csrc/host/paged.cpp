@@ -103,10 +103,11 @@ int ihip_enqueue_paged_slots(ihip_ctx* c, uint64_t past, uint64_t count, int64_t
          (int*)c->paged_plan, (int32_t)seqs, (int32_t)max_pages, (int32_t)page_size, (int32_t)pages,
          (int32_t)rows, rows <= PAGED_ROWS_HERE};
   const size_t shmem = (size_t)seqs * 5 * 4;
-  // a thread for 4 sequences, and where this block writes the rows one for a row
-  // and a wave beside them for the pages that move
-  const int64_t threads = std::max<int64_t>((seqs + 3) / 4, a.here ? std::min<int64_t>(rows + 64, 1024) : 256);
-  int rc = launch(c, "paged_slots", dim3(1), dim3((unsigned)((threads + 63) / 64 * 64)), &a, shmem);
+  // a thread for the kernel's sequences, and where this block writes the rows one for
+  // a row and a wave beside them for the pages that move
+  const int per = seqs <= 256 ? 1 : 4;
+  const int64_t threads = std::max<int64_t>((seqs + per - 1) / per, a.here ? std::min<int64_t>(rows + 64, 1024) : 256);
+  int rc = launch(c, per == 1 ? "paged_slots_1" : "paged_slots_4", dim3(1), dim3((unsigned)((threads + 63) / 64 * 64)), &a, shmem);
   if (rc || a.here) return rc;
   return launch(c, "paged_slots_rows", dim3((unsigned)std::min<int64_t>(4 * c->cus, (rows + 1023) / 1024)),
                 dim3(256), &a, shmem);

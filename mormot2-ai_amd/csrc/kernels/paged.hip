@@ -12,13 +12,12 @@ struct SlotArgs {
   const int64_t* ends;
   int64_t* ends_out;
   int *offsets, *lengths, *positions, *slots, *failed;
-  int* plan;  // [5][seqs], then 3: the plan between the two launches
+  int* plan;  // [5][seqs], then 4 numbers: the plan between the two launches
   int32_t seqs, max_pages, page_size, pages, rows;
   int32_t here;  // 1: the rows in this launch too
 };
 
-constexpr int SLOT_THREADS = 1024, SLOT_PER = 4;  // sequences: 4 a thread
-static_assert(SLOT_THREADS * SLOT_PER == 4096, "IHIP_PAGED_SEQS");
+constexpr int SLOT_THREADS = 1024;  // and up to 4 sequences a thread: IHIP_PAGED_SEQS
 
 // one step of a scan over the wave: v and what lane - CTRL's shift holds (0 beyond
 // the row of 16; broadcasts of a row's last lane: to the rows of `rows`)
@@ -126,11 +125,14 @@ __device__ __forceinline__ void slot_rows(const SlotArgs& a, const SlotPlan& p, 
   }
 }
 
-// one block: two scans over the sequences (rows and pages put back; then the
-// pages taken, which depend on the rows that fit), the plan in LDS. Everything
-// that a caller may pass as input and output is read before the barrier behind
-// which it is written. Latency bound.
-extern "C" __global__ __launch_bounds__(SLOT_THREADS) void paged_slots(SlotArgs a)
+// One block: scans over the sequences (rows and pages put back; the pages taken,
+// which depend on the rows that fit; the moves), the plan in LDS. Everything that a
+// caller may pass as input and output is read before the barrier behind which it is
+// written. Latency bound: the lengths, then a table entry or a free page, then the
+// stores. 64 sequences' decode step 6.7 us; 500 with 150000 rows 6.0 us and 8.6 for
+// paged_slots_rows.
+template <int SLOT_PER>
+__device__ __forceinline__ void paged_slots_t(const SlotArgs& a)
 {
   extern __shared__ int slot_lds[];
   SlotPlan p = slot_plan(slot_lds, a.seqs);
@@ -139,8 +141,10 @@ extern "C" __global__ __launch_bounds__(SLOT_THREADS) void paged_slots(SlotArgs 
   const int64_t first = a.ends[0], last = a.ends[1];
   int64_t free_pages = first >= 0 && last > first ? last - first : 0;
   if (free_pages > a.pages) free_pages = a.pages;
-  p.first = first >= 0 ? (int)(first % a.pages) : 0;
-  p.last = last >= 0 ? (int)(last % a.pages) : 0;
+  // (a 64-bit remainder is a long way around, for a ring turned 2^32 times)
+  auto turned = [&](int64_t v) { return v >> 32 ? (int)(v % a.pages) : (int)((uint32_t)v % (uint32_t)a.pages); };
+  p.first = first >= 0 ? turned(first) : 0;
+  p.last = last >= 0 ? turned(last) : 0;
 
   int past[SLOT_PER], live[SLOT_PER], fresh[SLOT_PER], have[SLOT_PER];
   int64_t rows = 0, back = 0;
@@ -245,6 +249,12 @@ extern "C" __global__ __launch_bounds__(SLOT_THREADS) void paged_slots(SlotArgs 
   }
 }
 
+// one sequence a thread up to 256 (a decode step of 64 6.7 us; four a thread, whose
+// code is longer and comes from a cold cache, 8.3), else four (500 sequences 6.0 us,
+// one a thread, whose scans have four times the waves, 6.5)
+extern "C" __global__ __launch_bounds__(SLOT_THREADS) void paged_slots_1(SlotArgs a) { paged_slots_t<1>(a); }
+extern "C" __global__ __launch_bounds__(SLOT_THREADS) void paged_slots_4(SlotArgs a) { paged_slots_t<4>(a); }
+
 // the rows of a step with prompts, by as many blocks as they fill: the plan
 // from paged_slots' launch
 extern "C" __global__ __launch_bounds__(256) void paged_slots_rows(SlotArgs a)
@@ -317,7 +327,7 @@ __device__ __forceinline__ uint16_t float_to_bf16(float f)
   return (uint16_t)((b + 0x7fffu + ((b >> 16) & 1u)) >> 16);
 }
 
-// N (2 or 4) consecutive values of a cache row; T: 0 float, 1 half, 2 bf16
+// consecutive values of a cache row; T: 0 float, 1 half, 2 bf16
 template <int T>
 __device__ __forceinline__ void store4(char* p, const float (&v)[4])
 {
@@ -341,7 +351,10 @@ __device__ __forceinline__ void store1(char* p, float v)
 // heads (q, k, then v), 8 values (4 pairs) a lane, a head in `seg` lanes, so that
 // the norm is a sum over aligned lanes. Sums, angles and the rotation are in
 // double (full rate on this chip) and rounded once to single, then to the
-// cache's type. Bound by HBM: 4 bytes in and 4 (q) or the cache's (k, v) out.
+// cache's type (halves and bf16 so in two steps, a 2^-13 or 2^-16 of a step more
+// than in one). Bound by HBM: 4 bytes in and 4 (q) or the cache's (k, v) out; 8000
+// rows of 64 + 8 heads of 64 into a bf16 cache 59 us (5.2 TB/s, beside 4.7 of a large
+// copy), 32 rows of 32 + 4 heads of 128 4.8 us (launch and two round trips).
 template <int T>
 __device__ __forceinline__ void paged_qkrope_t(const PagedRopeArgs& a)
 {
@@ -532,13 +545,11 @@ __device__ __forceinline__ float quad_sum(float v)
   return v + xpart<32>(v);
 }
 
-// what a block works on: keys [lo, hi) of a sequence, one KV head, 16 of its
-// query heads
+// what a block works on: a sequence, one of its KV heads, 16 of that one's query heads
 struct AttnItem {
-  int s, kv, tile;  // sequence, KV head, tile of its group
+  int s, kv;        // sequence, KV head
   int heads;        // query heads of the tile
   int head0;        // the first of them
-  int64_t lo, hi;   // the keys
 };
 
 template <int T, int D>
@@ -706,10 +717,16 @@ __device__ __forceinline__ void stage_query(const PagedAttnArgs& a, const AttnIt
 // registers. No key, value or weight goes through LDS, and the running maximum, sum
 // and rescale are a lane's own. Queries and weights enter as 2 half or 3 bf16
 // parts (f32 caches: the f32 matrix cores), so the sums are those of single.
-// HBM bound: the cache is read once. Heads beyond 256 give a wave half of the
+//
+// HBM bound: the cache is read once (again for each 16 query heads of a KV head
+// beyond 16). 64 sequences of 16384 keys, 8 KV heads of 128 in bf16 735 us, 5.8 TB/s
+// of the 6.2 that a streaming read takes; single 6.3, heads of 256 5.5, of 64 5.0 to
+// 5.8; few long sequences lose the join (three of 110000: 136 us, 5.0), one short one
+// is a chain of round trips (1152 keys 12.5 us). Pages of [kv_heads, page_size,
+// head_dim] read up to 6% faster than [page_size, kv_heads, head_dim]. Heads beyond 256 give a wave half of the
 // dimensions, two waves adding their shares of the scores in LDS, as the values of
 // 512 do not fit the registers beside the keys (one wave each, spilling: 16
-// sequences of 8192, 2 KV heads 252 us).
+// sequences of 8192, 2 KV heads 252 us, so 116).
 template <int T, int D, bool FULL>
 __device__ __forceinline__ void paged_attention_t(const PagedAttnArgs& a)
 {
@@ -785,11 +802,9 @@ __device__ __forceinline__ void paged_attention_t(const PagedAttnArgs& a)
     AttnItem it;
     it.s = seq;
     it.kv = item / a.tiles;
-    it.tile = item - it.kv * a.tiles;
-    it.heads = min(16, a.group - 16 * it.tile);
-    it.head0 = it.kv * a.group + 16 * it.tile;
-    it.lo = lo;
-    it.hi = hi;
+    const int tile16 = item - it.kv * a.tiles;
+    it.heads = min(16, a.group - 16 * tile16);
+    it.head0 = it.kv * a.group + 16 * tile16;
     const char* const kb = a.kc + (int64_t)it.kv * a.head_stride * S::ES;
     const char* const vb = a.vc + (int64_t)it.kv * a.head_stride * S::ES;
     const int* const table = a.table + (int64_t)seq * a.max_pages;

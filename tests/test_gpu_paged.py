@@ -124,6 +124,18 @@ def test_slots_default_count_and_edges(ctx, dev):
         assert (got["slots"] == -1).all()
 
 
+def test_slots_ring_turned_often(ctx, dev):
+    """Ends beyond 32 bits."""
+    rng = np.random.default_rng(10)
+    past, count, table, ring, ends = batch(rng, 40, 4, 30, 3, 50)
+    for turns in (2 ** 33, 2 ** 45 + 7):
+        e = ends + turns * len(ring)
+        want = R.slots(past, count, table, 4, ring, e, 120)
+        got = run_slots(ctx, dev, past, count, table, 4, ring, e, 120)
+        for k in want:
+            assert np.array_equal(got[k], want[k]), k
+
+
 def test_slots_captured(ctx, dev):
     """Decode steps replayed from one graph: lengths, pages and the ring go on from replay to
     replay, in place."""
