@@ -663,6 +663,15 @@ int ihip_enqueue_paged_attention(ihip_ctx* ctx, uint64_t q, int64_t q_stride,
                                  const ihip_pages* cache, uint64_t table, int64_t max_pages,
                                  uint64_t lengths, uint64_t y, int64_t seqs, int64_t heads,
                                  int64_t window, uint64_t sinks, double scale);
+/* the same for a batch whose rows are _paged_slots': offsets [seqs + 1], rows as
+ * given there; the query of sequence s is the last of its rows, offsets[s + 1] -
+ * 1, and so is its row of y. A sequence without a row (or with one beyond rows)
+ * is passed over. offsets 0: row s, as above. */
+int ihip_enqueue_paged_attention_at(ihip_ctx* ctx, uint64_t q, int64_t q_stride,
+                                    const ihip_pages* cache, uint64_t table, int64_t max_pages,
+                                    uint64_t lengths, uint64_t offsets, int64_t rows, uint64_t y,
+                                    int64_t seqs, int64_t heads, int64_t window, uint64_t sinks,
+                                    double scale);
 /* what a row of logits says of its tokens: logits [rows, vocab], `stride` floats
  * from a row to the next (0: vocab);
  * - logprobs [rows] (or 0): log softmax of token ids[r] (int32), NaN for an id

@@ -179,6 +179,15 @@ int ihip_enqueue_paged_attention(ihip_ctx* c, uint64_t q, int64_t q_stride, cons
                                  uint64_t table, int64_t max_pages, uint64_t lengths, uint64_t y,
                                  int64_t seqs, int64_t heads, int64_t window, uint64_t sinks, double scale)
 {
+  return ihip_enqueue_paged_attention_at(c, q, q_stride, cache, table, max_pages, lengths, 0, seqs, y, seqs, heads,
+                                         window, sinks, scale);
+}
+
+int ihip_enqueue_paged_attention_at(ihip_ctx* c, uint64_t q, int64_t q_stride, const ihip_pages* cache,
+                                    uint64_t table, int64_t max_pages, uint64_t lengths, uint64_t offsets,
+                                    int64_t rows, uint64_t y, int64_t seqs, int64_t heads, int64_t window,
+                                    uint64_t sinks, double scale)
+{
   const char* who = "ihip_enqueue_paged_attention";
   Pool p;
   if (int rc = check_pool(who, cache, &p)) return rc;
@@ -186,12 +195,12 @@ int ihip_enqueue_paged_attention(ihip_ctx* c, uint64_t q, int64_t q_stride, cons
   if (!q || !table || !lengths || !y) return refuse(who, "a missing array");
   if (seqs > IHIP_PAGED_SEQS) return refuse(who, "more sequences than IHIP_PAGED_SEQS", IHIP_E_NOMEM);
   if (seqs < 1 || heads < 1 || heads > 65535 || heads % kvh || window < 0 || max_pages < 1 ||
-      max_pages > INT32_MAX / cache->page_size)
-    return refuse(who, "seqs, heads, window or max_pages out of range");
+      max_pages > INT32_MAX / cache->page_size || rows < 1 || rows > INT32_MAX)
+    return refuse(who, "seqs, heads, window, max_pages or rows out of range");
   q_stride = q_stride ? q_stride : heads * hd;
   if (q_stride < heads * hd) return refuse(who, "a stride below a row");
   if (q_stride > STRIDE_MOST) return refuse(who, "a stride beyond 2^36");
-  if ((q | y | sinks | lengths | table) % 4) return refuse(who, "arrays aligned to 4 bytes");
+  if ((q | y | sinks | lengths | offsets | table) % 4) return refuse(who, "arrays aligned to 4 bytes");
   if (std::isnan(scale) || std::isinf(scale)) return refuse(who, "scale");
   // the kernels take tiles of 128 keys of 16-bit caches, 64 of single ones, half as
   // many of heads beyond 256
@@ -205,21 +214,21 @@ int ihip_enqueue_paged_attention(ihip_ctx* c, uint64_t q, int64_t q_stride, cons
   struct {
     const float* q;
     const char *kc, *vc;
-    const int *table, *lengths;
+    const int *table, *lengths, *offsets;
     float* y;
     const float* sinks;
     float* part;
     int* done;
     int64_t q_stride, pages, page_stride, slot_stride, head_stride, window;
     float scale;
-    int32_t seqs, heads, kvh, hd, page_size, max_pages, group, tiles;
+    int32_t seqs, heads, kvh, hd, page_size, max_pages, group, tiles, rows;
   } a = {(const float*)q, (const char*)cache->k, (const char*)cache->v, (const int*)table,
-         (const int*)lengths, (float*)y, (const float*)sinks, (float*)c->paged_part,
+         (const int*)lengths, (const int*)offsets, (float*)y, (const float*)sinks, (float*)c->paged_part,
          (int*)(c->paged_part + PAGED_PART_BYTES), q_stride, cache->pages, p.page_stride,
          p.slot_stride, p.head_stride, window,
          (float)((scale > 0 ? scale : 1.0 / std::sqrt((double)hd)) * 1.4426950408889634), (int32_t)seqs,
          (int32_t)heads, (int32_t)kvh, (int32_t)hd, cache->page_size, (int32_t)max_pages, (int32_t)group,
-         (int32_t)tiles};
+         (int32_t)tiles, (int32_t)rows};
   const int d = hd <= 64 ? 64 : hd <= 128 ? 128 : hd <= 256 ? 256 : 512;
   char name[40];
   snprintf(name, sizeof name, "paged_attention_%s_%d%s", p.type, d, hd == d ? "" : "_part");

@@ -467,6 +467,7 @@ struct PagedAttnArgs {
   const float* q;
   const char *kc, *vc;
   const int *table, *lengths;
+  const int* offsets;  // [seqs + 1]: a sequence's row of q and y is its last, offsets[s + 1] - 1; null: row s
   float* y;
   const float* sinks;
   float* part;  // [blocks][2][16 * hd + 32]: a block's pieces of sequences that other blocks share
@@ -475,6 +476,7 @@ struct PagedAttnArgs {
   float scale;  // of the scores, times log2 e
   int32_t seqs, heads, kvh, hd, page_size, max_pages;
   int32_t group, tiles;  // query heads of a KV head, in tiles of 16
+  int32_t rows;          // of q and y
 };
 
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
@@ -547,7 +549,7 @@ __device__ __forceinline__ float quad_sum(float v)
 
 // what a block works on: a sequence, one of its KV heads, 16 of that one's query heads
 struct AttnItem {
-  int s, kv;        // sequence, KV head
+  int s, row, kv;   // sequence, its row of q and y, KV head
   int heads;        // query heads of the tile
   int head0;        // the first of them
 };
@@ -599,7 +601,7 @@ __device__ __forceinline__ void paged_walk(const PagedAttnArgs& a, const AttnIte
 #pragma unroll
     for (int i = 0; i < NV; i++) {
       const int d = lane + 64 * i;
-      q[i] = d < a.hd ? a.q[it.s * a.q_stride + (int64_t)(it.head0 + h) * a.hd + d] * a.scale : 0.f;
+      q[i] = d < a.hd ? a.q[it.row * a.q_stride + (int64_t)(it.head0 + h) * a.hd + d] * a.scale : 0.f;
       acc[i] = 0.f;
     }
     float m = -__builtin_inff(), l = 0.f;
@@ -660,7 +662,7 @@ __device__ __forceinline__ void stage_query(const PagedAttnArgs& a, const AttnIt
 {
   using S = AttnShape<T, D>;
   const int t = threadIdx.x;
-  const float* const q = a.q + it.s * a.q_stride + (int64_t)it.head0 * a.hd;
+  const float* const q = a.q + it.row * a.q_stride + (int64_t)it.head0 * a.hd;
   if constexpr (T == 1) {
     const int c = t >> 4;
     float top = 0.f;
@@ -737,7 +739,15 @@ __device__ __forceinline__ void paged_attention_t(const PagedAttnArgs& a)
   const uint32_t grid = gridDim.x, b = blockIdx.x, per = a.kvh * a.tiles;
   const int hd = FULL ? D : a.hd, row_out = a.heads * a.hd;
 
+  // a sequence's row, -1 where it has none in this step
+  auto row_of = [&](int seq) {
+    if (!a.offsets) return seq;
+    const int r = a.offsets[seq + 1] - 1;
+    return r >= a.offsets[seq] && r < a.rows && r >= 0 ? r : -1;
+  };
   auto tiles_of = [&](int seq, int64_t& lo, int64_t& hi) {
+    lo = hi = 0;
+    if (row_of(seq) < 0) return 0u;
     paged_range(a.lengths[seq], a.window, a.max_pages, a.page_size, &lo, &hi);
     return (uint32_t)((hi - lo + S::TK - 1) / S::TK);
   };
@@ -752,11 +762,11 @@ __device__ __forceinline__ void paged_attention_t(const PagedAttnArgs& a)
       int64_t lo, hi;
       n = tiles_of(seq, lo, hi);
       if (s0 == 0) n0 = n, lo0 = lo, hi0 = hi;
-      zero = n == 0 && a.lengths[seq] >= 0 && (uint32_t)seq % grid == b;
+      zero = n == 0 && a.lengths[seq] >= 0 && row_of(seq) >= 0 && (uint32_t)seq % grid == b;
     }
     all += n * per;
     for (uint64_t z = __ballot(zero); z; z &= z - 1) {
-      float* const y = a.y + (int64_t)(s0 + __builtin_ctzll(z)) * row_out;
+      float* const y = a.y + (int64_t)row_of(s0 + __builtin_ctzll(z)) * row_out;
       for (int i = t; i < row_out; i += 256) y[i] = 0.f;
     }
   }
@@ -801,6 +811,7 @@ __device__ __forceinline__ void paged_attention_t(const PagedAttnArgs& a)
     const uint32_t tile1 = min(n, tile0 + (end - u));
     AttnItem it;
     it.s = seq;
+    it.row = row_of(seq);
     it.kv = item / a.tiles;
     const int tile16 = item - it.kv * a.tiles;
     it.heads = min(16, a.group - 16 * tile16);
@@ -1022,7 +1033,7 @@ __device__ __forceinline__ void paged_attention_t(const PagedAttnArgs& a)
     if (__syncthreads_or(odd))
       paged_walk<T, D>(a, it, lo + (int64_t)tile0 * S::TK, min(hi, lo + (int64_t)tile1 * S::TK), s);
 
-    float* const y = a.y + (int64_t)seq * row_out + (int64_t)it.head0 * a.hd;
+    float* const y = a.y + (int64_t)it.row * row_out + (int64_t)it.head0 * a.hd;
     // with the sink: its weight beside the sum's, both against the larger maximum
     auto finish = [&](int h, float m2, float l2, float& f2) {
       f2 = 1.f;

@@ -183,6 +183,9 @@ def lib():
                                                 C.POINTER(Pages), u64]),
             "ihip_enqueue_paged_attention": (i32, [vp, u64, i64, C.POINTER(Pages), u64, i64, u64,
                                                    u64, i64, i64, i64, u64, C.c_double]),
+            "ihip_enqueue_paged_attention_at": (i32, [vp, u64, i64, C.POINTER(Pages), u64, i64, u64,
+                                                      u64, i64, u64, i64, i64, i64, u64,
+                                                      C.c_double]),
             "ihip_enqueue_logprobs": (i32, [vp, u64, i64, i64, i64, u64, u64, u64, i64, u64, u64]),
             "ihip_synth_blocks": (i32, [vp, i32, i64, i64, u64, i32, i32, i32]),
             "ihip_synth_normal": (i32, [vp, i32, i64, i64, u64, C.c_float, i32]),

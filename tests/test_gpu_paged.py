@@ -627,3 +627,83 @@ def test_attention_shares_pages(ctx, dev):
 
     rng = np.random.default_rng(63)
     assert_close(*attention_case(ctx, dev, rng, "f16", 128, 8, 2, 16, [90, 60], change=change))
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+def test_attention_by_rows(ctx, dev, dtype):
+    """Sequences whose rows are a step's: the last row of each, none of an empty or ended place,
+    none beyond the rows there are."""
+    rng = np.random.default_rng(71)
+    n, heads, kvh, hd, ps, width, rows = 9, 8, 2, 128, 16, 12, 14
+    counts = np.array([1, 0, 3, 1, 0, 5, 2, 1, 4])  # the last ends beyond the rows
+    offsets = np.concatenate([[0], np.cumsum(counts)]).astype(np.int32)
+    lengths = np.array([40, 33, 0, 150, -1, 90, -1, 77, 60], np.int32)
+    pages = n * width
+    k, v = (R.pack(rng.standard_normal((pages, ps, kvh, hd)), dtype) for _ in range(2))
+    table = rng.permutation(pages).reshape(n, width).astype(np.int32)
+    q = rng.standard_normal((rows, heads, hd)).astype(np.float32)
+    pool = pages_struct(dev(k), dev(v), pages, ps, kvh, hd, dtype)
+    y = dev.out(q.nbytes)
+    H.check(H.lib().ihip_enqueue_paged_attention_at(
+        ctx.h, dev(q), 0, C.byref(pool), dev(table), width, dev(lengths), dev(offsets), rows, y.ptr, n, heads, 0, 0,
+        0.0))
+    got = y.download(np.float32, q.size).reshape(q.shape)
+    written = np.zeros(rows, bool)
+    for s in range(n):
+        r = offsets[s + 1] - 1
+        if counts[s] == 0 or r >= rows or lengths[s] < 0:
+            continue
+        written[r] = True
+        want, tol = R.attention(q[r:r + 1].astype(np.float64), R.unpack(k, dtype), R.unpack(v, dtype), table[s:s + 1],
+                                lengths[s:s + 1], ps)
+        assert_close(got[r], want[0], tol[0])
+    assert written.tolist() == [i in (0, 3, 4, 9, 12) for i in range(rows)]
+    assert (got[~written].view(np.uint8) == 0x5A).all()
+
+
+def test_decode_steps_by_rows(ctx, dev):
+    """Replayed steps of a batch with empty places: each sequence's query is its own row of the
+    step, its output there too, against a host model that keeps every sequence's keys apart."""
+    hd, heads, kvh, ps, width, n, pages = 64, 4, 2, 4, 12, 6, 60
+    rng = np.random.default_rng(81)
+    past = np.array([0, -1, 0, 0, -1, 0], np.int32)
+    row = (heads + 2 * kvh) * hd
+    b = {}
+    for name, a in dict(past=past, count=np.zeros(n, np.int32), table=np.full((n, width), -1, np.int32),
+                        ring=rng.permutation(pages).astype(np.int32), ends=np.array([0, pages], np.int64)).items():
+        b[name] = dev.out(a.nbytes)
+        b[name].upload(a)
+    kc, vc = dev.out(pages * ps * kvh * hd * 4, 0xFF), dev.out(pages * ps * kvh * hd * 4, 0xFF)
+    pool = pages_struct(kc.ptr, vc.ptr, pages, ps, kvh, hd, "f32")
+    x, y = dev.out(n * row * 4), dev.out(n * heads * hd * 4)
+    offs, pos, slots, failed = (dev.out(4 * m) for m in (n + 1, n, n, 1))
+    H.check(H.lib().ihip_capture_begin(ctx.h))
+    H.check(H.lib().ihip_enqueue_paged_slots(
+        ctx.h, b["past"].ptr, b["count"].ptr, n, b["table"].ptr, width, ps, b["ring"].ptr, pages, b["ends"].ptr,
+        b["ends"].ptr, offs.ptr, b["past"].ptr, pos.ptr, slots.ptr, n, failed.ptr))
+    H.check(H.lib().ihip_enqueue_paged_qkrope(
+        ctx.h, x.ptr, row, x.ptr + 4 * heads * hd, row, x.ptr + 4 * (heads + kvh) * hd, row, n, heads, 0, 0, 0.0, None,
+        pos.ptr, slots.ptr, C.byref(pool), 0))
+    H.check(H.lib().ihip_enqueue_paged_attention_at(
+        ctx.h, x.ptr, row, C.byref(pool), b["table"].ptr, width, b["past"].ptr, offs.ptr, n, y.ptr, n, heads, 0, 0, 0.0))
+    H.check(H.lib().ihip_capture_end(ctx.h, 12))
+    keys = {s: ([], []) for s in range(n) if past[s] >= 0}
+    for step in range(20):
+        count = np.array([1, 1, step % 2, 1, 1, -1 if step == 11 else 1], np.int32)
+        data = rng.standard_normal((n, row)).astype(np.float32)
+        b["count"].upload(count), x.upload(data)
+        H.check(H.lib().ihip_graph_launch(ctx.h, 12))
+        if step == 11:
+            del keys[5]
+        got = y.download(np.float32, n * heads * hd).reshape(n, heads, hd)
+        assert failed.download(np.int32, 1)[0] == 0
+        r = 0
+        for s in sorted(keys):
+            if not count[s]:
+                continue
+            q, kk, vv = np.split(data[r].reshape(-1, hd), (heads, heads + kvh))
+            keys[s][0].append(kk), keys[s][1].append(vv)
+            k64, v64 = (np.array(a).astype(np.float64)[None] for a in keys[s])
+            want, tol = R.attention(q[None].astype(np.float64), k64, v64, np.array([[0]]), [k64.shape[1]], k64.shape[1])
+            assert_close(got[r], want[0], tol[0])
+            r += 1

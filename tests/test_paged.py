@@ -87,6 +87,20 @@ def test_attention_refused():
     refused(lambda: attention(pages(slot_stride=64, head_stride=1024)), -1, "no context")
 
 
+def test_attention_at_refused():
+    def call(**kw):
+        a = dict(q=A, qs=0, pool=C.byref(pages()), table=A, mp=4, lengths=A, offsets=A, rows=5, y=A, seqs=3,
+                 heads=4, window=0, sinks=0, scale=0.0)
+        a.update(kw)
+        return H.lib().ihip_enqueue_paged_attention_at(None, *a.values())
+
+    for bad in (dict(rows=0), dict(rows=-1), dict(rows=1 << 31), dict(seqs=0)):
+        refused(lambda: call(**bad), -1, "out of range")
+    refused(lambda: call(offsets=A + 1), -1, "aligned")
+    refused(lambda: call(lengths=0), -1, "missing array")
+    refused(lambda: call(), -1, "no context")
+
+
 def test_qkrope_refused():
     refused(lambda: qkrope(None), -1, "no cache")
     for name in ("q", "k", "v", "positions", "slots"):
