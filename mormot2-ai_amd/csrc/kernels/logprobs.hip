@@ -127,6 +127,9 @@ __device__ __forceinline__ uint32_t kth_of_lanes(uint32_t v, int k)
   return t ? max(t, ORDER_LEAST) : 0;
 }
 
+constexpr float LOWEST = -3.40282347e38f;
+constexpr float LOG2E = 1.44269504088896340736f;
+
 // a thread's sums (m their maximum): sum of e^(x - m) and of (x - m) e^(x - m)
 struct Sums {
   float m;
@@ -134,7 +137,11 @@ struct Sums {
   __device__ __forceinline__ void rescale(float m2)
   {
     if (m2 == m) return;
-    const double d = (double)m - (double)m2, f = exp(d);
+    // the factor in single: its error is that of the sums so far alone, U (2 + |d|) of
+    // what e^d leaves of them (a double exponential was a fifth of a short part's
+    // instructions)
+    const double d = (double)m - (double)m2;
+    const double f = (double)__builtin_amdgcn_exp2f((m - m2) * LOG2E);
     w = f * (w + (s > 0 ? d * s : 0.0));
     s = f * s;
     m = m2;
@@ -148,8 +155,6 @@ struct Sums {
   }
 };
 
-constexpr float LOWEST = -3.40282347e38f;
-constexpr float LOG2E = 1.44269504088896340736f;
 constexpr int TILE = 1024;  // a wave's logits of one step, 16 a lane
 
 // A block takes a row, or one of `parts` of a row where the rows do not fill the
