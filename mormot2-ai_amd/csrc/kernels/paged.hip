@@ -725,10 +725,10 @@ __device__ __forceinline__ void stage_query(const PagedAttnArgs& a, const AttnIt
 // of the 6.2 that a streaming read takes; single 6.3, heads of 256 5.5, of 64 5.0 to
 // 5.8; few long sequences lose the join (three of 110000: 136 us, 5.0), one short one
 // is a chain of round trips (1152 keys 12.5 us). Pages of [kv_heads, page_size,
-// head_dim] read up to 6% faster than [page_size, kv_heads, head_dim]. Heads beyond 256 give a wave half of the
-// dimensions, two waves adding their shares of the scores in LDS, as the values of
-// 512 do not fit the registers beside the keys (one wave each, spilling: 16
-// sequences of 8192, 2 KV heads 252 us, so 116).
+// head_dim] read up to 6% faster than [page_size, kv_heads, head_dim]. Heads
+// beyond 256 give a wave half of the dimensions, two waves adding their shares of the
+// scores in LDS, as the values of 512 do not fit the registers beside the keys (one
+// wave each, spilling: 16 sequences of 8192, 2 KV heads 252 us, so 116).
 template <int T, int D, bool FULL>
 __device__ __forceinline__ void paged_attention_t(const PagedAttnArgs& a)
 {
@@ -821,10 +821,11 @@ __device__ __forceinline__ void paged_attention_t(const PagedAttnArgs& a)
     const int* const table = a.table + (int64_t)seq * a.max_pages;
     const int kg = w / S::DS, dh = w % S::DS;  // the wave's keys of a tile, its dimensions
     const int64_t wlo = lo + kg * S::KS;
+    const int64_t jend = min(hi, lo + (int64_t)tile1 * S::TK);  // the piece's keys end here
     // a step's key of this lane: its page's table entry
     auto entry = [&](uint32_t tile) {
       const int64_t j = wlo + (int64_t)tile * S::TK + (lane & (S::KS - 1));
-      return j < hi ? table[(uint32_t)j / (uint32_t)a.page_size] : -1;
+      return j < jend ? table[(uint32_t)j / (uint32_t)a.page_size] : -1;
     };
     // the offsets of a step's keys into LDS, the keys that are there as bits
     auto locate = [&](uint32_t tile, int page) {
@@ -871,8 +872,8 @@ __device__ __forceinline__ void paged_attention_t(const PagedAttnArgs& a)
       steps = min(tile1, mine) - tile0;
     }
     // The loop has no branch between a product and what reads it, so keys are
-    // located and loaded one step past the last too: entry() has no page there and
-    // the loads read the pool's first row.
+    // located and loaded one step past the piece's last too: entry() has no page there
+    // and the loads read the pool's first row.
     uint32_t there = locate(tile, page0);
     if (steps) load_keys(tile);
     for (uint32_t i = 0; i < steps; i++, tile++) {
