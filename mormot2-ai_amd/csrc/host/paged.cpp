@@ -221,14 +221,14 @@ int ihip_enqueue_paged_attention_at(ihip_ctx* c, uint64_t q, int64_t q_stride, c
     int* done;
     int64_t q_stride, pages, page_stride, slot_stride, head_stride, window;
     float scale;
-    int32_t seqs, heads, kvh, hd, page_size, max_pages, group, tiles, rows;
+    int32_t seqs, heads, kvh, hd, page_size, max_pages, group, tiles, rows, cus;
   } a = {(const float*)q, (const char*)cache->k, (const char*)cache->v, (const int*)table,
          (const int*)lengths, (const int*)offsets, (float*)y, (const float*)sinks, (float*)c->paged_part,
          (int*)(c->paged_part + PAGED_PART_BYTES), q_stride, cache->pages, p.page_stride,
          p.slot_stride, p.head_stride, window,
          (float)((scale > 0 ? scale : 1.0 / std::sqrt((double)hd)) * 1.4426950408889634), (int32_t)seqs,
          (int32_t)heads, (int32_t)kvh, (int32_t)hd, cache->page_size, (int32_t)max_pages, (int32_t)group,
-         (int32_t)tiles, (int32_t)rows};
+         (int32_t)tiles, (int32_t)rows, c->cus};
   const int d = hd <= 64 ? 64 : hd <= 128 ? 128 : hd <= 256 ? 256 : 512;
   char name[40];
   snprintf(name, sizeof name, "paged_attention_%s_%d%s", p.type, d, hd == d ? "" : "_part");

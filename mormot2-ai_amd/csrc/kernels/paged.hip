@@ -477,6 +477,7 @@ struct PagedAttnArgs {
   int32_t seqs, heads, kvh, hd, page_size, max_pages;
   int32_t group, tiles;  // query heads of a KV head, in tiles of 16
   int32_t rows;          // of q and y
+  int32_t cus;
 };
 
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
@@ -752,7 +753,7 @@ __device__ __forceinline__ void paged_attention_t(const PagedAttnArgs& a)
     return (uint32_t)((hi - lo + S::TK - 1) / S::TK);
   };
   // all tiles (each wave for itself); rows without a key are zeros
-  uint32_t all = 0, n0 = 0;
+  uint32_t all = 0, n0 = 0, live = 0;  // tiles, those of the lane's first sequence; sequences with any
   int64_t lo0 = 0, hi0 = 0;  // of the first 64 sequences, a lane each
   for (int s0 = 0; s0 < a.seqs; s0 += 64) {
     const int seq = s0 + lane;
@@ -765,14 +766,19 @@ __device__ __forceinline__ void paged_attention_t(const PagedAttnArgs& a)
       zero = n == 0 && a.lengths[seq] >= 0 && row_of(seq) >= 0 && (uint32_t)seq % grid == b;
     }
     all += n * per;
+    live += __popcll(__ballot(n != 0));
     for (uint64_t z = __ballot(zero); z; z &= z - 1) {
       float* const y = a.y + (int64_t)row_of(s0 + __builtin_ctzll(z)) * row_out;
       for (int i = t; i < row_out; i += 256) y[i] = 0.f;
     }
   }
   all = __builtin_amdgcn_readfirstlane(wave_sum(all, 64));
-  // block i of those with a tile takes tiles first(i) .. first(i + 1) - 1
-  const uint32_t B = min(grid, all);
+  // Block i of B takes tiles first(i) .. first(i + 1) - 1. One block a CU where the
+  // blocks have 32 tiles and more and the items 24 (their streams then cover each
+  // other's latencies: 64 sequences of 8192, 8 KV heads of 64, two blocks a CU 222 us,
+  // one 196; 16384 of 128 731, 718; of 200 sequences up to 4000, 16 tiles an item, the
+  // starts and ends of pieces need the second block: 301, one 313), else all.
+  const uint32_t B = all >= 32 * grid && all / 24 >= live * per ? min(grid, (uint32_t)a.cus) : min(grid, all);
   if (b >= B) return;
   const uint32_t quot = all / B, rem = all % B;
   auto first = [&](uint32_t i) { return i * quot + i * rem / B; };

@@ -340,6 +340,13 @@ def test_attention_split_over_the_length(ctx, dev, dtype, hd, heads, kvh, ps, le
     assert_close(*attention_case(ctx, dev, rng, dtype, hd, heads, kvh, ps, lengths))
 
 
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+def test_attention_with_long_streams(ctx, dev, dtype):
+    """Tiles enough for one block a CU, a block's pieces of several heads and sequences."""
+    rng = np.random.default_rng(17)
+    assert_close(*attention_case(ctx, dev, rng, dtype, 8, 64, 64, 64, [8300, 8192, 0, 8400, 8250, 30]))
+
+
 @pytest.mark.parametrize("dtype", ["f16", "bf16", "f32"])
 def test_attention_large_scores_and_queries(ctx, dev, dtype):
     """Scores far apart, a query of tiny and one of huge values, equal keys."""
