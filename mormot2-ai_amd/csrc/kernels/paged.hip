@@ -570,7 +570,7 @@ struct AttnShape {
   static constexpr int VL = T != 0 && D > 64 ? 8 : 4;  // values of a value load
   static constexpr int NJ = DW / (16 * VL);            // value loads of a lane and key
   static constexpr int OS = D + 4;                     // a head's row in o_s
-  static constexpr float P0 = T == 1 ? 15.f : 0.f;     // weights times 2^P0: halves' normal range
+  static constexpr float PS = T == 1 ? 32768.f : 1.f;  // weights enter the product times this: halves' normal range
 };
 
 template <int T, int D>
@@ -964,7 +964,7 @@ __device__ __forceinline__ void paged_attention_t(const PagedAttnArgs& a)
 #pragma unroll
           for (int e = 0; e < S::VL; e++) o[j][e] *= f;
       }
-      const float shift = (m == -__builtin_inff() ? 0.f : m) - S::P0;
+      const float shift = m == -__builtin_inff() ? 0.f : m;
       float p[NV];
 #pragma unroll
       for (int k = 0; k < NV; k++) {
@@ -982,7 +982,7 @@ __device__ __forceinline__ void paged_attention_t(const PagedAttnArgs& a)
       } else {
         uint32_t part[4][S::NP];
 #pragma unroll
-        for (int k = 0; k < 4; k++) split2<T>(p[2 * k], p[2 * k + 1], part[k]);
+        for (int k = 0; k < 4; k++) split2<T>(p[2 * k] * S::PS, p[2 * k + 1] * S::PS, part[k]);
 #pragma unroll
         for (int j = 0; j < S::NJ; j++)
 #pragma unroll
@@ -1009,12 +1009,12 @@ __device__ __forceinline__ void paged_attention_t(const PagedAttnArgs& a)
 #pragma unroll
     for (int i = 1; i < S::KG; i++) M = fmaxf(M, s.wm[i][c]);
     const float Ms = M == -__builtin_inff() ? 0.f : M;
-    const float f = exp2_fast(m - Ms - S::P0);
+    const float f = exp2_fast(m - Ms) * (1.f / S::PS);
     bool odd = false;
     if (w == 0 && g == 0) {
       float L = 0.f;
 #pragma unroll
-      for (int i = 0; i < S::KG; i++) L += s.wl[i][c] * exp2_fast(s.wm[i][c] - Ms - S::P0);
+      for (int i = 0; i < S::KG; i++) L += s.wl[i][c] * exp2_fast(s.wm[i][c] - Ms);
       s.m[c] = M;
       s.l[c] = L;
       odd = c < it.heads && !finite(L);
