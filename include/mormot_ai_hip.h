@@ -638,11 +638,11 @@ int ihip_enqueue_paged_slots(ihip_ctx* ctx, uint64_t past, uint64_t count, int64
                              int64_t pages, uint64_t ends, uint64_t ends_out, uint64_t offsets,
                              uint64_t lengths, uint64_t positions, uint64_t slots, int64_t rows,
                              uint64_t failed);
-/* the new rows' q, k and v between the q/k/v Linear and the attention: per row
- * and head the RMSNorm of q and k heads (qn, kn device [head_dim] or 0), rotary
- * positions (rope, NULL: none), q written to q_out ([rows, heads, head_dim], or 0:
- * in place; elsewhere it does not overlap q), k and v stored into the cache at
- * the row's slot. Strides: floats from a row to the next (0: the rows are
+/* the new rows' (up to 2^23) q, k and v between the q/k/v Linear and the
+ * attention: per row and head the RMSNorm of q and k heads (qn, kn device
+ * [head_dim] or 0), rotary positions (rope, NULL: none), q written to q_out
+ * ([rows, heads, head_dim], or 0: in place; elsewhere it does not overlap q), k
+ * and v stored into the cache at the row's slot. Strides: floats from a row to the next (0: the rows are
  * contiguous). A row with position < 0 is left as it was; a slot outside the
  * pool stores nothing. The rows of one call have slots of their own: of two in
  * one slot either may stay, value by value. (ihip_enqueue_qkrope over a paged
@@ -658,7 +658,8 @@ int ihip_enqueue_paged_qkrope(ihip_ctx* ctx, uint64_t q, int64_t q_stride, uint6
  * head_dim)); table [seqs, max_pages], q rows of q_stride floats (0: heads *
  * head_dim). A key whose table entry is outside the pool is not there, one whose
  * score is -infinity has weight 0. A sequence with no key (length 0) gives
- * zeros, one with lengths[s] < 0 leaves its row of y as it was. (ihip_enqueue_attention over a paged cache) */
+ * zeros, one with lengths[s] < 0 leaves its row of y as it was.
+ * (ihip_enqueue_attention over a paged cache) */
 int ihip_enqueue_paged_attention(ihip_ctx* ctx, uint64_t q, int64_t q_stride,
                                  const ihip_pages* cache, uint64_t table, int64_t max_pages,
                                  uint64_t lengths, uint64_t y, int64_t seqs, int64_t heads,
@@ -672,8 +673,8 @@ int ihip_enqueue_paged_attention_at(ihip_ctx* ctx, uint64_t q, int64_t q_stride,
                                     uint64_t lengths, uint64_t offsets, int64_t rows, uint64_t y,
                                     int64_t seqs, int64_t heads, int64_t window, uint64_t sinks,
                                     double scale);
-/* what a row of logits says of its tokens: logits [rows, vocab], `stride` floats
- * from a row to the next (0: vocab);
+/* what a row of logits says of its tokens: logits [rows, vocab] (vocab up to
+ * 2^22, rows to 2^24), `stride` floats from a row to the next (0: vocab);
  * - logprobs [rows] (or 0): log softmax of token ids[r] (int32), NaN for an id
  *   outside the vocabulary;
  * - entropy [rows] (or 0): of the softmax, in nats;
