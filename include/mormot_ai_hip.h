@@ -666,8 +666,8 @@ int ihip_enqueue_paged_attention(ihip_ctx* ctx, uint64_t q, int64_t q_stride,
                                  int64_t window, uint64_t sinks, double scale);
 /* the same for a batch whose rows are _paged_slots': offsets [seqs + 1], rows as
  * given there; the query of sequence s is the last of its rows, offsets[s + 1] -
- * 1, and so is its row of y. A sequence without a row (or with one beyond rows)
- * is passed over. offsets 0: row s, as above. */
+ * 1, and so is its row of y. offsets 0: row s. A sequence without a row, or whose
+ * row is not below `rows`, is passed over: neither q nor y is touched there. */
 int ihip_enqueue_paged_attention_at(ihip_ctx* ctx, uint64_t q, int64_t q_stride,
                                     const ihip_pages* cache, uint64_t table, int64_t max_pages,
                                     uint64_t lengths, uint64_t offsets, int64_t rows, uint64_t y,

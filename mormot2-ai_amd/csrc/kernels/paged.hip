@@ -467,7 +467,7 @@ struct PagedAttnArgs {
   const float* q;
   const char *kc, *vc;
   const int *table, *lengths;
-  const int* offsets;  // [seqs + 1]: a sequence's row of q and y is its last, offsets[s + 1] - 1; null: row s
+  const int* offsets;  // [seqs + 1]: a sequence's row of q and y is its last, offsets[s + 1] - 1; null: row s (both below rows)
   float* y;
   const float* sinks;
   float* part;  // [blocks][2][16 * hd + 32]: a block's pieces of sequences that other blocks share
@@ -742,9 +742,7 @@ __device__ __forceinline__ void paged_attention_t(const PagedAttnArgs& a)
 
   // a sequence's row, -1 where it has none in this step
   auto row_of = [&](int seq) {
-    if (!a.offsets) return seq;
-    const int r = a.offsets[seq + 1] - 1;
-    return r >= a.offsets[seq] && r < a.rows && r >= 0 ? r : -1;
+    return a.offsets ? paged_row(a.offsets[seq], a.offsets[seq + 1], a.rows) : paged_row(seq, seq + 1, a.rows);
   };
   auto tiles_of = [&](int seq, int64_t& lo, int64_t& hi) {
     lo = hi = 0;

@@ -22,6 +22,13 @@ IHIP_HD void paged_range(int32_t length, int64_t window, int64_t max_pages, int3
   *lo = window > 0 && n > window ? n - window : 0;
 }
 
+// the row of q and y of a sequence whose rows of the step are [first, end): the
+// last of them, or -1 where it has none or its last is not among the `rows`
+IHIP_HD int32_t paged_row(int32_t first, int32_t end, int32_t rows)
+{
+  return end > first && end >= 1 && end <= rows ? end - 1 : -1;
+}
+
 // the first value of token `at` of page `page`, in values from the pool's start
 // (of KV head 0), or -1 where the page is outside the pool
 IHIP_HD int64_t paged_value(int32_t page, int32_t at, int64_t pages, int64_t page_stride,

@@ -19,3 +19,5 @@ int64_t orc_paged_slot_value(int32_t slot, int32_t page_size, int64_t pages, int
 {
   return paged_slot_value(slot, page_size, pages, page_stride, slot_stride);
 }
+
+int32_t orc_paged_row(int32_t first, int32_t end, int32_t rows) { return paged_row(first, end, rows); }

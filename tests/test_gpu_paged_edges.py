@@ -1,0 +1,68 @@
+"""The paged operators on the device at the edges of what a call may hold,
+against paged_ref.py's definitions in 64 bits."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+import infer_hip as H
+import paged_ref as R
+from test_gpu_paged import assert_close, ctx, dev, pages_struct  # noqa: F401 (fixtures)
+
+pytestmark = pytest.mark.gpu
+
+
+# ----------------------------------------------------------------- attention
+class Batch:
+    """Keys, values, tables and queries of a batch, by default of full pages of its own each."""
+
+    def __init__(self, rng, dtype, hd, heads, kvh, ps, lengths, width=None):
+        self.dtype, self.hd, self.heads, self.kvh, self.ps = dtype, hd, heads, kvh, ps
+        self.lengths = np.array(lengths, np.int32)
+        n = len(lengths)
+        self.width = width or max(1, int(-(-self.lengths.clip(0) // ps).max()))
+        self.pages = n * self.width
+        self.table = rng.permutation(self.pages).reshape(n, self.width).astype(np.int32)
+        self.k, self.v = (rng.standard_normal((self.pages, ps, kvh, hd)) for _ in range(2))
+        self.q = rng.standard_normal((n, heads, hd)).astype(np.float32)
+        self.sinks, self.window, self.scale = None, 0, 0.0
+
+    def upload(self, dev):
+        self.raw = [R.pack(a, self.dtype) for a in (self.k, self.v)]
+        self.pool = pages_struct(dev(self.raw[0]), dev(self.raw[1]), self.pages, self.ps, self.kvh, self.hd, self.dtype)
+        self.dq, self.dt, self.dl = dev(self.q), dev(self.table), dev(self.lengths)
+        self.ds = dev(self.sinks) if self.sinks is not None else 0
+        self.y = dev.out(self.q.nbytes)
+
+    def enqueue(self, ctx):
+        H.check(H.lib().ihip_enqueue_paged_attention(
+            ctx.h, self.dq, 0, C.byref(self.pool), self.dt, self.width, self.dl, self.y.ptr, len(self.lengths),
+            self.heads, self.window, self.ds, self.scale), "attention")
+
+    def read(self):
+        return self.y.download(np.float32, self.q.size).reshape(self.q.shape)
+
+    def want(self):
+        with np.errstate(invalid="ignore", over="ignore"):
+            return R.attention(self.q.astype(np.float64), R.unpack(self.raw[0], self.dtype),
+                               R.unpack(self.raw[1], self.dtype), self.table, self.lengths, self.ps, self.window,
+                               self.sinks, self.scale)
+
+    def run(self, ctx, dev):
+        self.upload(dev)
+        self.enqueue(ctx)
+        return self.read()
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("rows", [1, 3, 5, 9])
+def test_attention_by_rows_without_offsets(ctx, dev, dtype, rows):
+    """Row s of sequence s where q and y have one; the other sequences are passed over."""
+    rng = np.random.default_rng(rows)
+    b = Batch(rng, dtype, 64, 4, 2, 16, [40, 0, 33, 1, 70])
+    b.upload(dev)
+    H.check(H.lib().ihip_enqueue_paged_attention_at(
+        ctx.h, b.dq, 0, C.byref(b.pool), b.dt, b.width, b.dl, 0, rows, b.y.ptr, 5, b.heads, 0, 0, 0.0), "attention")
+    got, (want, tol) = b.read(), b.want()
+    assert_close(got[:rows], want[:rows], tol[:rows])
+    assert (got[rows:].view(np.uint8) == 0x5A).all()

@@ -1,0 +1,30 @@
+"""The paged operators on the host (no device), at the edges of what a call may
+hold: rows beyond the step's, refusals."""
+import ctypes as C
+
+import pytest
+
+import oracle_lib as O
+
+
+def row(first, end, rows):
+    f = O.lib().orc_paged_row
+    f.restype = C.c_int32
+    f.argtypes = [C.c_int32, C.c_int32, C.c_int32]
+    return f(first, end, rows)
+
+
+@pytest.mark.parametrize("rows", [1, 2, 7, 2 ** 31 - 1])
+def test_rows_stay_in_the_step(rows):
+    """A sequence's row is the last of its own, and never one that the arrays do not have."""
+    low, high = -2 ** 31, 2 ** 31 - 1
+    for first in (low, -1, 0, 1, 5, 6, high - 1, high):
+        for end in (low, -1, 0, 1, 2, 6, 7, 8, high):
+            r = row(first, end, rows)
+            assert r == (end - 1 if end > first and 1 <= end <= rows else -1), (first, end)
+            assert -1 <= r < rows
+
+
+def test_rows_without_offsets():
+    """Row s of sequence s, where there is one."""
+    assert [row(s, s + 1, 3) for s in range(6)] == [0, 1, 2, -1, -1, -1]
