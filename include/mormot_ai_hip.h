@@ -657,8 +657,9 @@ int ihip_enqueue_paged_qkrope(ihip_ctx* ctx, uint64_t q, int64_t q_stride, uint6
  * the last `window` of them; sinks: device [heads] or 0; scale 0: 1 / sqrt(
  * head_dim)); table [seqs, max_pages], q rows of q_stride floats (0: heads *
  * head_dim). A key whose table entry is outside the pool is not there, one whose
- * score is -infinity has weight 0. A sequence with no key (length 0) gives
- * zeros, one with lengths[s] < 0 leaves its row of y as it was.
+ * score is -infinity has weight 0, and so has a sink of -infinity. A sequence with
+ * no key (length 0), or whose keys have no weight, gives zeros, one with lengths[s]
+ * < 0 leaves its row of y as it was.
  * (ihip_enqueue_attention over a paged cache) */
 int ihip_enqueue_paged_attention(ihip_ctx* ctx, uint64_t q, int64_t q_stride,
                                  const ihip_pages* cache, uint64_t table, int64_t max_pages,

@@ -1047,7 +1047,7 @@ __device__ __forceinline__ void paged_attention_t(const PagedAttnArgs& a)
         if (sk > m2) {
           f2 = exp2_fast(m2 - sk);
           l2 = l2 * f2 + 1.f;
-        } else {
+        } else if (sk != -__builtin_inff()) {  // (switched off: no weight, where no key has one either)
           l2 += exp2_fast(sk - m2);
         }
       }

@@ -66,3 +66,29 @@ def test_attention_by_rows_without_offsets(ctx, dev, dtype, rows):
     got, (want, tol) = b.read(), b.want()
     assert_close(got[:rows], want[:rows], tol[:rows])
     assert (got[rows:].view(np.uint8) == 0x5A).all()
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("off", [-np.inf, np.finfo(np.float32).min])
+def test_attention_sinks_switched_off(ctx, dev, dtype, off):
+    """A sink of -infinity, or one that its scaling makes so, has no weight: sequences whose keys are
+    none, all outside the pool, or all of score -infinity (in one piece, and split over the length)
+    give zeros, the others what they give without a sink."""
+    rng = np.random.default_rng(11)
+    b = Batch(rng, dtype, 128, 8, 2, 16, [50, 0, 64, 9000, 9000, 200])
+    b.table[0, :] = -1
+    b.table[4, :] = b.pages + 3
+    b.q = np.abs(b.q)
+    for s in (2, 3):  # scores of -infinity, whatever the query
+        b.k[b.table[s], :, :, 5] = -np.inf
+    b.sinks = rng.standard_normal(8).astype(np.float32)
+    b.sinks[[0, 3, 5]] = off
+    got, (want, tol) = b.run(ctx, dev), (None, None)
+    assert (got[:5] == 0).all(), np.isnan(got[:5]).sum((1, 2))
+    want, tol = b.want()
+    assert_close(got[5], want[5], tol[5])
+    b.sinks[1], b.sinks[4] = np.nan, np.inf
+    got = b.run(ctx, dev)
+    assert np.isnan(got[5, 1]).all() and (got[5, 4] == 0).all()
+    others = [0, 2, 3, 5, 6, 7]
+    assert_close(got[5][others], want[5][others], tol[5][others])
