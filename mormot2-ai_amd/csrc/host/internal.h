@@ -103,7 +103,7 @@ struct ihip_ctx {
   uint64_t scratch_split = 0, scratch_split_bytes = 0;  // split sums of the float-weight GEMM
   uint64_t scratch_argmax = 0;  // [ARGMAX_PARTS] block results of argmax_part
   uint64_t scratch_attn = 0, scratch_attn_bytes = 0;
-  uint64_t paged_plan = 0;  // the step plan between ihip_enqueue_paged_slots' two launches
+  uint64_t paged_plan = 0;  // the step plan between ihip_enqueue_paged_slots' two launches, a counter behind it
   uint64_t paged_part = 0;  // paged_attention's shared pieces and counters (zero between launches)
   uint64_t logprobs_part = 0;  // the same of ihip_enqueue_logprobs
   uint64_t scratch_planes = 0, scratch_planes_bytes = 0;  // e4m3 activation planes (gemm_mxfp4_f8)
@@ -162,7 +162,7 @@ constexpr uint64_t PAGED_PART_BYTES = 17u << 20;
 // doubles and IHIP_LOGPROBS_TOP alternatives each), and a counter of 32 bytes a row
 constexpr int64_t LOGPROBS_BLOCKS = 1024;
 constexpr uint64_t LOGPROBS_PART_BYTES = LOGPROBS_BLOCKS * (3 + IHIP_LOGPROBS_TOP) * 8;
-constexpr uint64_t PAGED_PLAN_BYTES = (5 * IHIP_PAGED_SEQS + 4) * 4;
+constexpr uint64_t PAGED_PLAN_BYTES = (5 * IHIP_PAGED_SEQS + 8) * 4;
 
 struct LinearCall {
   uint64_t x = 0;      // float activations [rows, in]

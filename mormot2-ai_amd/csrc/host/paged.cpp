@@ -96,11 +96,11 @@ int ihip_enqueue_paged_slots(ihip_ctx* c, uint64_t past, uint64_t count, int64_t
     const int64_t* ends;
     int64_t* ends_out;
     int *offsets, *lengths, *positions, *slots, *failed;
-    int* plan;
+    int *plan, *meet;
     int32_t seqs, max_pages, page_size, pages, rows, here;
   } a = {(const int*)past, (const int*)count, (int*)table, (int*)ring, (const int64_t*)ends,
          (int64_t*)ends_out, (int*)offsets, (int*)lengths, (int*)positions, (int*)slots, (int*)failed,
-         (int*)c->paged_plan, (int32_t)seqs, (int32_t)max_pages, (int32_t)page_size, (int32_t)pages,
+         (int*)c->paged_plan, (int*)(c->paged_plan + PAGED_PLAN_BYTES), (int32_t)seqs, (int32_t)max_pages, (int32_t)page_size, (int32_t)pages,
          (int32_t)rows, rows <= PAGED_ROWS_HERE};
   const size_t shmem = (size_t)seqs * 5 * 4;
   // a thread for the kernel's sequences, and where this block writes the rows one for
@@ -109,7 +109,7 @@ int ihip_enqueue_paged_slots(ihip_ctx* c, uint64_t past, uint64_t count, int64_t
   const int64_t threads = std::max<int64_t>((seqs + per - 1) / per, a.here ? std::min<int64_t>(rows + 64, 1024) : 256);
   int rc = launch(c, per == 1 ? "paged_slots_1" : "paged_slots_4", dim3(1), dim3((unsigned)((threads + 63) / 64 * 64)), &a, shmem);
   if (rc || a.here) return rc;
-  return launch(c, "paged_slots_rows", dim3((unsigned)std::min<int64_t>(4 * c->cus, (rows + 1023) / 1024)),
+  return launch(c, "paged_slots_rows", dim3(2 * (unsigned)std::min<int64_t>(4 * c->cus, (rows + 1023) / 1024)),
                 dim3(256), &a, shmem);
 }
 

@@ -216,14 +216,9 @@ int ihip_create(int device, ihip_ctx** out)
     return fail(IHIP_E_NOMEM, "hipMalloc");
   }
   c->scratch_argmax = (uint64_t)am;
-  void* plan = nullptr;
-  if (hipMalloc(&plan, PAGED_PLAN_BYTES) != hipSuccess) {
-    ihip_destroy(c);
-    return fail(IHIP_E_NOMEM, "hipMalloc");
-  }
-  c->paged_plan = (uint64_t)plan;
   // fixed, so that a captured call holds an address that stays; the counters behind zeroed
-  for (auto [to, bytes, counters] : {std::tuple(&c->paged_part, PAGED_PART_BYTES, PAGED_BLOCKS * 128),
+  for (auto [to, bytes, counters] : {std::tuple(&c->paged_plan, PAGED_PLAN_BYTES, (int64_t)128),
+                                     std::tuple(&c->paged_part, PAGED_PART_BYTES, PAGED_BLOCKS * 128),
                                      std::tuple(&c->logprobs_part, LOGPROBS_PART_BYTES, LOGPROBS_BLOCKS * 32)}) {
     void* q = nullptr;
     if (hipMalloc(&q, bytes + counters) != hipSuccess) {

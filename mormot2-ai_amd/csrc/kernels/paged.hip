@@ -12,7 +12,8 @@ struct SlotArgs {
   const int64_t* ends;
   int64_t* ends_out;
   int *offsets, *lengths, *positions, *slots, *failed;
-  int* plan;  // [5][seqs], then 4 numbers: the plan between the two launches
+  int* plan;  // [5][seqs], then SlotPlan's numbers: the plan between the two launches
+  int* meet;  // a counter of its blocks and a flag, zero between launches
   int32_t seqs, max_pages, page_size, pages, rows;
   int32_t here;  // 1: the rows in this launch too
 };
@@ -68,11 +69,13 @@ __device__ __forceinline__ void scan_block(const int64_t (&v)[N], int64_t (&befo
 struct SlotPlan {
   int *row, *move, *rank, *past, *state;
   int rows, moves, first, last;  // all rows, all moves, ends[0] and ends[1] modulo pages
+  int back, room;  // entries put back, pages that the ring has place for
+  int closed;      // 1: sequences end, 2: and not all of their tables' entries find a place
 };
 
 __device__ __forceinline__ SlotPlan slot_plan(int* p, int n)
 {
-  return {p, p + n, p + 2 * n, p + 3 * n, p + 4 * n, 0, 0, 0, 0};
+  return {p, p + n, p + 2 * n, p + 3 * n, p + 4 * n, 0, 0, 0, 0, 0, 0, 0};
 }
 
 // the last s of the n with first[s] <= i (first ascending, first[0] <= i)
@@ -93,17 +96,39 @@ __device__ __forceinline__ int ring_at(uint32_t base, uint32_t i, uint32_t pages
   return (int)(at >= pages ? at % pages : at);
 }
 
-// rows and page moves i0, i0 + step, ... of the plan
-__device__ __forceinline__ void slot_rows(const SlotArgs& a, const SlotPlan& p, int i0, int step)
+__device__ __forceinline__ bool page_there(const SlotArgs& a, int page) { return page >= 0 && page < a.pages; }
+
+// (through to memory: another block may write the entry again, put_back)
+__device__ __forceinline__ void ring_store(const SlotArgs& a, const SlotPlan& p, uint32_t at, int page)
+{
+  __hip_atomic_store(a.ring + ring_at(p.last, at, a.pages), page, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// page moves i0, i0 + step, ... of the plan; whether an entry put back is no page of the
+// pool
+__device__ __forceinline__ bool slot_moves(const SlotArgs& a, const SlotPlan& p, int i0, int step)
 {
   const uint32_t ps = a.page_size;
-  for (int64_t i = step - 1 - i0; i < p.moves; i += step) {  // (other waves than the first rows')
+  bool hole = false;
+  for (int64_t i = i0; i < p.moves; i += step) {
     const int s = slot_find(p.move, a.seqs, (int)i), j = (int)i - p.move[s];
     int* const t = a.table + (int64_t)s * a.max_pages;
     const uint32_t at = (uint32_t)p.rank[s] + (uint32_t)j;
-    if (p.state[s] == 2) a.ring[ring_at(p.last, at, a.pages)] = t[j];
-    else t[((uint32_t)p.past[s] + ps - 1) / ps + j] = a.ring[ring_at(p.first, at, a.pages)];
+    if (p.state[s] == 2) {
+      const int page = t[j];
+      hole |= !page_there(a, page);
+      ring_store(a, p, at, page);
+    } else {
+      t[((uint32_t)p.past[s] + ps - 1) / ps + j] = a.ring[ring_at(p.first, at, a.pages)];
+    }
   }
+  return hole;
+}
+
+// rows i0, i0 + step, ... of the plan
+__device__ __forceinline__ void slot_rows(const SlotArgs& a, const SlotPlan& p, int i0, int step)
+{
+  const uint32_t ps = a.page_size;
   for (int64_t i = i0; i < a.rows; i += step) {
     int pos = -1, slot = -1;
     if (i < p.rows) {
@@ -117,11 +142,55 @@ __device__ __forceinline__ void slot_rows(const SlotArgs& a, const SlotPlan& p, 
         const int have = (int)(((uint32_t)p.past[s] + ps - 1) / ps), j = (int)((uint32_t)pos / ps);
         const int page = j < have ? a.table[(int64_t)s * a.max_pages + j]
                                   : a.ring[ring_at(p.first, p.rank[s] + j - have, a.pages)];
-        if (page >= 0 && page < a.pages) slot = page * (int)ps + (int)((uint32_t)pos % ps);
+        if (page_there(a, page)) slot = page * (int)ps + (int)((uint32_t)pos % ps);
       }
     }
     a.positions[i] = pos;
     a.slots[i] = slot;
+  }
+}
+
+// The ended sequences' pages into the ring once more, by one block, where a table has
+// entries that are no page of the pool (holes, which are no free pages) or where with
+// them the entries passed the ring's place: those that are pages alone, in order. Rare,
+// so that the others' way has no look at the tables before the plan is made (with it
+// 500 sequences 28 us for 15).
+__device__ __forceinline__ void put_back(const SlotArgs& a, const SlotPlan& p)
+{
+  const int t = threadIdx.x, lane = t & 63, waves = blockDim.x >> 6, per = (a.seqs + blockDim.x - 1) / blockDim.x;
+  auto entries = [&](int s, auto&& each) {
+    const int n = p.state[s] == 2 ? (int)min(((uint32_t)p.past[s] + a.page_size - 1) / (uint32_t)a.page_size, (uint32_t)a.max_pages) : 0;
+    int kept = 0;
+#pragma unroll 1
+    for (int j = lane; j - lane < n; j += 64) {
+      const int page = j < n ? a.table[(int64_t)s * a.max_pages + j] : -1;
+      const uint64_t there = __ballot(page_there(a, page));
+      if (page_there(a, page))
+        each(kept + __builtin_amdgcn_mbcnt_hi((uint32_t)(there >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)there, 0u)), page);
+      kept += __popcll(there);
+    }
+    return kept;
+  };
+  for (int s = t >> 6; s < a.seqs; s += waves) {
+    const int kept = entries(s, [](int, int) {});
+    if (lane == 0) p.rank[s] = kept;
+  }
+  __syncthreads();
+  int64_t mine = 0, before[1], all[1];
+  for (int s = t * per; s < min((t + 1) * per, a.seqs); s++) mine += p.rank[s];
+  scan_block<1>({mine}, before, all);
+  int64_t put = before[0], back = 0;
+  for (int s = t * per; s < min((t + 1) * per, a.seqs); s++) {
+    const int n = p.rank[s];
+    p.move[s] = put + n <= p.room ? (int)put : -1;
+    if (put + n <= p.room) back += n;
+    put += n;
+  }
+  scan_block<1>({back}, before, all);
+  if (t == 0) a.ends_out[1] += all[0] - p.back;
+  for (int s = t >> 6; s < a.seqs; s += waves) {
+    const int at = p.move[s];
+    if (at >= 0) entries(s, [&](int i, int page) { ring_store(a, p, at + i, page); });
   }
 }
 
@@ -221,6 +290,9 @@ __device__ __forceinline__ void paged_slots_t(const SlotArgs& a)
   }
   p.rows = (int)(all_rows < INT32_MAX ? all_rows : INT32_MAX);
   p.moves = (int)all4[0];
+  p.back = (int)all4[1];
+  p.room = (int)(a.pages - free_pages);
+  p.closed = all2[1] ? all2[1] > p.back ? 2 : 1 : 0;
   __syncthreads();  // the inputs are read, the plan is in LDS
 #pragma unroll
   for (int i = 0; i < SLOT_PER; i++) {
@@ -236,7 +308,10 @@ __device__ __forceinline__ void paged_slots_t(const SlotArgs& a)
     if (a.failed) a.failed[0] = (int)all4[3];
   }
   if (a.here) {
+    // (the moves by other waves than the first rows')
+    const bool hole = slot_moves(a, p, blockDim.x - 1 - t, blockDim.x);
     slot_rows(a, p, t, blockDim.x);
+    if (p.closed && __syncthreads_or(hole || p.closed == 2)) put_back(a, p);
     return;
   }
   for (int i = t; i < 5 * a.seqs; i += blockDim.x) a.plan[i] = slot_lds[i];
@@ -246,6 +321,9 @@ __device__ __forceinline__ void paged_slots_t(const SlotArgs& a)
     e[1] = p.moves;
     e[2] = p.first;
     e[3] = p.last;
+    e[4] = p.back;
+    e[5] = p.room;
+    e[6] = p.closed;
   }
 }
 
@@ -255,8 +333,9 @@ __device__ __forceinline__ void paged_slots_t(const SlotArgs& a)
 extern "C" __global__ __launch_bounds__(SLOT_THREADS) void paged_slots_1(SlotArgs a) { paged_slots_t<1>(a); }
 extern "C" __global__ __launch_bounds__(SLOT_THREADS) void paged_slots_4(SlotArgs a) { paged_slots_t<4>(a); }
 
-// the rows of a step with prompts, by as many blocks as they fill: the plan
-// from paged_slots' launch
+// the rows of a step with prompts, by as many blocks as they fill, and as many again for
+// the page moves, which are through with their meeting before the rows are: the plan from
+// paged_slots' launch
 extern "C" __global__ __launch_bounds__(256) void paged_slots_rows(SlotArgs a)
 {
   extern __shared__ int slot_lds[];
@@ -267,8 +346,28 @@ extern "C" __global__ __launch_bounds__(256) void paged_slots_rows(SlotArgs a)
   p.moves = e[1];
   p.first = e[2];
   p.last = e[3];
+  p.back = e[4];
+  p.room = e[5];
+  p.closed = e[6];
   __syncthreads();
-  slot_rows(a, p, blockIdx.x * 256 + threadIdx.x, gridDim.x * 256);
+  const int half = gridDim.x / 2, b = blockIdx.x;
+  if (b < half) {
+    slot_rows(a, p, b * 256 + threadIdx.x, half * 256);
+    return;
+  }
+  const bool hole = slot_moves(a, p, (b - half) * 256 + threadIdx.x, half * 256);
+  if (!p.closed) return;
+  // what the blocks found meets in the last of them
+  if (__syncthreads_or(hole) && threadIdx.x == 0)
+    __hip_atomic_store(a.meet + 1, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  if (!last_block(a.meet, half)) return;
+  const int any = __hip_atomic_load(a.meet + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    __hip_atomic_store(a.meet, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __hip_atomic_store(a.meet + 1, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  if (any || p.closed == 2) put_back(a, p);
 }
 
 // ------------------------------------------------------------ paged_qkrope

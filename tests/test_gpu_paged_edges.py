@@ -7,7 +7,7 @@ import pytest
 
 import infer_hip as H
 import paged_ref as R
-from test_gpu_paged import assert_close, ctx, dev, pages_struct  # noqa: F401 (fixtures)
+from test_gpu_paged import assert_close, batch, ctx, dev, pages_struct, run_slots  # noqa: F401 (fixtures)
 
 pytestmark = pytest.mark.gpu
 
@@ -92,3 +92,69 @@ def test_attention_sinks_switched_off(ctx, dev, dtype, off):
     assert np.isnan(got[5, 1]).all() and (got[5, 4] == 0).all()
     others = [0, 2, 3, 5, 6, 7]
     assert_close(got[5][others], want[5][others], tol[5][others])
+
+
+# ---------------------------------------------------------------------- plan
+def plan_with_holes(past, count, table, page_size, ring, ends, rows):
+    """The plan in which an ended sequence holds the pages of the pool that its table has, and no
+    others; the table itself is left as it is."""
+    t, held = table.copy(), past.copy()
+    ended = np.flatnonzero((past >= 0) & (count < 0))
+    for s in ended:
+        have = min(-(-int(past[s]) // page_size), t.shape[1])
+        own = t[s, :have]
+        own = own[(own >= 0) & (own < len(ring))]
+        t[s, :len(own)], held[s] = own, len(own) * page_size
+    want = R.slots(held, count, t, page_size, ring, ends, rows)
+    want["table"][ended] = table[ended]
+    return want
+
+
+@pytest.mark.parametrize("n,page_size,most,new,spare,rows", [
+    (1, 16, 900, 1, 4, 1), (3, 1, 300, 3, 20, 16), (64, 16, 300, 1, 64, 64), (200, 24, 500, 40, 500, 9000),
+    (257, 4, 700, 9, 300, 4097), (1000, 3, 20, 9, 4000, 3000), (4096, 2, 30, 2, 2000, 12000)])
+@pytest.mark.parametrize("share", [0.02, 0.5, 1.0])
+def test_slots_ended_tables_with_holes(ctx, dev, n, page_size, most, new, spare, rows, share):
+    """An ended sequence's entries outside the pool (a window's pages, released before) do not come
+    into the ring, and those behind them do, in order."""
+    rng = np.random.default_rng(n + int(100 * share))
+    past, count, table, ring, ends = batch(rng, n, page_size, most, new, spare, ended=0.4)
+    if n == 1:
+        past[:], count[:] = most, -1
+        table[:, :-(-most // page_size)] = np.arange(-(-most // page_size)) % len(ring)
+    ended = np.flatnonzero(count < 0)
+    hole = rng.random((len(ended), table.shape[1])) < share
+    bad = rng.choice(np.array([-1, -2 ** 31, len(ring), 2 ** 31 - 1], np.int32), hole.shape)
+    table[ended] = np.where(hole, bad, table[ended])
+    want = plan_with_holes(past, count, table, page_size, ring, ends, rows)
+    got = run_slots(ctx, dev, past, count, table, page_size, ring, ends, rows)
+    for k in want:
+        if k != "ring":
+            assert np.array_equal(got[k], want[k]), k
+    # the free pages (what the ring holds outside its ends is nothing)
+    at = np.arange(*want["ends"]) % len(ring)
+    assert np.array_equal(got["ring"][at], want["ring"][at])
+    assert len(set(at.tolist())) == len(at)
+
+
+def test_slots_shared_pages_ended(ctx, dev):
+    """Two sequences over a common prompt: the one that ends first has the shared entries taken out of
+    its table, and only its own pages are free afterwards; then all pages are given out once."""
+    ps, width, pages = 4, 8, 12
+    table = np.full((3, width), -1, np.int32)
+    table[0, :4], table[1, :4] = (3, 7, 1, 9), (3, 7, 0, 4)
+    ring = np.array([2, 5, 6, 8, 10, 11, -7, -7, -7, -7, -7, -7], np.int32)
+    past, ends = np.array([16, 16, 0], np.int32), np.array([0, 6], np.int64)
+    table[1, :2] = -1
+    got = run_slots(ctx, dev, past, np.array([1, -1, 1], np.int32), table, ps, ring, ends, 2)
+    assert got["ends"].tolist() == [2, 8] and got["ring"][6:8].tolist() == [0, 4]
+    assert got["table"][0, :5].tolist() == [3, 7, 1, 9, 2] and got["failed"][0] == 0
+    past = got["lengths"].copy()
+    past[1] = 0
+    got = run_slots(ctx, dev, past, np.array([0, 24, 0], np.int32), got["table"], ps, got["ring"], got["ends"], 30)
+    held = np.concatenate([got["table"][0, :5], got["table"][1, :6], got["table"][2, :1]])
+    assert sorted(held.tolist()) == list(range(pages)) and got["failed"][0] == 0
+    assert (got["slots"][:24] >= 0).all() and got["ends"].tolist() == [8, 8]
+    # none is left
+    got = run_slots(ctx, dev, got["lengths"], np.array([0, 1, 0], np.int32), got["table"], ps, got["ring"], got["ends"], 3)
+    assert got["failed"][0] == 1 and got["slots"][0] == -1
