@@ -622,8 +622,12 @@ int ihip_model_frequencies(const ihip_model_desc* desc, float* freq, double* sca
  *   new tokens need are taken from the free ones, in the sequences' order, and
  *   written behind those it has;
  * - ring [pages] and ends (int64[2]): the free pages are ring[i mod pages] for
- *   ends[0] <= i < ends[1]; ends_out receives the ends after the call. Pages
- *   that ended sequences give back are there from the next call on;
+ *   ends[0] <= i < ends[1]; ends_out receives the ends after the call, and what
+ *   the ring holds outside them is nobody's. Pages that ended sequences give back
+ *   are there from the next call on, those of the pool alone (an entry outside it,
+ *   as a window's page that the host released before, is none). A page is one
+ *   sequence's or the ring's: one that another sequence still holds (a common
+ *   prompt's) is taken out of the table, as -1, before its sequence ends;
  * - offsets [seqs + 1]: the rows of sequence s are offsets[s] .. offsets[s + 1];
  * - lengths [seqs]: past + count, -1 of an ended sequence or an empty place;
  * - positions, slots [rows]: of every new token; -1 in the rows behind the last;
