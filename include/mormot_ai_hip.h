@@ -658,8 +658,8 @@ int ihip_enqueue_paged_qkrope(ihip_ctx* ctx, uint64_t q, int64_t q_stride, uint6
                               const ihip_pages* cache, uint64_t q_out);
 /* attention of one new token of each sequence over its pages: y [seqs, heads,
  * head_dim] = softmax(scale q k) v over the keys 0 .. lengths[s] - 1 (window > 0:
- * the last `window` of them; sinks: device [heads] or 0; scale 0: 1 / sqrt(
- * head_dim)); table [seqs, max_pages], q rows of q_stride floats (0: heads *
+ * the last `window` of them; sinks: device [heads] or 0; scale >= 0, 0: 1 /
+ * sqrt(head_dim)); table [seqs, max_pages], q rows of q_stride floats (0: heads *
  * head_dim). A key whose table entry is outside the pool is not there, one whose
  * score is -infinity has weight 0, and so has a sink of -infinity. A sequence with
  * no key (length 0), or whose keys have no weight, gives zeros, one with lengths[s]

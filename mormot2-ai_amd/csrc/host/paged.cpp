@@ -201,7 +201,9 @@ int ihip_enqueue_paged_attention_at(ihip_ctx* c, uint64_t q, int64_t q_stride, c
   if (q_stride < heads * hd) return refuse(who, "a stride below a row");
   if (q_stride > STRIDE_MOST) return refuse(who, "a stride beyond 2^36");
   if ((q | y | sinks | lengths | offsets | table) % 4) return refuse(who, "arrays aligned to 4 bytes");
-  if (std::isnan(scale) || std::isinf(scale)) return refuse(who, "scale");
+  // (the kernel's scores are in base 2, in single)
+  const float scale2 = (float)((scale != 0 ? scale : 1.0 / std::sqrt((double)hd)) * 1.4426950408889634);
+  if (!(scale >= 0) || !std::isfinite(scale2)) return refuse(who, "scale is 0 or positive, times log2 e within single");
   // the kernels take tiles of 128 keys of 16-bit caches, 64 of single ones, half as
   // many of heads beyond 256
   const int64_t group = heads / kvh, tiles = (group + 15) / 16;
@@ -226,7 +228,7 @@ int ihip_enqueue_paged_attention_at(ihip_ctx* c, uint64_t q, int64_t q_stride, c
          (const int*)lengths, (const int*)offsets, (float*)y, (const float*)sinks, (float*)c->paged_part,
          (int*)(c->paged_part + PAGED_PART_BYTES), q_stride, cache->pages, p.page_stride,
          p.slot_stride, p.head_stride, window,
-         (float)((scale > 0 ? scale : 1.0 / std::sqrt((double)hd)) * 1.4426950408889634), (int32_t)seqs,
+         scale2, (int32_t)seqs,
          (int32_t)heads, (int32_t)kvh, (int32_t)hd, cache->page_size, (int32_t)max_pages, (int32_t)group,
          (int32_t)tiles, (int32_t)rows, c->cus};
   const int d = hd <= 64 ? 64 : hd <= 128 ? 128 : hd <= 256 ? 256 : 512;

@@ -4,7 +4,9 @@ import ctypes as C
 
 import pytest
 
+import infer_hip as H
 import oracle_lib as O
+from test_paged import A, attention, pages, refused
 
 
 def row(first, end, rows):
@@ -28,3 +30,16 @@ def test_rows_stay_in_the_step(rows):
 def test_rows_without_offsets():
     """Row s of sequence s, where there is one."""
     assert [row(s, s + 1, 3) for s in range(6)] == [0, 1, 2, -1, -1, -1]
+
+
+# ------------------------------------------------------------------ refusals
+@pytest.mark.parametrize("scale", [-0.125, -1e-300, 1e39, 3e38])
+def test_attention_scales_refused(scale):
+    """A scale below 0 (which no formula here has: 0 alone stands for the default), and one that
+    leaves single when the exponential's base is 2."""
+    refused(lambda: attention(pages(), scale=scale), -1, "scale")
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.0, 1e-30, 2.3e38])
+def test_attention_scales_taken(scale):
+    refused(lambda: attention(pages(), scale=scale), -1, "no context")
