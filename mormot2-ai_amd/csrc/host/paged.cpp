@@ -88,6 +88,8 @@ int ihip_enqueue_paged_slots(ihip_ctx* c, uint64_t past, uint64_t count, int64_t
       pages > INT32_MAX / page_size || max_pages < 1 || max_pages > INT32_MAX / page_size)
     return refuse(who, "seqs, rows, page_size, pages or max_pages out of range");
   if (ends % 8 || ends_out % 8) return refuse(who, "ends are int64, aligned to 8 bytes");
+  if ((past | count | table | ring | offsets | lengths | positions | slots | failed) % 4)
+    return refuse(who, "arrays aligned to 4 bytes");
   if (!c) return no_context(who);
   OnDevice on(c);
   struct {
@@ -133,7 +135,7 @@ int ihip_enqueue_paged_qkrope(ihip_ctx* c, uint64_t q, int64_t q_stride, uint64_
   if (q_stride < qw || k_stride < kw || v_stride < kw) return refuse(who, "a stride below a row");
   if (std::max({q_stride, k_stride, v_stride}) > STRIDE_MOST) return refuse(who, "a stride beyond 2^36");
   const uint64_t aligned = q | k | v | q_out | qn | kn;
-  if (aligned % 4) return refuse(who, "floats aligned to 4 bytes");
+  if ((aligned | positions | slots) % 4) return refuse(who, "arrays aligned to 4 bytes");
   if (!(eps >= 0) || !std::isfinite(eps)) return refuse(who, "eps");
   int64_t dims = 0;
   if (rope) {

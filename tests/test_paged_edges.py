@@ -6,7 +6,7 @@ import pytest
 
 import infer_hip as H
 import oracle_lib as O
-from test_paged import A, attention, pages, refused
+from test_paged import A, attention, pages, qkrope, refused
 
 
 def row(first, end, rows):
@@ -43,3 +43,20 @@ def test_attention_scales_refused(scale):
 @pytest.mark.parametrize("scale", [0.0, -0.0, 1e-30, 2.3e38])
 def test_attention_scales_taken(scale):
     refused(lambda: attention(pages(), scale=scale), -1, "no context")
+
+
+@pytest.mark.parametrize("skew", [1, 2, 3])
+def test_unaligned_numbers_refused(skew):
+    """Lengths, tables, positions and slots are int32, aligned to 4 bytes, as the attention's are."""
+    names = ("past", "count", "seqs", "table", "max_pages", "page_size", "ring", "pages", "ends", "ends_out", "offsets",
+             "lengths", "positions", "slots", "rows", "failed")
+    good = dict(zip(names, (A, A, 3, A, 4, 16, A, 9, A, A, A, A, A, A, 7, A)))
+
+    def slots(**kw):
+        return H.lib().ihip_enqueue_paged_slots(None, *dict(good, **kw).values())
+
+    refused(slots, -1, "no context")
+    for name in ("past", "count", "table", "ring", "offsets", "lengths", "positions", "slots", "failed"):
+        refused(lambda: slots(**{name: A + skew}), -1, "4 bytes")
+    for name in ("positions", "slots"):
+        refused(lambda: qkrope(pages(), **{name: A + skew}), -1, "4 bytes")
