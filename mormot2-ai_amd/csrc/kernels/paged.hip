@@ -628,6 +628,17 @@ __device__ __forceinline__ void split2(float x, float y, uint32_t* part)
   }
 }
 
+// At least 64 clocks: what reads the products before it may lie behind any branch, where
+// the compiler counts the wait states (40 clocks at most) along one of the ways alone.
+// (A sleep: an asm statement costs these kernels two registers, and bf16 heads of 128 the
+// second block of a CU.)
+__device__ __forceinline__ void products_done()
+{
+  __builtin_amdgcn_sched_barrier(0);
+  __builtin_amdgcn_s_sleep(1);
+  __builtin_amdgcn_sched_barrier(0);
+}
+
 __device__ __forceinline__ uint64_t lane_value(uint64_t v, int lane)
 {
   return (uint64_t)__builtin_amdgcn_readlane((uint32_t)(v >> 32), lane) << 32 |
@@ -974,9 +985,11 @@ __device__ __forceinline__ void paged_attention_t(const PagedAttnArgs& a)
       const uint32_t mine = (uint32_t)((hi - wlo + S::TK - 1) / S::TK);
       steps = min(tile1, mine) - tile0;
     }
-    // The loop has no branch between a product and what reads it, so keys are
-    // located and loaded one step past the piece's last too: entry() has no page there
-    // and the loads read the pool's first row.
+    // The scores are read on both sides of branches, and the values' sums in a block that
+    // few steps enter and behind the loop: products_done() stands before each. Keys are
+    // located and loaded one step past the piece's last too, as a condition there would
+    // keep the loads from covering the products: entry() has no page there and the loads
+    // read the pool's first row.
     uint32_t there = locate(tile, page0);
     if (steps) load_keys(tile);
     for (uint32_t i = 0; i < steps; i++, tile++) {
@@ -1022,6 +1035,7 @@ __device__ __forceinline__ void paged_attention_t(const PagedAttnArgs& a)
         }
       }
       load_keys(tile + 1);
+      products_done();
       if constexpr (S::DS > 1) {
         // the scores of all dimensions: two waves' shares added, the same sum in both
 #pragma unroll
@@ -1096,6 +1110,7 @@ __device__ __forceinline__ void paged_attention_t(const PagedAttnArgs& a)
     }
 
     // the waves' sums meet
+    products_done();
     l = quad_sum(l);
     if (g == 0 && dh == 0) {
       s.wm[kg][c] = m;
