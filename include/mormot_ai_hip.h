@@ -634,7 +634,10 @@ int ihip_model_frequencies(const ihip_model_desc* desc, float* freq, double* sca
  * - failed [1] (or 0): the sequences that got none of their new tokens, because
  *   the free pages, max_pages or rows do not hold them: their slots are -1 and
  *   their length stays past[s] (positions are given). Free pages too few for a
- *   sequence leave none for those behind it that need one.
+ *   sequence leave none for those behind it that need one. The rows of such a
+ *   sequence are in the step all the same: nothing is stored for them, and the
+ *   attention answers the last of them from the keys that the sequence had. The
+ *   host drops what comes of them (the rows with a position and no slot).
  * ends_out may be ends, and lengths may be past. */
 #define IHIP_PAGED_SEQS 4096
 int ihip_enqueue_paged_slots(ihip_ctx* ctx, uint64_t past, uint64_t count, int64_t seqs,

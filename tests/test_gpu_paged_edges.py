@@ -158,3 +158,40 @@ def test_slots_shared_pages_ended(ctx, dev):
     # none is left
     got = run_slots(ctx, dev, got["lengths"], np.array([0, 1, 0], np.int32), got["table"], ps, got["ring"], got["ends"], 3)
     assert got["failed"][0] == 1 and got["slots"][0] == -1
+
+
+# ------------------------------------------------------------------ together
+def test_failed_sequence_in_a_step(ctx, dev):
+    """A sequence that finds no page has its row in the step all the same: nothing is stored for it, and
+    the attention answers the row from the keys that the sequence had; the others go on."""
+    rng = np.random.default_rng(41)
+    heads, kvh, hd, ps, width, n, pages = 4, 2, 64, 4, 6, 3, 5
+    table = np.full((n, width), -1, np.int32)
+    table[0, :2], table[1, :2] = (4, 0), (2, 1)
+    ring, ends = np.array([3, -7, -7, -7, -7], np.int32), np.array([0, 1], np.int64)
+    past, count = np.array([7, 8, 4], np.int32), np.array([1, 1, 1], np.int32)
+    table[2, 0] = 1  # (its page is shared: it has one key more to come, and no page left for it)
+    got = run_slots(ctx, dev, past, count, table, ps, ring, ends, n)
+    assert got["failed"][0] == 1 and got["lengths"].tolist() == [8, 9, 4]
+    assert got["offsets"].tolist() == [0, 1, 2, 3] and got["positions"].tolist() == [7, 8, 4]
+    assert got["slots"].tolist() == [3, 3 * ps, -1]
+    k, v = (rng.standard_normal((pages, ps, kvh, hd)).astype(np.float32) for _ in range(2))
+    x = rng.standard_normal((n, heads + 2 * kvh, hd)).astype(np.float32)
+    dk, dv = dev.out(k.nbytes), dev.out(v.nbytes)
+    dk.upload(k), dv.upload(v)
+    pool = pages_struct(dk.ptr, dv.ptr, pages, ps, kvh, hd, "f32")
+    dx, y, row = dev(x), dev.out(n * heads * hd * 4), (heads + 2 * kvh) * hd
+    H.check(H.lib().ihip_enqueue_paged_qkrope(
+        ctx.h, dx, row, dx + 4 * heads * hd, row, dx + 4 * (heads + kvh) * hd, row, n, heads, 0, 0, 0.0, None,
+        dev(got["positions"]), dev(got["slots"]), C.byref(pool), 0))
+    H.check(H.lib().ihip_enqueue_paged_attention_at(
+        ctx.h, dx, row, C.byref(pool), dev(got["table"]), width, dev(got["lengths"]), dev(got["offsets"]), n, y.ptr, n,
+        heads, 0, 0, 0.0))
+    for i, cache in enumerate((k, v)):
+        at = cache.reshape(pages * ps, kvh, hd)
+        at[[3, 3 * ps]] = x[:2, heads + i * kvh:heads + (i + 1) * kvh]
+    assert np.array_equal(dk.download(np.float32, k.size), k.ravel())
+    assert np.array_equal(dv.download(np.float32, v.size), v.ravel())
+    want, tol = R.attention(x[:, :heads].astype(np.float64), k.astype(np.float64), v.astype(np.float64), got["table"],
+                            got["lengths"], ps)
+    assert_close(y.download(np.float32, want.size).reshape(want.shape), want, tol)
