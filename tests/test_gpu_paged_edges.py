@@ -20,7 +20,7 @@ class Batch:
         self.dtype, self.hd, self.heads, self.kvh, self.ps = dtype, hd, heads, kvh, ps
         self.lengths = np.array(lengths, np.int32)
         n = len(lengths)
-        self.width = width or max(1, int(-(-self.lengths.clip(0) // ps).max()))
+        self.width = width or max(1, int((-(-self.lengths.clip(0) // ps)).max()))
         self.pages = n * self.width
         self.table = rng.permutation(self.pages).reshape(n, self.width).astype(np.int32)
         self.k, self.v = (rng.standard_normal((self.pages, ps, kvh, hd)) for _ in range(2))
@@ -195,3 +195,76 @@ def test_failed_sequence_in_a_step(ctx, dev):
     want, tol = R.attention(x[:, :heads].astype(np.float64), k.astype(np.float64), v.astype(np.float64), got["table"],
                             got["lengths"], ps)
     assert_close(y.download(np.float32, want.size).reshape(want.shape), want, tol)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("sinks", [False, True])
+def test_attention_scores_of_minus_infinity(ctx, dev, dtype, sinks):
+    """A key of score -infinity has weight 0 and the others theirs; the KV head that does not see the
+    infinity has its keys all."""
+    rng = np.random.default_rng(6)
+    b = Batch(rng, dtype, 128, 8, 2, 1, [48, 200, 5, 3000])
+    b.q = np.abs(b.q)
+    if sinks:
+        b.sinks = rng.standard_normal(8).astype(np.float32)
+    b.upload(dev)
+    plain, _ = b.want()
+    hidden = [(s, j) for s, n in enumerate(b.lengths) for j in (0, 3, n // 2, n - 1)]
+    for s, j in hidden:
+        b.k[b.table[s, j], 0, 1, 7] = -np.inf
+    got = b.run(ctx, dev)
+    b.k[~np.isfinite(b.k)] = 0  # (as a key that is not there)
+    b.raw[0], table = R.pack(b.k, dtype), b.table.copy()
+    want, tol = b.want()
+    assert_close(got[:, :4], want[:, :4], tol[:, :4])
+    for s, j in hidden:
+        b.table[s, j] = -1
+    want, tol = b.want()
+    b.table = table
+    assert_close(got[:, 4:], want[:, 4:], tol[:, 4:])
+    assert np.abs(got[2, 4:] - plain[2, 4:]).max() > 1e-2  # (4 of 5 keys fewer)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16", "f32"])
+def test_attention_lengths_beyond_the_table(ctx, dev, dtype):
+    """A length that the table does not hold is cut to it, every page of which is there; a window is the
+    last keys of those."""
+    rng = np.random.default_rng(13)
+    for window in (0, 20):
+        b = Batch(rng, dtype, 128, 8, 2, 16, [2 ** 31 - 1, 80, 81, 79, 5000], width=5)
+        b.window = window
+        got = b.run(ctx, dev)
+        want, tol = b.want()
+        assert_close(got, want, tol)
+        b.lengths = np.array([80, 80, 80, 79, 80], np.int32)
+        again, _ = b.want()
+        assert np.array_equal(want, again)
+
+
+def test_two_contexts_at_once(ctx):
+    """Calls of two contexts on their own streams, all enqueued before the first is read."""
+    rng = np.random.default_rng(32)
+    with H.Context(0) as other:
+        class Dev:
+            def __init__(self, c):
+                self.c = c
+
+            def __call__(self, a):
+                return self.c.array(a).ptr
+
+            def out(self, nbytes, fill=0x5A):
+                return self.c.array(np.full(nbytes, fill, np.uint8))
+
+        calls = []
+        for i in range(4):
+            for c in (ctx, other):
+                b = Batch(rng, ("f16", "bf16")[i % 2], 128, 16, 2, 16, [1500 + 100 * i, 3, 700, 4000])
+                b.upload(Dev(c))
+                calls.append((c, b))
+        for _ in range(3):
+            for c, b in calls:
+                b.enqueue(c)
+        for c, b in calls:
+            want, tol = b.want()
+            assert_close(b.read(), want, tol)
+        ctx.sync()
