@@ -198,8 +198,8 @@ __device__ __forceinline__ void put_back(const SlotArgs& a, const SlotPlan& p)
 // which depend on the rows that fit; the moves), the plan in LDS. Everything that a
 // caller may pass as input and output is read before the barrier behind which it is
 // written. Latency bound: the lengths, then a table entry or a free page, then the
-// stores. 64 sequences' decode step 6.7 us; 500 with 150000 rows 6.0 us and 8.6 for
-// paged_slots_rows.
+// stores, then whether any page put back was none. 64 sequences' decode step 7.4 us; 500
+// with 150000 rows 6.2 us and 9.4 for paged_slots_rows.
 template <int SLOT_PER>
 __device__ __forceinline__ void paged_slots_t(const SlotArgs& a)
 {
@@ -327,9 +327,10 @@ __device__ __forceinline__ void paged_slots_t(const SlotArgs& a)
   }
 }
 
-// one sequence a thread up to 256 (a decode step of 64 6.7 us; four a thread, whose
-// code is longer and comes from a cold cache, 8.3), else four (500 sequences 6.0 us,
-// one a thread, whose scans have four times the waves, 6.5)
+// one sequence a thread up to 256 (a decode step of 64 6.7 us, four a thread, whose
+// code is longer and comes from a cold cache, 8.3; both without the look at what is put
+// back, 0.6 more), else four (500 sequences 6.0 us, one a thread, whose scans have four
+// times the waves, 6.5)
 extern "C" __global__ __launch_bounds__(SLOT_THREADS) void paged_slots_1(SlotArgs a) { paged_slots_t<1>(a); }
 extern "C" __global__ __launch_bounds__(SLOT_THREADS) void paged_slots_4(SlotArgs a) { paged_slots_t<4>(a); }
 
@@ -680,7 +681,10 @@ struct AttnShape {
   static constexpr int VL = T != 0 && D > 64 ? 8 : 4;  // values of a value load
   static constexpr int NJ = DW / (16 * VL);            // value loads of a lane and key
   static constexpr int OS = D + 4;                     // a head's row in o_s
-  static constexpr float PS = T == 1 ? 32768.f : 1.f;  // weights enter the product times this: halves' normal range
+  // weights enter the product times this: into the halves' normal range. The two parts
+  // hold 22 bits of those down to 2^-18 of the largest; smaller ones are off by 2^-40 of
+  // the largest at most
+  static constexpr float PS = T == 1 ? 32768.f : 1.f;
 };
 
 template <int T, int D>
@@ -832,8 +836,8 @@ __device__ __forceinline__ void stage_query(const PagedAttnArgs& a, const AttnIt
 // parts (f32 caches: the f32 matrix cores), so the sums are those of single.
 //
 // HBM bound: the cache is read once (again for each 16 query heads of a KV head
-// beyond 16). 64 sequences of 16384 keys, 8 KV heads of 128 in bf16 735 us, 5.8 TB/s
-// of the 6.2 that a streaming read takes; single 6.3, heads of 256 5.5, of 64 5.0 to
+// beyond 16). 64 sequences of 16384 keys, 8 KV heads of 128 in bf16 705 to 718 us, 6.0
+// TB/s of the 6.2 that a streaming read takes; single 6.3, heads of 256 5.5, of 64 5.0 to
 // 5.8; few long sequences lose the join (three of 110000: 136 us, 5.0), one short one
 // is a chain of round trips (1152 keys 12.5 us). Pages of [kv_heads, page_size,
 // head_dim] read up to 6% faster than [page_size, kv_heads, head_dim]. Heads
@@ -1293,9 +1297,11 @@ __device__ __forceinline__ void paged_attention_t(const PagedAttnArgs& a)
   }
 }
 
-// heads between two sizes: two blocks a CU up to 128 (the bound costs the join of few
-// long sequences, 24 us became 32, so the others, which stay below 256 registers on
-// their own, have none)
+// heads between two sizes: two blocks a CU up to 128. The others have no bound, which
+// costs the join of few long sequences (24 us became 32). On their own those up to 128
+// take 189 to 256 registers, two blocks a CU - but for halves of 128, whose 260 leave
+// one: 64 ragged sequences up to 4000 keys, 16 heads over 8, 140 us where bf16 takes 115,
+// 200 of them 350 and 310.
 #define PAGED_ATTENTION(NAME, T, D)                                                                         \
   extern "C" __global__ __launch_bounds__(256) void paged_attention_##NAME##_##D(PagedAttnArgs a)           \
   {                                                                                                         \
