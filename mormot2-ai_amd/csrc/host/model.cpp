@@ -2088,7 +2088,9 @@ extern "C" {
 
 int ihip_model_frequencies(const ihip_model_desc* d, float* freq, double* scale)
 {
-  if (!d || !freq || rope_dims(*d) < 2 || rope_dims(*d) & 1 || !(d->rope_theta > 0))
+  // (the shares that ihip_model_create takes)
+  if (!d || !freq || d->head_dim > 512 || rope_dims(*d) < 2 || rope_dims(*d) > d->head_dim || rope_dims(*d) & 1 ||
+      !(d->rope_theta > 0))
     return fail(IHIP_E_ARG, "ihip_model_frequencies: rotary dims or theta");
   std::vector<float> f;
   float rs;

@@ -2,10 +2,12 @@
 hold: rows beyond the step's, refusals."""
 import ctypes as C
 
+import numpy as np
 import pytest
 
 import infer_hip as H
 import oracle_lib as O
+from infer_hip import models
 from test_paged import A, attention, pages, qkrope, refused
 
 
@@ -60,3 +62,14 @@ def test_unaligned_numbers_refused(skew):
         refused(lambda: slots(**{name: A + skew}), -1, "4 bytes")
     for name in ("positions", "slots"):
         refused(lambda: qkrope(pages(), **{name: A + skew}), -1, "4 bytes")
+
+
+@pytest.mark.parametrize("dims,head_dim", [(66, 64), (2 ** 31 - 2, 64), (0, 514), (514, 514), (0, 2 ** 31 - 2), (0, 0),
+                                           (0, -64), (0, 63), (63, 64)])
+def test_frequencies_refused(dims, head_dim):
+    """The shares of a head that a model is refused for, before anything of their size is allocated."""
+    spec = models.Spec(models.tiny("qwen3-0.6b-q8_0", layers=1, vocab=64), seed=3)
+    spec.struct.rope_dims, spec.struct.head_dim = dims, head_dim
+    f = np.zeros(256, np.float32)
+    refused(lambda: H.lib().ihip_model_frequencies(C.addressof(spec.struct), f.ctypes.data, None), -1, "frequencies")
+    assert (f == 0).all()
