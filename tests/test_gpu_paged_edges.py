@@ -268,3 +268,77 @@ def test_two_contexts_at_once(ctx):
             want, tol = b.want()
             assert_close(b.read(), want, tol)
         ctx.sync()
+
+
+@pytest.mark.parametrize("rows", [40, 9000])
+def test_slots_windows_released(ctx, dev, rows):
+    """Sequences of which only the last pages are left in a small pool, the others released by the host:
+    the entries of those that end pass the pool's size many times, their pages come back all."""
+    rng = np.random.default_rng(rows)
+    n, ps, width, keep = 20, 16, 700, 6
+    pages = n * keep + 30
+    past = rng.integers(9000, 11000, n).astype(np.int32)
+    have = -(-past // ps)
+    order = rng.permutation(pages).astype(np.int32)
+    table = np.full((n, width), -1, np.int32)
+    for s in range(n):
+        table[s, have[s] - keep:have[s]] = order[s * keep:(s + 1) * keep]
+    ring = np.full(pages, -7, np.int32)
+    ring[:30] = order[n * keep:]
+    count = np.where(np.arange(n) % 3 == 0, -1, 1).astype(np.int32)
+    if rows > 4096:
+        count[1] = 100
+    ends = np.array([0, 30], np.int64)
+    want = plan_with_holes(past, count, table, ps, ring, ends, rows)
+    got = run_slots(ctx, dev, past, count, table, ps, ring, ends, rows)
+    assert want["ends"][1] == 30 + keep * 7
+    for k in want:
+        if k != "ring":
+            assert np.array_equal(got[k], want[k]), k
+    at = np.arange(*want["ends"]) % pages
+    assert np.array_equal(got["ring"][at], want["ring"][at])
+    used = got["table"][count >= 0]
+    used = used[(used >= 0) & (used < pages)]
+    assert sorted(np.concatenate([used, got["ring"][at]]).tolist()) == list(range(pages))
+
+
+@pytest.mark.parametrize("rows", [64, 5000])
+def test_slots_with_holes_captured(ctx, dev, rows):
+    """One graph over several batches, with holes and without, in place: what the blocks leave for each
+    other is as it was before."""
+    rng = np.random.default_rng(rows)
+    n, ps, width = 40, 4, 40
+    shape = dict(past=n, count=n, table=n * width, ring=2000, ends=2)
+    b = {k: dev.out(m * (8 if k == "ends" else 4)) for k, m in shape.items()}
+    o, q, s, f = dev.out(4 * n + 4), dev.out(4 * rows), dev.out(4 * rows), dev.out(4)
+
+    def step():
+        H.check(H.lib().ihip_enqueue_paged_slots(
+            ctx.h, b["past"].ptr, b["count"].ptr, n, b["table"].ptr, width, ps, b["ring"].ptr, 2000, b["ends"].ptr,
+            b["ends"].ptr, o.ptr, b["past"].ptr, q.ptr, s.ptr, rows, f.ptr))
+
+    H.check(H.lib().ihip_capture_begin(ctx.h))
+    step()
+    H.check(H.lib().ihip_capture_end(ctx.h, 13))
+    for i in range(8):
+        past, count = rng.integers(0, 120, n).astype(np.int32), rng.integers(-1, 20, n).astype(np.int32)
+        order = rng.permutation(2000).astype(np.int32)
+        table = order[:n * width].reshape(n, width).copy()
+        have = -(-past // ps)
+        table[np.arange(width) >= have[:, None]] = -1
+        if i % 3:
+            table[(rng.random(table.shape) < 0.3) & (count < 0)[:, None]] = 2 ** 31 - 1
+        ring, ends = np.full(2000, -7, np.int32), np.array([1900 + 2000 * i, 2300 + 2000 * i], np.int64)
+        ring[np.arange(*ends) % 2000] = order[n * width:]
+        for k, a in dict(past=past, count=count, table=table, ring=ring, ends=ends).items():
+            b[k].upload(a)
+        want = plan_with_holes(past, count, table, ps, ring, ends, rows)
+        H.check(H.lib().ihip_graph_launch(ctx.h, 13))
+        for k, d, dt in (("table", b["table"], np.int32), ("ends", b["ends"], np.int64), ("lengths", b["past"], np.int32),
+                         ("slots", s, np.int32), ("positions", q, np.int32), ("offsets", o, np.int32),
+                         ("failed", f, np.int32)):
+            assert np.array_equal(d.download(dt, want[k].size), want[k].ravel()), (i, k)
+        at = np.arange(*want["ends"]) % 2000
+        assert np.array_equal(b["ring"].download(np.int32, 2000)[at], want["ring"][at]), i
+        if i % 2:  # an eager call between the replays
+            run_slots(ctx, dev, past, count, table, ps, ring, ends, rows)
