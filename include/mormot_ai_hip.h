@@ -648,8 +648,9 @@ int ihip_enqueue_paged_slots(ihip_ctx* ctx, uint64_t past, uint64_t count, int64
 /* the new rows' (up to 2^23) q, k and v between the q/k/v Linear and the
  * attention: per row and head the RMSNorm of q and k heads (qn, kn device
  * [head_dim] or 0), rotary positions (rope, NULL: none), q written to q_out
- * ([rows, heads, head_dim], or 0: in place; elsewhere it does not overlap q), k
- * and v stored into the cache at the row's slot. Strides: floats from a row to the next (0: the rows are
+ * ([rows, heads, head_dim], or 0: in place; an output that overlaps q, k or v in
+ * another way than q's own contiguous rows is refused), k and v stored into the
+ * cache at the row's slot. Strides: floats from a row to the next (0: the rows are
  * contiguous). A row with position < 0 is left as it was; a slot outside the
  * pool stores nothing. The rows of one call have slots of their own: of two in
  * one slot either may stay, value by value. (ihip_enqueue_qkrope over a paged
@@ -663,10 +664,11 @@ int ihip_enqueue_paged_qkrope(ihip_ctx* ctx, uint64_t q, int64_t q_stride, uint6
  * head_dim] = softmax(scale q k) v over the keys 0 .. lengths[s] - 1 (window > 0:
  * the last `window` of them; sinks: device [heads] or 0; scale >= 0, 0: 1 /
  * sqrt(head_dim)); table [seqs, max_pages], q rows of q_stride floats (0: heads *
- * head_dim). A key whose table entry is outside the pool is not there, one whose
- * score is -infinity has weight 0, and so has a sink of -infinity. A sequence with
- * no key (length 0), or whose keys have no weight, gives zeros, one with lengths[s]
- * < 0 leaves its row of y as it was.
+ * head_dim); y may be q's own contiguous rows, and is refused where it overlaps
+ * them in another way. A key whose table entry is outside the pool is not there,
+ * one whose score is -infinity has weight 0, and so has a sink of -infinity. A
+ * sequence with no key (length 0), or whose keys have no weight, gives zeros, one
+ * with lengths[s] < 0 leaves its row of y as it was.
  * (ihip_enqueue_attention over a paged cache) */
 int ihip_enqueue_paged_attention(ihip_ctx* ctx, uint64_t q, int64_t q_stride,
                                  const ihip_pages* cache, uint64_t table, int64_t max_pages,

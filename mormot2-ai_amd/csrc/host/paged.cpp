@@ -39,6 +39,16 @@ int refuse(const char* who, const char* why, int code = IHIP_E_ARG)
 // floats from a row to the next: rows times it stay far from 64 bits
 constexpr int64_t STRIDE_MOST = (int64_t)1 << 36;
 
+// whether the bytes [a, a + n) meet any of the rows of `width` bytes at s, s + stride, ..
+bool overlaps(uint64_t a, __int128 n, uint64_t s, __int128 stride, __int128 width, int64_t rows)
+{
+  // row r is met where s + r stride < a + n and s + r stride + width > a
+  const __int128 d = (__int128)a - (__int128)s;
+  if (d + n <= 0 || (rows - 1) * stride + width <= d) return false;
+  const __int128 first = d < width ? 0 : (d - width) / stride + 1, last = (d + n - 1) / stride;
+  return first <= last && first < rows;
+}
+
 // a pool with its strides filled in
 struct Pool {
   int64_t page_stride = 0, slot_stride = 0, head_stride = 0;
@@ -136,6 +146,11 @@ int ihip_enqueue_paged_qkrope(ihip_ctx* c, uint64_t q, int64_t q_stride, uint64_
   if (std::max({q_stride, k_stride, v_stride}) > STRIDE_MOST) return refuse(who, "a stride beyond 2^36");
   const uint64_t aligned = q | k | v | q_out | qn | kn;
   if ((aligned | positions | slots) % 4) return refuse(who, "arrays aligned to 4 bytes");
+  // (a row's values are read and written by several blocks and waves in any order)
+  const __int128 out = (__int128)rows * qw * 4;
+  if (q_out && ((overlaps(q_out, out, q, q_stride * 4, qw * 4, rows) && !(q_out == q && q_stride == qw)) ||
+                overlaps(q_out, out, k, k_stride * 4, kw * 4, rows) || overlaps(q_out, out, v, v_stride * 4, kw * 4, rows)))
+    return refuse(who, "q_out overlaps q, k or v, and is not q's contiguous rows");
   if (!(eps >= 0) || !std::isfinite(eps)) return refuse(who, "eps");
   int64_t dims = 0;
   if (rope) {
@@ -203,6 +218,9 @@ int ihip_enqueue_paged_attention_at(ihip_ctx* c, uint64_t q, int64_t q_stride, c
   if (q_stride < heads * hd) return refuse(who, "a stride below a row");
   if (q_stride > STRIDE_MOST) return refuse(who, "a stride beyond 2^36");
   if ((q | y | sinks | lengths | offsets | table) % 4) return refuse(who, "arrays aligned to 4 bytes");
+  if (overlaps(y, (__int128)rows * heads * hd * 4, q, q_stride * 4, heads * hd * 4, rows) &&
+      !(y == q && q_stride == heads * hd))
+    return refuse(who, "y overlaps q, and is not q's contiguous rows");
   // (the kernel's scores are in base 2, in single)
   const float scale2 = (float)((scale != 0 ? scale : 1.0 / std::sqrt((double)hd)) * 1.4426950408889634);
   if (!(scale >= 0) || !std::isfinite(scale2)) return refuse(who, "scale is 0 or positive, times log2 e within single");

@@ -342,3 +342,23 @@ def test_slots_with_holes_captured(ctx, dev, rows):
         assert np.array_equal(b["ring"].download(np.int32, 2000)[at], want["ring"][at]), i
         if i % 2:  # an eager call between the replays
             run_slots(ctx, dev, past, count, table, ps, ring, ends, rows)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16", "f32"])
+def test_attention_in_place(ctx, dev, dtype):
+    """y in q's own rows: whole pieces, split ones, rows without a key, and one with an infinity."""
+    rng = np.random.default_rng(23)
+    b = Batch(rng, dtype, 128, 40, 2, 16, [50, 0, 9000, 1, -1, 70])
+    b.k[b.table[5, 0], 3, 0, 9] = np.inf
+    apart = b.run(ctx, dev)
+    y = dev.out(b.q.nbytes)
+    y.upload(b.q)
+    b.dq, b.y = y.ptr, y
+    b.enqueue(ctx)
+    got = b.read()
+    # bit for bit, NaN among them, and the place that is passed over holds its query
+    assert np.array_equal(got[[0, 1, 2, 3, 5]].view(np.uint32), apart[[0, 1, 2, 3, 5]].view(np.uint32))
+    assert np.array_equal(got[4], b.q[4])
+    nan = np.zeros(40, bool)
+    nan[:20] = b.q[5, :20, 9] > 0  # (a score of infinity; of -infinity the key has no weight)
+    assert np.isnan(got[5][nan]).all() and np.isfinite(got[5][~nan]).all() and 0 < nan.sum() < 20

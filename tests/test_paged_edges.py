@@ -73,3 +73,32 @@ def test_frequencies_refused(dims, head_dim):
     f = np.zeros(256, np.float32)
     refused(lambda: H.lib().ihip_model_frequencies(C.addressof(spec.struct), f.ctypes.data, None), -1, "frequencies")
     assert (f == 0).all()
+
+
+# (addresses of rows of 4 heads of 64 and 2 KV heads each of k and v: 256, 128 and 128 floats)
+W = 4 * 512
+
+
+@pytest.mark.parametrize("where,strides,ok", [
+    (A, 0, True), (A, 512, False), (A + 1024, 0, False), (A - 1024, 0, False), (A + 4, 0, False),
+    (A + 5 * 1024, 0, True), (A - 5 * 1024, 0, True), (A + W - 4, 512, False), (A + 5 * W, 512, True),
+    (A + 4 * W + 3 * 512, 512, False), (A + 4 * W + 4 * 512, 512, True), (A + 2048, 2048, True), (A + 1024, 2048, False),
+    (A + 8192 - 5 * 1024, 2048, True), (A + 8192 - 5 * 1024 + 4, 2048, False), (A + 4 * 8192 + 2048, 2048, True)])
+def test_qkrope_outputs_over_inputs(where, strides, ok):
+    """q_out is q's own rows, contiguous, or apart from q, k and v: rows of a call are turned at once."""
+    kw = dict(qs=strides, ks=strides, vs=strides, k=A + 1024, v=A + 1536) if strides else dict(k=A << 1, v=A << 2)
+    refused(lambda: qkrope(pages(), out=where, **kw), -1, "no context" if ok else "q_out")
+
+
+def test_qkrope_output_over_keys():
+    for name in ("k", "v"):
+        refused(lambda: qkrope(pages(), q=A << 3, k=A << 4, v=A << 5, out=(A << (4 if name == "k" else 5)) + 512), -1, "q_out")
+    refused(lambda: qkrope(pages(), q=A << 3, k=A << 4, v=A << 5, out=A << 6), -1, "no context")
+
+
+@pytest.mark.parametrize("where,stride,ok", [
+    (A, 0, True), (A, 256, True), (A, 512, False), (A + 1024, 0, False), (A - 1024, 256, False), (A + 3 * 1024, 0, True),
+    (A - 3 * 1024, 0, True), (A + 1024, 512, False), (A + 1024, 1024, True), (A + 2 * 4096 + 1024, 1024, True)])
+def test_attention_output_over_queries(where, stride, ok):
+    """y is q's own rows, contiguous, or apart from them."""
+    refused(lambda: attention(pages(), y=where, q_stride=stride), -1, "no context" if ok else "y overlaps")
