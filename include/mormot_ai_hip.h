@@ -637,7 +637,8 @@ int ihip_model_frequencies(const ihip_model_desc* desc, float* freq, double* sca
  *   sequence leave none for those behind it that need one. The rows of such a
  *   sequence are in the step all the same: nothing is stored for them, and the
  *   attention answers the last of them from the keys that the sequence had. The
- *   host drops what comes of them (the rows with a position and no slot).
+ *   host drops what comes of them (the rows with a position and no slot). A
+ *   sequence without new tokens counts too where the rows before it pass `rows`.
  * ends_out may be ends, and lengths may be past. */
 #define IHIP_PAGED_SEQS 4096
 int ihip_enqueue_paged_slots(ihip_ctx* ctx, uint64_t past, uint64_t count, int64_t seqs,
