@@ -584,18 +584,28 @@ int ihip_prompt_cache_stats(ihip_prompt_cache* pc, int64_t* requests, int64_t* h
  * outside the pool is read as "not there", never followed.
  * ==================================================================== */
 
+/* 8-bit pages (ihip_pages.dtype alone, not an element type of tensors): the values
+ * of a head of a token are int8 codes times one single scale, 1 / 127 of the head's
+ * largest magnitude; 0.52 of a half's bytes for heads of 128 */
+#define IHIP_Q8_HEAD 64
+
 /* the pool of one layer. A slot is page * page_size + token: the values of a
  * token's KV head h start at page * page_stride + token * slot_stride + h *
  * head_stride. Strides in values, 0 for those of [pages, page_size, kv_heads,
  * head_dim]; [pages, kv_heads, page_size, head_dim] has head_stride
  * page_size * head_dim and slot_stride head_dim. head_dim is a multiple of 8,
- * up to 512; the addresses and strides are multiples of 16 bytes. */
+ * up to 512; the addresses and strides are multiples of 16 bytes. 8-bit pages:
+ * head_dim a multiple of 16 and strides of head_dim; the scale of the head whose
+ * values start at offset o is at o / head_dim, so that the scales lie as the heads do
+ * ([pages, page_size, kv_heads] with strides 0). */
 typedef struct {
   uint64_t k, v;           /* device addresses of the keys and the values */
   int64_t pages;
   int64_t page_stride, slot_stride, head_stride;
   int32_t page_size, kv_heads, head_dim;
-  int32_t dtype;           /* IHIP_F32, IHIP_F16 or IHIP_BF16 */
+  int32_t dtype;           /* IHIP_F32, IHIP_F16, IHIP_BF16 or IHIP_Q8_HEAD */
+  /* of IHIP_Q8_HEAD (not read for the others): device addresses of the scales */
+  uint64_t k_scale, v_scale;
 } ihip_pages;
 
 /* rotary positions of q and k: value pairs (i, i + dims / 2) of a head's
@@ -654,8 +664,10 @@ int ihip_enqueue_paged_slots(ihip_ctx* ctx, uint64_t past, uint64_t count, int64
  * cache at the row's slot. Strides: floats from a row to the next (0: the rows are
  * contiguous). A row with position < 0 is left as it was; a slot outside the
  * pool stores nothing. The rows of one call have slots of their own: of two in
- * one slot either may stay, value by value. (ihip_enqueue_qkrope over a paged
- * cache) */
+ * one slot either may stay, value by value (of 8-bit pages codes of one and the scale
+ * of the other). In 8-bit pages a code is the whole number nearest to its value over the
+ * scale (the even one between two); a NaN or an infinity makes the scale of its head
+ * NaN. (ihip_enqueue_qkrope over a paged cache) */
 int ihip_enqueue_paged_qkrope(ihip_ctx* ctx, uint64_t q, int64_t q_stride, uint64_t k,
                               int64_t k_stride, uint64_t v, int64_t v_stride, int64_t rows,
                               int64_t heads, uint64_t qn, uint64_t kn, double eps,
@@ -684,6 +696,18 @@ int ihip_enqueue_paged_attention_at(ihip_ctx* ctx, uint64_t q, int64_t q_stride,
                                     uint64_t lengths, uint64_t offsets, int64_t rows, uint64_t y,
                                     int64_t seqs, int64_t heads, int64_t window, uint64_t sinks,
                                     double scale);
+/* cached tokens read back as contiguous rows, as the caches of
+ * ihip_enqueue_attention and ihip_enqueue_qkrope hold them (a prompt's next chunk over
+ * a history in pages, a sequence that leaves the pool): row r of k_out and v_out ([rows,
+ * kv_heads, head_dim] of out_type, IHIP_F32 or IHIP_F16, aligned to 16 bytes) is token
+ * first[s] + r - offsets[s] of sequence s, the one with offsets[s] <= r < offsets[s + 1]
+ * (offsets [seqs + 1], ascending; first [seqs], 0: from token 0; table [seqs,
+ * max_pages]). A token whose table entry is outside the pool or the table reads as
+ * zeros; rows before the first sequence's and behind the last one's are left as they
+ * were. Rows that overlap each other or the cache are refused. */
+int ihip_enqueue_paged_read(ihip_ctx* ctx, const ihip_pages* cache, uint64_t table, int64_t max_pages,
+                            uint64_t first, uint64_t offsets, int64_t seqs, int64_t rows, int out_type,
+                            uint64_t k_out, uint64_t v_out);
 /* what a row of logits says of its tokens: logits [rows, vocab] (vocab up to
  * 2^22, rows to 2^24), `stride` floats from a row to the next (0: vocab);
  * - logprobs [rows] (or 0): log softmax of token ids[r] (int32), NaN for an id

@@ -49,25 +49,39 @@ bool overlaps(uint64_t a, __int128 n, uint64_t s, __int128 stride, __int128 widt
   return first <= last && first < rows;
 }
 
-// a pool with its strides filled in
+// a pool with its strides filled in, in values and in scales (of 8-bit pages)
 struct Pool {
   int64_t page_stride = 0, slot_stride = 0, head_stride = 0;
+  int64_t s_page = 0, s_slot = 0, s_head = 0;
+  int64_t es = 0;  // bytes of a value
   const char* type = "";
 };
 
-const char* type_name(int t) { return t == IHIP_F32 ? "f32" : t == IHIP_F16 ? "f16" : t == IHIP_BF16 ? "bf16" : nullptr; }
+const char* type_name(int t)
+{
+  return t == IHIP_F32 ? "f32" : t == IHIP_F16 ? "f16" : t == IHIP_BF16 ? "bf16" : t == IHIP_Q8_HEAD ? "q8" : nullptr;
+}
+
+// the scales of a pool's keys or values (the fields of other pools are not looked at)
+uint64_t q8_scales(const ihip_pages* p, int values)
+{
+  return p->dtype != IHIP_Q8_HEAD ? 0 : values ? p->v_scale : p->k_scale;
+}
 
 int check_pool(const char* who, const ihip_pages* p, Pool* out)
 {
   if (!p || !p->k || !p->v) return refuse(who, "no cache");
   out->type = type_name(p->dtype);
-  if (!out->type) return refuse(who, "a cache that is not F32, F16 or BF16", IHIP_E_UNSUPPORTED);
+  if (!out->type) return refuse(who, "a cache that is not F32, F16 or BF16, nor Q8_HEAD", IHIP_E_UNSUPPORTED);
   if (p->head_dim < 8 || p->head_dim > 512 || p->head_dim % 8)
     return refuse(who, "head_dim is a multiple of 8 up to 512", IHIP_E_UNSUPPORTED);
+  const bool q8 = p->dtype == IHIP_Q8_HEAD;
+  if (q8 && p->head_dim % 16) return refuse(who, "head_dim of 8-bit pages is a multiple of 16", IHIP_E_UNSUPPORTED);
   if (p->kv_heads < 1 || p->kv_heads > 65535 || p->page_size < 1 || p->pages < 1 ||
       p->pages > INT32_MAX / p->page_size)
     return refuse(who, "kv_heads, page_size or pages out of range");
-  const int64_t row = (int64_t)p->kv_heads * p->head_dim, es = p->dtype == IHIP_F32 ? 4 : 2;
+  const int64_t row = (int64_t)p->kv_heads * p->head_dim, es = p->dtype == IHIP_F32 ? 4 : q8 ? 1 : 2;
+  out->es = es;
   out->head_stride = p->head_stride ? p->head_stride : p->head_dim;
   out->slot_stride = p->slot_stride ? p->slot_stride : row;
   out->page_stride = p->page_stride ? p->page_stride : row * p->page_size;
@@ -78,6 +92,15 @@ int check_pool(const char* who, const ihip_pages* p, Pool* out)
   if (out->slot_stride * (p->page_size - 1) + out->head_stride * (p->kv_heads - 1) + p->head_dim > INT32_MAX)
     return refuse(who, "a page of more than 2^31 values");
   if (p->k % 16 || p->v % 16) return refuse(who, "a cache that is not aligned to 16 bytes");
+  if (q8) {
+    if (!p->k_scale || !p->v_scale || (p->k_scale | p->v_scale) % 4)
+      return refuse(who, "8-bit pages without scales, or scales not aligned to 4 bytes");
+    if (out->head_stride % p->head_dim || out->slot_stride % p->head_dim || out->page_stride % p->head_dim)
+      return refuse(who, "a stride of 8-bit pages that is no multiple of head_dim");
+    out->s_page = out->page_stride / p->head_dim;
+    out->s_slot = out->slot_stride / p->head_dim;
+    out->s_head = out->head_stride / p->head_dim;
+  }
   return 0;
 }
 
@@ -171,6 +194,8 @@ int ihip_enqueue_paged_qkrope(ihip_ctx* c, uint64_t q, int64_t q_stride, uint64_
     int64_t pages, page_stride, slot_stride, head_stride;
     double eps, scale;
     int32_t rows, heads, kvh, hd, page_size, half, interleaved, wide, seg, parts;
+    uint64_t ks, vs;  // (of 8-bit pages' kernel alone, as what follows)
+    int64_t s_page, s_slot, s_head;
   } a = {(const float*)q, (const float*)k, (const float*)v, (float*)(q_out ? q_out : q), (const float*)qn,
          (const float*)kn, (const float*)(rope ? rope->freq : 0), (const int*)positions, (const int*)slots,
          (char*)cache->k, (char*)cache->v, q_stride, k_stride, v_stride, q_out ? qw : q_stride,
@@ -180,7 +205,7 @@ int ihip_enqueue_paged_qkrope(ihip_ctx* c, uint64_t q, int64_t q_stride, uint64_
          // 16-byte loads: rows aligned, and no unit of 4 pairs that only half turns
          aligned % 16 == 0 && (q_stride | k_stride | v_stride) % 4 == 0 &&
              (!rope || rope->interleaved || dims % 8 == 0),
-         1, 1};
+         1, 1, q8_scales(cache, 0), q8_scales(cache, 1), p.s_page, p.s_slot, p.s_head};
   while (a.seg * 8 < hd) a.seg *= 2;  // lanes of a head: 8 values each
   const int64_t lanes = (heads + 2 * kvh) * a.seg;
   // a block of 256 lanes a row (512 lanes, which leave no remainder, take 66 us for
@@ -224,8 +249,8 @@ int ihip_enqueue_paged_attention_at(ihip_ctx* c, uint64_t q, int64_t q_stride, c
   // (the kernel's scores are in base 2, in single)
   const float scale2 = (float)((scale != 0 ? scale : 1.0 / std::sqrt((double)hd)) * 1.4426950408889634);
   if (!(scale >= 0) || !std::isfinite(scale2)) return refuse(who, "scale is 0 or positive, times log2 e within single");
-  // the kernels take tiles of 128 keys of 16-bit caches, 64 of single ones, half as
-  // many of heads beyond 256
+  // the kernels take tiles of 128 keys of 16-bit and 8-bit caches, 64 of single ones,
+  // half as many of heads beyond 256
   const int64_t group = heads / kvh, tiles = (group + 15) / 16;
   const int64_t tk = (cache->dtype == IHIP_F32 ? 64 : 128) / (hd > 256 ? 2 : 1);
   const int64_t keys = window > 0 ? std::min(window, max_pages * cache->page_size) : max_pages * cache->page_size;
@@ -244,13 +269,15 @@ int ihip_enqueue_paged_attention_at(ihip_ctx* c, uint64_t q, int64_t q_stride, c
     int64_t q_stride, pages, page_stride, slot_stride, head_stride, window;
     float scale;
     int32_t seqs, heads, kvh, hd, page_size, max_pages, group, tiles, rows, cus;
+    uint64_t ks, vs;  // (of 8-bit pages' kernel alone, as what follows)
+    int64_t s_page, s_slot, s_head;
   } a = {(const float*)q, (const char*)cache->k, (const char*)cache->v, (const int*)table,
          (const int*)lengths, (const int*)offsets, (float*)y, (const float*)sinks, (float*)c->paged_part,
          (int*)(c->paged_part + PAGED_PART_BYTES), q_stride, cache->pages, p.page_stride,
          p.slot_stride, p.head_stride, window,
          scale2, (int32_t)seqs,
          (int32_t)heads, (int32_t)kvh, (int32_t)hd, cache->page_size, (int32_t)max_pages, (int32_t)group,
-         (int32_t)tiles, (int32_t)rows, c->cus};
+         (int32_t)tiles, (int32_t)rows, c->cus, q8_scales(cache, 0), q8_scales(cache, 1), p.s_page, p.s_slot, p.s_head};
   const int d = hd <= 64 ? 64 : hd <= 128 ? 128 : hd <= 256 ? 256 : 512;
   char name[40];
   snprintf(name, sizeof name, "paged_attention_%s_%d%s", p.type, d, hd == d ? "" : "_part");
@@ -258,6 +285,47 @@ int ihip_enqueue_paged_attention_at(ihip_ctx* c, uint64_t q, int64_t q_stride, c
   int64_t blocks = (int64_t)c->cus * resident_blocks(c, name, 256);
   blocks = std::min<int64_t>({blocks, PAGED_BLOCKS, (int64_t)(PAGED_PART_BYTES / (2 * (16 * hd + 32) * 4)), units * seqs});
   return launch(c, name, dim3((unsigned)blocks), dim3(256), &a);
+}
+
+int ihip_enqueue_paged_read(ihip_ctx* c, const ihip_pages* cache, uint64_t table, int64_t max_pages,
+                            uint64_t first, uint64_t offsets, int64_t seqs, int64_t rows, int out_type,
+                            uint64_t k_out, uint64_t v_out)
+{
+  const char* who = "ihip_enqueue_paged_read";
+  Pool p;
+  if (int rc = check_pool(who, cache, &p)) return rc;
+  if (!table || !offsets || !k_out || !v_out) return refuse(who, "a missing array");
+  if (out_type != IHIP_F32 && out_type != IHIP_F16) return refuse(who, "rows are F32 or F16", IHIP_E_UNSUPPORTED);
+  if (seqs > IHIP_PAGED_SEQS) return refuse(who, "more sequences than IHIP_PAGED_SEQS", IHIP_E_NOMEM);
+  if (seqs < 1 || rows < 1 || rows > INT32_MAX || max_pages < 1 || max_pages > INT32_MAX / cache->page_size)
+    return refuse(who, "seqs, rows or max_pages out of range");
+  if ((table | first | offsets) % 4) return refuse(who, "arrays aligned to 4 bytes");
+  if ((k_out | v_out) % 16) return refuse(who, "rows aligned to 16 bytes");
+  const int64_t hd = cache->head_dim, kvh = cache->kv_heads, width = kvh * hd, os = out_type == IHIP_F32 ? 4 : 2;
+  const __int128 out = (__int128)rows * width * os;
+  const __int128 held = ((__int128)(cache->pages - 1) * p.page_stride + p.slot_stride * (cache->page_size - 1) + p.head_stride * (kvh - 1) + hd) * p.es;
+  const __int128 scales = held / (p.es * hd) * 4;
+  auto meets = [](__int128 a, __int128 n, __int128 b, __int128 m) { return a < b + m && b < a + n; };
+  bool over = meets(k_out, out, v_out, out);
+  for (uint64_t o : {k_out, v_out})
+    over |= meets(o, out, cache->k, held) || meets(o, out, cache->v, held) ||
+            (cache->dtype == IHIP_Q8_HEAD && (meets(o, out, cache->k_scale, scales) || meets(o, out, cache->v_scale, scales)));
+  if (over) return refuse(who, "rows that overlap each other or the cache");
+  if (!c) return no_context(who);
+  OnDevice on(c);
+  struct {
+    uint64_t kc, vc, ks, vs, table, first, offsets, k_out, v_out;
+    int64_t pages, page_stride, slot_stride, head_stride, s_page, s_slot, s_head;
+    int32_t rows, seqs, max_pages, page_size, hd, units, chunk;
+  } a = {cache->k, cache->v, q8_scales(cache, 0), q8_scales(cache, 1), table, first, offsets, k_out, v_out,
+         cache->pages, p.page_stride, p.slot_stride, p.head_stride, p.s_page, p.s_slot, p.s_head,
+         (int32_t)rows, (int32_t)seqs, (int32_t)max_pages, cache->page_size, (int32_t)hd, (int32_t)(width * os / 16), 1};
+  // a wave's rows: as many as leave 16 waves a CU, up to 16
+  a.chunk = (int32_t)std::max<int64_t>(1, std::min<int64_t>(16, rows / (16 * c->cus)));
+  const int64_t turns = (rows + a.chunk - 1) / a.chunk;
+  char name[32];
+  snprintf(name, sizeof name, "paged_read_%s_%s", p.type, out_type == IHIP_F32 ? "f32" : "f16");
+  return launch(c, name, dim3((unsigned)std::min<int64_t>((turns + 3) / 4, 64 * c->cus)), dim3(256), &a);
 }
 
 int ihip_enqueue_logprobs(ihip_ctx* c, uint64_t logits, int64_t rows, int64_t vocab, int64_t stride,

@@ -1,7 +1,10 @@
 // paged.hip - several sequences decoded together over one paged cache: the
 // plan of a step, q/k/v of the new rows into the pages, attention over them.
+#include <type_traits>
+
 #include "common.h"
 #include "../paged.h"
+#include "paged_attention.h"
 
 using namespace ihip;
 
@@ -389,6 +392,12 @@ struct PagedRopeArgs {
   int32_t parts;        // blocks of a row
 };
 
+// 8-bit pages: codes in kc and vc, single scales of a token's heads
+struct PagedRope8Args : PagedRopeArgs {
+  float *ks, *vs;
+  int64_t s_page, s_slot, s_head;
+};
+
 // cosine and sine of an angle of up to 2^31 radians, in double: the angle less
 // its nearest multiple of pi / 2 (the product exact in the fused steps, pi / 2 in
 // two parts), then their Taylor series on [-pi / 4, pi / 4], whose first left-out
@@ -427,6 +436,41 @@ __device__ __forceinline__ uint16_t float_to_bf16(float f)
   return (uint16_t)((b + 0x7fffu + ((b >> 16) & 1u)) >> 16);
 }
 
+// 8 values of a head in `seg` lanes as codes, and the scale by which they count: 1 / 127
+// of the head's largest magnitude, in single. A code is the nearest whole number to its
+// value over the scale, the even one between two (the division of doubles is exact to
+// its last place, so that a tie is one). Codes pass 127 only where the scale is subnormal
+// and was rounded down by more than one in 254: they are cut to it. A NaN or an infinity
+// makes the scale NaN, and the head reads as NaN.
+__device__ __forceinline__ uint2 codes8(const double (&x)[8], bool on, int seg, float& scale)
+{
+  double m = 0;
+#pragma unroll
+  for (int j = 0; j < 8; j++) {
+    const double v = on ? fabs(x[j]) : 0.0;
+    m = v > m || v != v ? v : m;
+  }
+  auto top = [&](double o) { m = o > m || o != o ? o : m; };
+  if (seg > 1) top(xpart<1>(m));
+  if (seg > 2) top(xpart<2>(m));
+  if (seg > 4) top(xpart<4>(m));
+  if (seg > 8) top(xpart<8>(m));
+  if (seg > 16) top(xpart<16>(m));
+  if (seg > 32) top(xpart<32>(m));
+  scale = (float)(m / 127.0);
+  const bool bad = (float_bits(scale) & 0x7f800000u) == 0x7f800000u;
+  if (bad) scale = bits_float(0x7fc00000u);
+  uint32_t b[2] = {0, 0};
+  if (!bad && scale != 0.f) {
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      const double c = fmin(fmax(rint(x[j] / (double)scale), -127.0), 127.0);
+      b[j / 4] |= ((uint32_t)(int)c & 255u) << (8 * (j & 3));
+    }
+  }
+  return make_uint2(b[0], b[1]);
+}
+
 // consecutive values of a cache row; T: 0 float, 1 half, 2 bf16
 template <int T>
 __device__ __forceinline__ void store4(char* p, const float (&v)[4])
@@ -452,13 +496,15 @@ __device__ __forceinline__ void store1(char* p, float v)
 // the norm is a sum over aligned lanes. Sums, angles and the rotation are in
 // double (full rate on this chip) and rounded once to single, then to the
 // cache's type (halves and bf16 so in two steps, a 2^-13 or 2^-16 of a step more
-// than in one). Bound by HBM: 4 bytes in and 4 (q) or the cache's (k, v) out; 8000
+// than in one; 8-bit codes from the doubles, codes8, a head's values in order through
+// LDS where its pairs lie in two halves). Bound by HBM: 4 bytes in and 4 (q) or the cache's (k, v) out; 8000
 // rows of 64 + 8 heads of 64 into a bf16 cache 59 us (5.2 TB/s, beside 4.7 of a large
 // copy), 32 rows of 32 + 4 heads of 128 4.8 us (launch and two round trips).
-template <int T>
-__device__ __forceinline__ void paged_qkrope_t(const PagedRopeArgs& a)
+template <int T, typename A>
+__device__ __forceinline__ void paged_qkrope_t(const A& a)
 {
-  constexpr int ES = T == 0 ? 4 : 2;
+  constexpr int ES = T == 0 ? 4 : T == 3 ? 1 : 2;
+  typedef typename std::conditional<T == 3, double, float>::type real;  // a turned value
   __shared__ double2 cs[256];
   const int row = blockIdx.x, t = threadIdx.x;
   const int pos = a.positions[row];
@@ -521,28 +567,59 @@ __device__ __forceinline__ void paged_qkrope_t(const PagedRopeArgs& a)
         if (on) s = __builtin_fma((double)x[j], (double)x[j], s);
       inv = 1.0 / sqrt(wave_sum(s, seg) / (double)hd + a.eps);
     }
-    if (!on) continue;
-    float o[8];
+    if (T != 3 && !on) continue;
+    real o[8];
 #pragma unroll
     for (int j = 0; j < 4; j++) {
       const double x0 = (double)x[2 * j] * inv * (double)wv[2 * j];
       const double x1 = (double)x[2 * j + 1] * inv * (double)wv[2 * j + 1];
       const bool rot = 4 * u + j < half;
       const double2 e = rot ? cs[4 * u + j] : make_double2(1.0, 0.0);
-      o[2 * j] = rot ? (float)(x0 * e.x - x1 * e.y) : (float)x0;
-      o[2 * j + 1] = rot ? (float)(x1 * e.x + x0 * e.y) : (float)x1;
+      o[2 * j] = rot ? (real)(x0 * e.x - x1 * e.y) : (real)x0;
+      o[2 * j + 1] = rot ? (real)(x1 * e.x + x0 * e.y) : (real)x1;
+    }
+    if constexpr (T == 3) {
+      if (kind != 0) {
+        __shared__ double line[256 * 8];
+        if (half && !a.interleaved) {
+          // (a head's lanes are a wave's)
+#pragma unroll
+          for (int j = 0; j < 8; j++)
+            if (on) line[(t - u) * 8 + at(j / 2, j & 1)] = o[j];
+          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+          __builtin_amdgcn_wave_barrier();
+#pragma unroll
+          for (int j = 0; j < 8; j++)
+            if (on) o[j] = line[t * 8 + j];
+          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+          __builtin_amdgcn_wave_barrier();
+        }
+        float scale;
+        const uint2 codes = codes8(o, on, seg, scale);
+        if (on && base >= 0) {
+          *(uint2*)((kind == 1 ? a.kc : a.vc) + base + hh * a.head_stride + 8 * u) = codes;
+          if (u == 0)
+            (kind == 1 ? a.ks : a.vs)[paged_slot_value(a.slots[row], a.page_size, a.pages, a.s_page, a.s_slot) + hh * a.s_head] = scale;
+        }
+        continue;
+      }
+      if (!on) continue;
     }
     if (kind == 0) {
       float* out = a.q_out + row * a.out_stride + hh * hd;
       if (a.wide) {
         const int i0 = split ? 4 * u : 8 * u, i1 = split ? half + 4 * u : 8 * u + 4;
-        *(float4*)(out + i0) = split ? make_float4(o[0], o[2], o[4], o[6]) : make_float4(o[0], o[1], o[2], o[3]);
-        *(float4*)(out + i1) = split ? make_float4(o[1], o[3], o[5], o[7]) : make_float4(o[4], o[5], o[6], o[7]);
+        float f[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) f[j] = (float)o[j];
+        *(float4*)(out + i0) = split ? make_float4(f[0], f[2], f[4], f[6]) : make_float4(f[0], f[1], f[2], f[3]);
+        *(float4*)(out + i1) = split ? make_float4(f[1], f[3], f[5], f[7]) : make_float4(f[4], f[5], f[6], f[7]);
       } else {
 #pragma unroll
-        for (int j = 0; j < 8; j++) out[at(j / 2, j & 1)] = o[j];
+        for (int j = 0; j < 8; j++) out[at(j / 2, j & 1)] = (float)o[j];
       }
-    } else if (base >= 0) {
+    } else if constexpr (T != 3) {
+      if (base < 0) continue;
       char* out = (kind == 1 ? a.kc : a.vc) + (base + hh * a.head_stride) * ES;
       if (a.wide) {
         const int i0 = split ? 4 * u : 8 * u, i1 = split ? half + 4 * u : 8 * u + 4;
@@ -561,742 +638,114 @@ __device__ __forceinline__ void paged_qkrope_t(const PagedRopeArgs& a)
 extern "C" __global__ __launch_bounds__(256) void paged_qkrope_f32(PagedRopeArgs a) { paged_qkrope_t<0>(a); }
 extern "C" __global__ __launch_bounds__(256) void paged_qkrope_f16(PagedRopeArgs a) { paged_qkrope_t<1>(a); }
 extern "C" __global__ __launch_bounds__(256) void paged_qkrope_bf16(PagedRopeArgs a) { paged_qkrope_t<2>(a); }
+extern "C" __global__ __launch_bounds__(256) void paged_qkrope_q8(PagedRope8Args a) { paged_qkrope_t<3>(a); }
+
+// -------------------------------------------------------------- paged_read
+struct PagedReadArgs {
+  const char *kc, *vc;
+  const float *ks, *vs;
+  const int *table, *first, *offsets;
+  char *k_out, *v_out;
+  int64_t pages, page_stride, slot_stride, head_stride, s_page, s_slot, s_head;
+  int32_t rows, seqs, max_pages, page_size, hd, units, chunk;  // units of 16 bytes of a row's output, rows of a wave's turn
+};
+
+// The cached tokens of sequences as rows of single or half values. A wave takes `chunk`
+// rows a turn, one a lane, for the rows' places (the sequence by search, its table's
+// entry), then walks the rows' units, 16 bytes of output a lane, so that stores are
+// contiguous and loads too within a head. Bound by HBM, mostly by what it writes.
+template <int T, int OUT>
+__device__ __forceinline__ void paged_read_t(const PagedReadArgs& a)
+{
+  constexpr int ES = T == 0 ? 4 : T == 3 ? 1 : 2, N = OUT == 0 ? 4 : 8;
+  const int lane = threadIdx.x & 63;
+  const int waves = gridDim.x * 4, wave = blockIdx.x * 4 + (threadIdx.x >> 6);
+  const uint32_t units = a.units;
+  for (int64_t r0 = (int64_t)wave * a.chunk; r0 < a.rows; r0 += (int64_t)waves * a.chunk) {
+    const int n = (int)min((int64_t)a.chunk, a.rows - r0);
+    // the lane's row: its place in values and in scales, -1 nothing there, -2 no row of the call
+    int64_t at = -2, sat = 0;
+    if (lane < n) {
+      const int row = (int)r0 + lane;
+      if (row >= a.offsets[0] && row < a.offsets[a.seqs]) {
+        const int s = slot_find(a.offsets, a.seqs, row);
+        const int64_t pos = (int64_t)(a.first ? a.first[s] : 0) + ((int64_t)row - a.offsets[s]);
+        at = -1;
+        if (pos >= 0 && pos < (int64_t)a.max_pages * a.page_size) {
+          const int page = a.table[(int64_t)s * a.max_pages + (uint32_t)pos / (uint32_t)a.page_size];
+          const int in = (int)((uint32_t)pos % (uint32_t)a.page_size);
+          at = paged_value(page, in, a.pages, a.page_stride, a.slot_stride);
+          if (T == 3 && at >= 0) sat = page * a.s_page + (int64_t)in * a.s_slot;
+        }
+      }
+    }
+    const uint32_t all = n * units;
+    // 4 units a lane on their way at once, of k and of v
+    for (uint32_t i0 = 0; i0 < all; i0 += 256) {
+      uint64_t raw[2][4][T == 3 ? 1 : N * ES / 8];
+      float sc[2][4];
+      int64_t to[4];
+      bool there[4];
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        const uint32_t i = min(i0 + 64 * e + lane, all - 1), r = i / units, u = i - r * units;
+        const int64_t from = __shfl(at, r, 64), sfrom = T == 3 ? __shfl(sat, r, 64) : 0;
+        const uint32_t v = u * N, h = v / (uint32_t)a.hd, d = v - h * a.hd;
+        to[e] = i0 + 64 * e + lane < all && from != -2 ? (r0 + r) * (int64_t)units + u : -1;
+        there[e] = from >= 0;
+        const int64_t src = there[e] ? (from + h * a.head_stride + d) * ES : 0;
+#pragma unroll
+        for (int x = 0; x < 2; x++) {
+          const char* const p = (x ? a.vc : a.kc) + src;
+          if constexpr (T == 3) {
+            if constexpr (N == 4) raw[x][e][0] = *(const uint32_t*)p;
+            else raw[x][e][0] = *(const uint64_t*)p;
+            sc[x][e] = there[e] ? (x ? a.vs : a.ks)[sfrom + h * a.s_head] : 0.f;
+          } else {
+#pragma unroll
+            for (int j = 0; j < N * ES / 8; j++) raw[x][e][j] = ((const uint64_t*)p)[j];
+          }
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        if (to[e] < 0) continue;
+#pragma unroll
+        for (int x = 0; x < 2; x++) {
+          float f[N];
+#pragma unroll
+          for (int j = 0; j < N; j++) {
+            const uint32_t w = (uint32_t)(raw[x][e][j * ES / 8] >> (8 * (j * ES % 8)));
+            if constexpr (T == 0) f[j] = bits_float(w);
+            else if constexpr (T == 1) f[j] = half_to_float(w & 0xffffu);
+            else if constexpr (T == 2) f[j] = bits_float(w << 16);
+            else f[j] = (float)(int8_t)w * sc[x][e];
+            if (!there[e]) f[j] = 0.f;
+          }
+          char* const o = (x ? a.v_out : a.k_out) + to[e] * 16;
+          if constexpr (OUT == 0) {
+            *(float4*)o = make_float4(f[0], f[1], f[2], f[3]);
+          } else {
+            uint32_t h[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) h[j] = float_to_half(f[2 * j]) | (uint32_t)float_to_half(f[2 * j + 1]) << 16;
+            *(uint4*)o = make_uint4(h[0], h[1], h[2], h[3]);
+          }
+        }
+      }
+    }
+  }
+}
+
+#define PAGED_READ(NAME, T)                                                                                          \
+  extern "C" __global__ __launch_bounds__(256) void paged_read_##NAME##_f32(PagedReadArgs a) { paged_read_t<T, 0>(a); } \
+  extern "C" __global__ __launch_bounds__(256) void paged_read_##NAME##_f16(PagedReadArgs a) { paged_read_t<T, 1>(a); }
+PAGED_READ(f32, 0)
+PAGED_READ(f16, 1)
+PAGED_READ(bf16, 2)
+PAGED_READ(q8, 3)
 
 // --------------------------------------------------------- paged_attention
-struct PagedAttnArgs {
-  const float* q;
-  const char *kc, *vc;
-  const int *table, *lengths;
-  const int* offsets;  // [seqs + 1]: a sequence's row of q and y is its last, offsets[s + 1] - 1; null: row s (both below rows)
-  float* y;
-  const float* sinks;
-  float* part;  // [blocks][2][16 * hd + 32]: a block's pieces of sequences that other blocks share
-  int* done;    // [blocks] counters, 32 ints apart, zero between launches
-  int64_t q_stride, pages, page_stride, slot_stride, head_stride, window;
-  float scale;  // of the scores, times log2 e
-  int32_t seqs, heads, kvh, hd, page_size, max_pages;
-  int32_t group, tiles;  // query heads of a KV head, in tiles of 16
-  int32_t rows;          // of q and y
-  int32_t cus;
-};
-
-typedef _Float16 half8 __attribute__((ext_vector_type(8)));
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef float floatx4 __attribute__((ext_vector_type(4)));
-typedef uint32_t uintx4 __attribute__((ext_vector_type(4)));
-typedef uint32_t uintx2 __attribute__((ext_vector_type(2)));
-
-constexpr float LOG2E = 1.44269504088896340736f;
-__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
-__device__ __forceinline__ bool finite(float x) { return (float_bits(x) & 0x7f800000u) != 0x7f800000u; }
-
-template <int T>
-__device__ __forceinline__ float load1(const char* p)
-{
-  if constexpr (T == 0) return *(const float*)p;
-  else if constexpr (T == 1) return half_to_float(*(const uint16_t*)p);
-  else return bits_float((uint32_t)*(const uint16_t*)p << 16);
-}
-
-template <int T>
-__device__ __forceinline__ floatx4 mfma16(uintx4 a, uintx4 b, floatx4 c)
-{
-  if constexpr (T == 1)
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), c, 0, 0, 0);
-  else
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-}
-
-// two singles as NP parts of the cache's type that add up to them: halves (the
-// first towards zero, the second to nearest: 22 bits, of values scaled into a
-// half's normal range) or bf16 (towards zero: all 24 bits)
-template <int T>
-__device__ __forceinline__ void split2(float x, float y, uint32_t* part)
-{
-  if constexpr (T == 1) {
-    const auto hi = __builtin_amdgcn_cvt_pkrtz(x, y);
-    part[0] = __builtin_bit_cast(uint32_t, hi);
-    const _Float16 lx = (_Float16)(x - (float)hi[0]), ly = (_Float16)(y - (float)hi[1]);
-    part[1] = (uint32_t)__builtin_bit_cast(uint16_t, lx) | (uint32_t)__builtin_bit_cast(uint16_t, ly) << 16;
-  } else {
-#pragma unroll
-    for (int i = 0; i < 3; i++) {
-      const uint32_t hx = float_bits(x), hy = float_bits(y);
-      part[i] = __builtin_amdgcn_perm(hy, hx, 0x07060302u);
-      x = x - bits_float(hx & 0xffff0000u);
-      y = y - bits_float(hy & 0xffff0000u);
-    }
-  }
-}
-
-// At least 64 clocks: what reads the products before it may lie behind any branch, where
-// the compiler counts the wait states (40 clocks at most) along one of the ways alone.
-// (A sleep: an asm statement costs these kernels two registers, and bf16 heads of 128 the
-// second block of a CU.)
-__device__ __forceinline__ void products_done()
-{
-  __builtin_amdgcn_sched_barrier(0);
-  __builtin_amdgcn_s_sleep(1);
-  __builtin_amdgcn_sched_barrier(0);
-}
-
-__device__ __forceinline__ uint64_t lane_value(uint64_t v, int lane)
-{
-  return (uint64_t)__builtin_amdgcn_readlane((uint32_t)(v >> 32), lane) << 32 |
-         (uint32_t)__builtin_amdgcn_readlane((uint32_t)v, lane);
-}
-
-// the maximum and the sum over the four lanes of a head (lanes c, c + 16, c + 32,
-// c + 48)
-__device__ __forceinline__ float quad_max(float v)
-{
-  v = fmaxf(v, xpart<16>(v));
-  return fmaxf(v, xpart<32>(v));
-}
-__device__ __forceinline__ float quad_sum(float v)
-{
-  v = v + xpart<16>(v);
-  return v + xpart<32>(v);
-}
-
-// what a block works on: a sequence, one of its KV heads, 16 of that one's query heads
-struct AttnItem {
-  int s, row, kv;   // sequence, its row of q and y, KV head
-  int heads;        // query heads of the tile
-  int head0;        // the first of them
-};
-
-template <int T, int D>
-struct AttnShape {
-  static constexpr int ES = T == 0 ? 4 : 2;            // bytes of a value
-  static constexpr int KS = T == 0 ? 16 : 32;          // keys of a wave's step
-  static constexpr int DS = D == 512 ? 2 : 1;          // waves that share a head's dimensions (registers)
-  static constexpr int DW = D / DS;                    // dimensions of a wave
-  static constexpr int KG = 4 / DS;                    // groups of keys: the others' waves
-  static constexpr int TK = KG * KS;                   // keys of a block's tile
-  static constexpr int NT = KS / 16;                   // score tiles of a step
-  static constexpr int QL = 16 / ES;                   // values of a key load
-  static constexpr int NQ = DW / (4 * QL);             // key loads of a lane and key
-  static constexpr int NP = T == 0 ? 1 : T == 1 ? 2 : 3;  // parts of a single value
-  static constexpr int VL = T != 0 && D > 64 ? 8 : 4;  // values of a value load
-  static constexpr int NJ = DW / (16 * VL);            // value loads of a lane and key
-  static constexpr int OS = D + 4;                     // a head's row in o_s
-  // weights enter the product times this: into the halves' normal range. The two parts
-  // hold 22 bits of those down to 2^-18 of the largest; smaller ones are off by 2^-40 of
-  // the largest at most
-  static constexpr float PS = T == 1 ? 32768.f : 1.f;
-};
-
-template <int T, int D>
-struct AttnLds {
-  using S = AttnShape<T, D>;
-  uintx4 q[S::NP * S::DS * S::NQ * 64];  // the query tile as the matrix cores take it, by lane
-  float o[16 * S::OS];           // a piece's values
-  float m[16], l[16];            // its maxima and sums
-  float wm[4][16], wl[4][16];    // the waves'
-  float qs[16];                  // powers of two that the queries were divided by
-  int64_t off[4][2][S::KS];      // byte offsets of the steps' keys
-  floatx4 x[S::DS > 1 ? 2 : 1][S::DS > 1 ? 4 : 1][S::NT][64];  // the waves' shares of the scores
-};
-
-// The heads of a piece whose sums are not all finite, again by the formula's own
-// steps in single: the matrix cores' parts turn an infinity into NaN (0 times it
-// is added), and a key of score -infinity has weight 0. Waves take keys in turn,
-// lanes dimensions. Slow, and only for such data.
-template <int T, int D>
-__device__ __forceinline__ void paged_walk(const PagedAttnArgs& a, const AttnItem& it, int64_t j0, int64_t j1,
-                                           AttnLds<T, D>& s)
-{
-  using S = AttnShape<T, D>;
-  constexpr int NV = D / 64;
-  float* const tmp = (float*)s.q;
-  const int t = threadIdx.x, lane = t & 63, w = t >> 6;
-  for (int h = 0; h < it.heads; h++) {
-    float q[NV], acc[NV];
-#pragma unroll
-    for (int i = 0; i < NV; i++) {
-      const int d = lane + 64 * i;
-      q[i] = d < a.hd ? a.q[it.row * a.q_stride + (int64_t)(it.head0 + h) * a.hd + d] * a.scale : 0.f;
-      acc[i] = 0.f;
-    }
-    float m = -__builtin_inff(), l = 0.f;
-    for (int64_t j = j0 + w; j < j1; j += 4) {
-      const uint32_t pg = (uint32_t)j / (uint32_t)a.page_size;
-      const int64_t at = paged_value(a.table[(int64_t)it.s * a.max_pages + pg], (int)((uint32_t)j % (uint32_t)a.page_size),
-                                     a.pages, a.page_stride, a.slot_stride);
-      if (at < 0) continue;
-      const int64_t row = (at + it.kv * a.head_stride) * S::ES;
-      float x = 0.f;
-#pragma unroll
-      for (int i = 0; i < NV; i++)
-        if (lane + 64 * i < a.hd) x = __builtin_fmaf(q[i], load1<T>(a.kc + row + (lane + 64 * i) * S::ES), x);
-      x = wave_sum(x, 64);
-      if (x == -__builtin_inff()) continue;
-      const float m2 = x > m || x != x ? x : m;
-      const float f = m == -__builtin_inff() ? 0.f : exp2_fast(m - m2), p = exp2_fast(x - m2);
-      l = l * f + p;
-      m = m2;
-#pragma unroll
-      for (int i = 0; i < NV; i++)
-        if (lane + 64 * i < a.hd)
-          acc[i] = __builtin_fmaf(p, load1<T>(a.vc + row + (lane + 64 * i) * S::ES), acc[i] * f);
-    }
-#pragma unroll
-    for (int i = 0; i < NV; i++) tmp[w * D + lane + 64 * i] = acc[i];
-    if (lane == 0) {
-      s.wm[w][0] = m;
-      s.wl[w][0] = l;
-    }
-    __syncthreads();
-    float M = -__builtin_inff(), L = 0.f, f[4];
-    for (int i = 0; i < 4; i++) M = s.wm[i][0] > M || s.wm[i][0] != s.wm[i][0] ? s.wm[i][0] : M;
-    for (int i = 0; i < 4; i++) {
-      f[i] = s.wl[i][0] == 0.f ? 0.f : exp2_fast(s.wm[i][0] - M);
-      L += f[i] * s.wl[i][0];
-    }
-    for (int d = t; d < a.hd; d += 256) {
-      float v = 0.f;
-      for (int i = 0; i < 4; i++)
-        if (s.wl[i][0] != 0.f) v += f[i] * tmp[i * D + d];
-      s.o[h * S::OS + d] = v;
-    }
-    if (t == 0) {
-      s.m[h] = M;
-      s.l[h] = L;
-    }
-    __syncthreads();
-  }
-}
-
-// the query tile into LDS in the lanes' order: lane (c, g) = (l & 15, l >> 4) holds
-// head c, values 4 QL i + QL g .. of load i; heads past the tile and values past
-// head_dim are 0. Halves: a head's values times a power of two, so that the
-// largest is below 2^14 and the second parts stay normal.
-template <int T, int D>
-__device__ __forceinline__ void stage_query(const PagedAttnArgs& a, const AttnItem& it, AttnLds<T, D>& s)
-{
-  using S = AttnShape<T, D>;
-  const int t = threadIdx.x;
-  const float* const q = a.q + it.row * a.q_stride + (int64_t)it.head0 * a.hd;
-  if constexpr (T == 1) {
-    const int c = t >> 4;
-    float top = 0.f;
-    if (c < it.heads)
-      for (int d = t & 15; d < a.hd; d += 16) top = fmaxf(top, fabsf(q[c * a.hd + d] * a.scale));
-    top = fmaxf(top, xpart<1>(top));
-    top = fmaxf(top, xpart<2>(top));
-    top = fmaxf(top, xpart<4>(top));
-    top = fmaxf(top, xpart<8>(top));
-    if ((t & 15) == 0) {
-      int e = (int)(float_bits(top) >> 23) - 126;  // top < 2^e
-      if (top == 0.f || !finite(top)) e = 14;
-      s.qs[c] = ldexpf(1.f, max(e - 14, -120));
-    }
-    __syncthreads();
-  }
-  for (int i = t; i < S::DS * S::NQ * 64; i += 256) {
-    const int c = i & 15, d0 = (i >> 6) * 4 * S::QL + ((i >> 4) & 3) * S::QL;
-    float v[S::QL];
-    const bool in = c < it.heads && d0 < a.hd;
-    float f = a.scale;
-    if constexpr (T == 1) f = 1.f / s.qs[c];
-#pragma unroll
-    for (int j = 0; j < S::QL; j++) {
-      v[j] = in ? q[c * a.hd + d0 + j] : 0.f;
-      v[j] = T == 1 ? v[j] * a.scale * f : v[j] * f;
-    }
-    if constexpr (T == 0) {
-      s.q[i] = uintx4{float_bits(v[0]), float_bits(v[1]), float_bits(v[2]), float_bits(v[3])};
-    } else {
-      uint32_t part[4][S::NP];
-#pragma unroll
-      for (int j = 0; j < 4; j++) split2<T>(v[2 * j], v[2 * j + 1], part[j]);
-#pragma unroll
-      for (int n = 0; n < S::NP; n++) s.q[n * S::DS * S::NQ * 64 + i] = uintx4{part[0][n], part[1][n], part[2][n], part[3][n]};
-    }
-  }
-  __syncthreads();
-}
-
-// Attention of one token of each sequence. The work of all sequences and KV heads
-// is one row of tiles of TK keys, shared out evenly over the grid's blocks
-// (ragged lengths leave no block idle, and a captured grid fits the lengths of
-// every replay); a block walks its tiles in pieces of one (sequence, KV head). A
-// piece that is the whole of its item is written at once; the others go to
-// `part`, and the last block of an item to arrive joins them in order.
-//
-// A wave takes KS keys a step. Scores are K q^T with the keys as the matrix
-// cores' rows and the group's heads as columns (16 of them, zeros past the
-// group), so that lane (c, g) holds head c's scores of keys 4 g .. 4 g + 3 of each
-// 16 - which is how the value product takes its weights: values V^T with
-// dimensions as rows, keys as the inner index, each lane loading 8 dimensions of
-// the 8 keys that it has the weights of and turning them by byte permutes in its
-// registers. No key, value or weight goes through LDS, and the running maximum, sum
-// and rescale are a lane's own. Queries and weights enter as 2 half or 3 bf16
-// parts (f32 caches: the f32 matrix cores), so the sums are those of single.
-//
-// HBM bound: the cache is read once (again for each 16 query heads of a KV head
-// beyond 16). 64 sequences of 16384 keys, 8 KV heads of 128 in bf16 705 to 718 us, 6.0
-// TB/s of the 6.2 that a streaming read takes; single 6.3, heads of 256 5.5, of 64 5.0 to
-// 5.8; few long sequences lose the join (three of 110000: 136 us, 5.0), one short one
-// is a chain of round trips (1152 keys 12.5 us). Pages of [kv_heads, page_size,
-// head_dim] read up to 6% faster than [page_size, kv_heads, head_dim]. Heads
-// beyond 256 give a wave half of the dimensions, two waves adding their shares of the
-// scores in LDS, as the values of 512 do not fit the registers beside the keys (one
-// wave each, spilling: 16 sequences of 8192, 2 KV heads 252 us, so 116).
-template <int T, int D, bool FULL>
-__device__ __forceinline__ void paged_attention_t(const PagedAttnArgs& a)
-{
-  using S = AttnShape<T, D>;
-  __shared__ AttnLds<T, D> s;
-  const int t = threadIdx.x, lane = t & 63, c = lane & 15, g = lane >> 4;
-  const int w = __builtin_amdgcn_readfirstlane(t >> 6);
-  const uint32_t grid = gridDim.x, b = blockIdx.x, per = a.kvh * a.tiles;
-  const int hd = FULL ? D : a.hd, row_out = a.heads * a.hd;
-
-  // a sequence's row, -1 where it has none in this step
-  auto row_of = [&](int seq) {
-    return a.offsets ? paged_row(a.offsets[seq], a.offsets[seq + 1], a.rows) : paged_row(seq, seq + 1, a.rows);
-  };
-  auto tiles_of = [&](int seq, int64_t& lo, int64_t& hi) {
-    lo = hi = 0;
-    if (row_of(seq) < 0) return 0u;
-    paged_range(a.lengths[seq], a.window, a.max_pages, a.page_size, &lo, &hi);
-    return (uint32_t)((hi - lo + S::TK - 1) / S::TK);
-  };
-  // all tiles (each wave for itself); rows without a key are zeros
-  uint32_t all = 0, n0 = 0, live = 0;  // tiles, those of the lane's first sequence; sequences with any
-  int64_t lo0 = 0, hi0 = 0;  // of the first 64 sequences, a lane each
-  for (int s0 = 0; s0 < a.seqs; s0 += 64) {
-    const int seq = s0 + lane;
-    uint32_t n = 0;
-    bool zero = false;
-    if (seq < a.seqs) {
-      int64_t lo, hi;
-      n = tiles_of(seq, lo, hi);
-      if (s0 == 0) n0 = n, lo0 = lo, hi0 = hi;
-      zero = n == 0 && a.lengths[seq] >= 0 && row_of(seq) >= 0 && (uint32_t)seq % grid == b;
-    }
-    all += n * per;
-    live += __popcll(__ballot(n != 0));
-    for (uint64_t z = __ballot(zero); z; z &= z - 1) {
-      float* const y = a.y + (int64_t)row_of(s0 + __builtin_ctzll(z)) * row_out;
-      for (int i = t; i < row_out; i += 256) y[i] = 0.f;
-    }
-  }
-  all = __builtin_amdgcn_readfirstlane(wave_sum(all, 64));
-  // Block i of B takes tiles first(i) .. first(i + 1) - 1. One block a CU where the
-  // blocks have 32 tiles and more and the items 24 (their streams then cover each
-  // other's latencies: 64 sequences of 8192, 8 KV heads of 64, two blocks a CU 222 us,
-  // one 196; 16384 of 128 731, 718; of 200 sequences up to 4000, 16 tiles an item, the
-  // starts and ends of pieces need the second block: 301, one 313), else all.
-  const uint32_t B = all >= 32 * grid && all / 24 >= live * per ? min(grid, (uint32_t)a.cus) : min(grid, all);
-  if (b >= B) return;
-  const uint32_t quot = all / B, rem = all % B;
-  auto first = [&](uint32_t i) { return i * quot + i * rem / B; };
-  uint32_t u = first(b);
-  const uint32_t end = first(b + 1);
-  // the sequence of tile u
-  int seq = 0;
-  uint32_t before = 0, n = 0;  // tiles before the sequence, tiles of a KV head's item
-  int64_t lo = 0, hi = 0;
-  for (int s0 = 0;; s0 += 64) {
-    uint32_t m = s0 == 0 ? n0 : 0;
-    if (s0 > 0 && s0 + lane < a.seqs) m = tiles_of(s0 + lane, lo0, hi0);
-    const uint32_t items = m;
-    m *= per;
-    uint32_t upto = m;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-      const uint32_t o = __shfl_up(upto, d, 64);
-      if (lane >= d) upto += o;
-    }
-    const uint64_t there = __ballot(before + upto > u);
-    if (there) {
-      const int f = __builtin_ctzll(there);
-      seq = __builtin_amdgcn_readfirstlane(s0 + f);
-      before += __builtin_amdgcn_readlane(upto - m, f);
-      n = __builtin_amdgcn_readlane(items, f);
-      lo = (int64_t)lane_value((uint64_t)lo0, f);
-      hi = (int64_t)lane_value((uint64_t)hi0, f);
-      break;
-    }
-    before += __builtin_amdgcn_readlane(upto, 63);
-  }
-
-  for (;;) {
-    const uint32_t item = (u - before) / n, tile0 = (u - before) - item * n;
-    const uint32_t tile1 = min(n, tile0 + (end - u));
-    AttnItem it;
-    it.s = seq;
-    it.row = row_of(seq);
-    it.kv = item / a.tiles;
-    const int tile16 = item - it.kv * a.tiles;
-    it.heads = min(16, a.group - 16 * tile16);
-    it.head0 = it.kv * a.group + 16 * tile16;
-    const char* const kb = a.kc + (int64_t)it.kv * a.head_stride * S::ES;
-    const char* const vb = a.vc + (int64_t)it.kv * a.head_stride * S::ES;
-    const int* const table = a.table + (int64_t)seq * a.max_pages;
-    const int kg = w / S::DS, dh = w % S::DS;  // the wave's keys of a tile, its dimensions
-    const int64_t wlo = lo + kg * S::KS;
-    const int64_t jend = min(hi, lo + (int64_t)tile1 * S::TK);  // the piece's keys end here
-    // a step's key of this lane: its page's table entry
-    auto entry = [&](uint32_t tile) {
-      const int64_t j = wlo + (int64_t)tile * S::TK + (lane & (S::KS - 1));
-      return j < jend ? table[(uint32_t)j / (uint32_t)a.page_size] : -1;
-    };
-    // the offsets of a step's keys into LDS, the keys that are there as bits
-    auto locate = [&](uint32_t tile, int page) {
-      const int64_t j = wlo + (int64_t)tile * S::TK + (lane & (S::KS - 1));
-      const int64_t at = paged_value(page, (int)((uint32_t)j % (uint32_t)a.page_size), a.pages, a.page_stride, a.slot_stride);
-      if (lane < S::KS) s.off[w][tile & 1][lane] = at < 0 ? 0 : at * S::ES;
-      // other lanes read it: no instruction, but no reordering or forwarding past here
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      __builtin_amdgcn_wave_barrier();
-      return (uint32_t)__ballot(at >= 0) & (uint32_t)((1ull << S::KS) - 1);
-    };
-    uint32_t tile = tile0;
-    const int page0 = entry(tile);
-    int page = entry(tile + 1);
-    stage_query<T, D>(a, it, s);
-    const float sscale = T == 1 ? s.qs[c] : 1.f;
-
-    uintx4 kr[S::NT][S::NQ];
-    auto load_keys = [&](uint32_t tile) {
-#pragma unroll
-      for (int i = 0; i < S::NT; i++) {
-        const char* const p = kb + s.off[w][tile & 1][16 * i + c];
-#pragma unroll
-        for (int j = 0; j < S::NQ; j++) {
-          const int d0 = dh * S::DW + j * 4 * S::QL + g * S::QL;
-          const bool in = FULL || d0 < hd;
-          kr[i][j] = *(const uintx4*)(p + (in ? d0 : 0) * S::ES);
-          if (!in) kr[i][j] = uintx4{0, 0, 0, 0};
-        }
-      }
-    };
-
-    floatx4 o[S::NJ][S::VL];
-#pragma unroll
-    for (int i = 0; i < S::NJ; i++)
-#pragma unroll
-      for (int j = 0; j < S::VL; j++) o[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
-    float m = -__builtin_inff(), l = 0.f;
-    uint32_t steps = 0;  // of this wave: up to the last tile with a key of its own
-    if (S::DS > 1) {
-      steps = tile1 - tile0;  // the waves meet in each step
-    } else if (wlo + (int64_t)tile0 * S::TK < hi) {
-      const uint32_t mine = (uint32_t)((hi - wlo + S::TK - 1) / S::TK);
-      steps = min(tile1, mine) - tile0;
-    }
-    // The scores are read on both sides of branches, and the values' sums in a block that
-    // few steps enter and behind the loop: products_done() stands before each. Keys are
-    // located and loaded one step past the piece's last too, as a condition there would
-    // keep the loads from covering the products: entry() has no page there and the loads
-    // read the pool's first row.
-    uint32_t there = locate(tile, page0);
-    if (steps) load_keys(tile);
-    for (uint32_t i = 0; i < steps; i++, tile++) {
-      // the step's values, on their way while its scores are formed
-      constexpr int NV = 4 * S::NT;  // keys of a lane: 16 q + 4 g + r
-      uintx4 vr[NV][S::NJ];
-#pragma unroll
-      for (int k = 0; k < NV; k++) {
-        const char* const p = vb + s.off[w][tile & 1][16 * (k >> 2) + 4 * g + (k & 3)];
-#pragma unroll
-        for (int j = 0; j < S::NJ; j++) {
-          const int d0 = dh * S::DW + j * 16 * S::VL + c * S::VL;
-          const char* const v = p + (FULL || d0 < hd ? d0 : 0) * S::ES;
-          if constexpr (S::VL * S::ES == 16) {
-            vr[k][j] = *(const uintx4*)v;
-          } else {
-            const uintx2 h = *(const uintx2*)v;
-            vr[k][j] = uintx4{h[0], h[1], 0, 0};
-          }
-        }
-      }
-      const uint32_t now = there;
-      there = locate(tile + 1, page);
-      page = entry(tile + 2);
-      floatx4 x[S::NT];
-#pragma unroll
-      for (int k = 0; k < S::NT; k++) x[k] = floatx4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int j = 0; j < S::NQ; j++) {
-#pragma unroll
-        for (int n2 = 0; n2 < S::NP; n2++) {
-          const uintx4 q = s.q[(n2 * S::DS * S::NQ + dh * S::NQ + j) * 64 + lane];
-#pragma unroll
-          for (int k = 0; k < S::NT; k++) {
-            if constexpr (T == 0) {
-#pragma unroll
-              for (int e = 0; e < 4; e++)
-                x[k] = __builtin_amdgcn_mfma_f32_16x16x4f32(bits_float(kr[k][j][e]), bits_float(q[e]), x[k], 0, 0, 0);
-            } else {
-              x[k] = mfma16<T>(kr[k][j], q, x[k]);
-            }
-          }
-        }
-      }
-      load_keys(tile + 1);
-      products_done();
-      if constexpr (S::DS > 1) {
-        // the scores of all dimensions: two waves' shares added, the same sum in both
-#pragma unroll
-        for (int k = 0; k < S::NT; k++) s.x[tile & 1][w][k][lane] = x[k];
-        __syncthreads();
-#pragma unroll
-        for (int k = 0; k < S::NT; k++) x[k] += s.x[tile & 1][w ^ 1][k][lane];
-      }
-      // masked keys: no weight, and values of zero (0 times NaN is NaN)
-      float top = -__builtin_inff();
-      if (now == (uint32_t)((1ull << S::KS) - 1)) {
-#pragma unroll
-        for (int k = 0; k < S::NT; k++)
-#pragma unroll
-          for (int r = 0; r < 4; r++) {
-            x[k][r] = x[k][r] * sscale;
-            top = fmaxf(top, x[k][r]);
-          }
-      } else {
-#pragma unroll
-        for (int k = 0; k < NV; k++) {
-          const bool in = now >> (16 * (k >> 2) + 4 * g + (k & 3)) & 1;
-          x[k >> 2][k & 3] = in ? x[k >> 2][k & 3] * sscale : -__builtin_inff();
-          top = fmaxf(top, x[k >> 2][k & 3]);
-#pragma unroll
-          for (int j = 0; j < S::NJ; j++)
-            if (!in) vr[k][j] = uintx4{0, 0, 0, 0};
-        }
-      }
-      top = quad_max(top);
-      if (__any(top > m)) {
-        const float m2 = fmaxf(top, m), f = m == -__builtin_inff() ? 0.f : exp2_fast(m - m2);
-        m = m2;
-        l *= f;
-#pragma unroll
-        for (int j = 0; j < S::NJ; j++)
-#pragma unroll
-          for (int e = 0; e < S::VL; e++) o[j][e] *= f;
-      }
-      const float shift = m == -__builtin_inff() ? 0.f : m;
-      float p[NV];
-#pragma unroll
-      for (int k = 0; k < NV; k++) {
-        p[k] = exp2_fast(x[k >> 2][k & 3] - shift);
-        l += p[k];
-      }
-      if constexpr (T == 0) {
-#pragma unroll
-        for (int k = 0; k < NV; k++)
-#pragma unroll
-          for (int j = 0; j < S::NJ; j++)
-#pragma unroll
-            for (int e = 0; e < 4; e++)
-              o[j][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(bits_float(vr[k][j][e]), p[k], o[j][e], 0, 0, 0);
-      } else {
-        uint32_t part[4][S::NP];
-#pragma unroll
-        for (int k = 0; k < 4; k++) split2<T>(p[2 * k] * S::PS, p[2 * k + 1] * S::PS, part[k]);
-#pragma unroll
-        for (int j = 0; j < S::NJ; j++)
-#pragma unroll
-          for (int e = 0; e < S::VL; e++) {
-            uintx4 v;
-#pragma unroll
-            for (int k = 0; k < 4; k++)
-              v[k] = __builtin_amdgcn_perm(vr[2 * k + 1][j][e / 2], vr[2 * k][j][e / 2], e & 1 ? 0x07060302u : 0x05040100u);
-#pragma unroll
-            for (int n2 = 0; n2 < S::NP; n2++)
-              o[j][e] = mfma16<T>(v, uintx4{part[0][n2], part[1][n2], part[2][n2], part[3][n2]}, o[j][e]);
-          }
-      }
-    }
-
-    // the waves' sums meet
-    products_done();
-    l = quad_sum(l);
-    if (g == 0 && dh == 0) {
-      s.wm[kg][c] = m;
-      s.wl[kg][c] = l;
-    }
-    __syncthreads();
-    float M = s.wm[0][c];
-#pragma unroll
-    for (int i = 1; i < S::KG; i++) M = fmaxf(M, s.wm[i][c]);
-    const float Ms = M == -__builtin_inff() ? 0.f : M;
-    const float f = exp2_fast(m - Ms) * (1.f / S::PS);
-    bool odd = false;
-    if (w == 0 && g == 0) {
-      float L = 0.f;
-#pragma unroll
-      for (int i = 0; i < S::KG; i++) L += s.wl[i][c] * exp2_fast(s.wm[i][c] - Ms);
-      s.m[c] = M;
-      s.l[c] = L;
-      odd = c < it.heads && !finite(L);
-    }
-    for (int r4 = 0; r4 < S::KG; r4++) {
-      if (kg == r4) {
-#pragma unroll
-        for (int j = 0; j < S::NJ; j++)
-#pragma unroll
-          for (int r = 0; r < 4; r++)
-#pragma unroll
-            for (int e = 0; e < S::VL; e += 4) {
-              floatx4* const d = (floatx4*)&s.o[c * S::OS + dh * S::DW + j * 16 * S::VL + S::VL * (4 * g + r) + e];
-              floatx4 v = {o[j][e][r] * f, o[j][e + 1][r] * f, o[j][e + 2][r] * f, o[j][e + 3][r] * f};
-              if (r4) v += *d;
-              *d = v;
-            }
-      }
-      __syncthreads();
-    }
-    for (int h = w; h < it.heads; h += 4)
-      for (int d = lane; d < hd; d += 64) odd |= !finite(s.o[h * S::OS + d]);
-    if (__syncthreads_or(odd))
-      paged_walk<T, D>(a, it, lo + (int64_t)tile0 * S::TK, min(hi, lo + (int64_t)tile1 * S::TK), s);
-
-    float* const y = a.y + (int64_t)it.row * row_out + (int64_t)it.head0 * a.hd;
-    // with the sink: its weight beside the sum's, both against the larger maximum
-    auto finish = [&](int h, float m2, float l2, float& f2) {
-      f2 = 1.f;
-      if (a.sinks) {
-        const float sk = a.sinks[it.head0 + h] * LOG2E;
-        if (sk > m2) {
-          f2 = exp2_fast(m2 - sk);
-          l2 = l2 * f2 + 1.f;
-        } else if (sk != -__builtin_inff()) {  // (switched off: no weight, where no key has one either)
-          l2 += exp2_fast(sk - m2);
-        }
-      }
-      f2 = l2 != 0.f ? f2 / l2 : 0.f;
-    };
-    if (tile0 == 0 && tile1 == n) {
-      for (int h = w; h < it.heads; h += 4) {
-        float f2;
-        finish(h, s.m[h], s.l[h], f2);
-        for (int d = lane; d < hd; d += 64) y[h * a.hd + d] = f2 == 0.f ? 0.f : s.o[h * S::OS + d] * f2;
-      }
-      __syncthreads();
-    } else {
-      const int ps = 16 * a.hd + 32;  // floats of a piece
-      float* const pc = a.part + (int64_t)(2 * b + (tile0 ? 0 : 1)) * ps;
-      for (int h = w; h < it.heads; h += 4)
-        for (int d = lane; d < hd; d += 64) store_agent(pc + h * a.hd + d, s.o[h * S::OS + d]);
-      if (t < 16) {
-        store_agent(pc + 16 * a.hd + t, s.m[t]);
-        store_agent(pc + 16 * a.hd + 16 + t, s.l[t]);
-      }
-      // the blocks of the item's first and last tile
-      auto block_of = [&](uint32_t i) {
-        uint32_t k = (uint32_t)((double)i * B / all);
-        while (k > 0 && first(k) > i) k--;
-        while (first(k + 1) <= i) k++;
-        return k;
-      };
-      const uint32_t u0 = before + item * n, b0 = block_of(u0), np = block_of(u0 + n - 1) - b0 + 1;
-      auto piece = [&](uint32_t i) { return a.part + (int64_t)(2 * (b0 + i) + (i == 0)) * ps; };
-      // pieces i0, i0 + step, .. (cnt of them, at most 64) joined in that order: into
-      // the output, or into the first of them
-      auto join = [&](uint32_t i0, uint32_t step, uint32_t cnt, bool out) {
-        // 4 values of 16 pieces a thread, the first on their way while the weights are formed
-        const int total = it.heads * a.hd;
-        uint64_t x[16][2];
-        auto fetch = [&](int i, uint32_t j0) {
-#pragma unroll
-          for (uint32_t k = 0; k < 16; k++) {
-            const double* const e = (const double*)(piece(i0 + step * min(j0 + k, cnt - 1)) + i);
-            x[k][0] = __builtin_bit_cast(uint64_t, load_agent(e));
-            x[k][1] = __builtin_bit_cast(uint64_t, load_agent(e + 1));
-          }
-        };
-        if (4 * t < total) fetch(4 * t, 0);
-        float* const wt = s.o;  // [64][16]: a piece's weight for each head, 0 past the last
-        {
-          const int h = t >> 4;
-          float pm[4], pl[4], M2 = -__builtin_inff(), L = 0.f;
-#pragma unroll
-          for (int i = 0; i < 4; i++) {
-            const uint32_t j = (t & 15) + 16 * i;
-            const float* const e = piece(i0 + step * min(j, cnt - 1)) + 16 * a.hd + h;
-            pm[i] = j < cnt ? load_agent(e) : -__builtin_inff();
-            pl[i] = j < cnt ? load_agent(e + 16) : 0.f;
-            M2 = fmaxf(M2, pm[i]);
-          }
-          M2 = fmaxf(M2, xpart<1>(M2));
-          M2 = fmaxf(M2, xpart<2>(M2));
-          M2 = fmaxf(M2, xpart<4>(M2));
-          M2 = fmaxf(M2, xpart<8>(M2));
-          const float s2 = M2 == -__builtin_inff() ? 0.f : M2;
-#pragma unroll
-          for (int i = 0; i < 4; i++) {
-            const float f2 = exp2_fast(pm[i] - s2);
-            L += f2 * pl[i];
-            wt[((t & 15) + 16 * i) * 16 + h] = f2;
-          }
-          L = wave_sum(L, 16);
-          __syncthreads();
-          if ((t & 15) == 0) {
-            s.m[h] = M2;
-            s.l[h] = L;
-            if (!out) {
-              store_agent(piece(i0) + 16 * a.hd + h, M2);
-              store_agent(piece(i0) + 16 * a.hd + 16 + h, L);
-            }
-          }
-        }
-        __syncthreads();
-        for (int i = 4 * t; i < total; i += 1024) {
-          const int h = i / a.hd;
-          float v[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 1
-          for (uint32_t j0 = 0; j0 < cnt; j0 += 16) {
-            if (i != 4 * t || j0) fetch(i, j0);
-#pragma unroll
-            for (uint32_t k = 0; k < 16; k++) {
-              const float f2 = wt[(j0 + k) * 16 + h];
-#pragma unroll
-              for (int e = 0; e < 4; e++) {
-                const float p = bits_float((uint32_t)(x[k][e / 2] >> (32 * (e & 1))));
-                v[e] = __builtin_fmaf(f2, f2 != 0.f ? p : 0.f, v[e]);  // (a part of no weight may hold an infinity)
-              }
-            }
-          }
-          if (out) {
-            float f2;
-            finish(h, s.m[h], s.l[h], f2);
-#pragma unroll
-            for (int e = 0; e < 4; e++) y[i + e] = f2 == 0.f ? 0.f : v[e] * f2;
-          } else {
-#pragma unroll
-            for (int e = 0; e < 4; e++) store_agent(piece(i0) + i + e, v[e]);
-          }
-        }
-      };
-      // 16 pieces are joined by the last of their blocks, then those by the last of all
-      const uint32_t mine = b - b0, i0 = mine & ~15u, cnt = min(16u, np - i0);
-      int* const group = a.done + 32 * (b0 + i0) + (i0 == 0);
-      if (last_block(group, (int)cnt)) {
-        const uint32_t groups = (np + 15) / 16;
-        join(i0, 1, cnt, groups == 1);
-        if (t == 0) __hip_atomic_store(group, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        if (groups > 1 && last_block(a.done + 32 * b0 + 2, (int)groups)) {
-          join(0, 16, groups, true);
-          if (t == 0) __hip_atomic_store(a.done + 32 * b0 + 2, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        }
-      }
-      __syncthreads();
-    }
-    u += tile1 - tile0;
-    if (u >= end) return;
-    if (tile1 == n && item + 1 == per) {  // the next sequence with a key
-      before = u;
-      do n = tiles_of(++seq, lo, hi);
-      while (n == 0);
-    }
-  }
-}
-
 // heads between two sizes: two blocks a CU up to 128. The others have no bound, which
 // costs the join of few long sequences (24 us became 32). On their own those up to 128
 // take 189 to 256 registers, two blocks a CU - but for halves of 128, whose 260 leave

@@ -60,7 +60,7 @@ class Pages(C.Structure):
     _fields_ = [("k", C.c_uint64), ("v", C.c_uint64), ("pages", C.c_int64),
                 ("page_stride", C.c_int64), ("slot_stride", C.c_int64), ("head_stride", C.c_int64),
                 ("page_size", C.c_int32), ("kv_heads", C.c_int32), ("head_dim", C.c_int32),
-                ("dtype", C.c_int32)]
+                ("dtype", C.c_int32), ("k_scale", C.c_uint64), ("v_scale", C.c_uint64)]
 
 
 class Rope(C.Structure):
@@ -70,6 +70,7 @@ class Rope(C.Structure):
 
 
 PAGED_SEQS, LOGPROBS_TOP = 4096, 64
+Q8_HEAD = 64  # 8-bit pages (Pages.dtype alone)
 
 
 def row_bytes(dtype, cols):
@@ -181,6 +182,8 @@ def lib():
             "ihip_enqueue_paged_qkrope": (i32, [vp, u64, i64, u64, i64, u64, i64, i64, i64, u64,
                                                 u64, C.c_double, C.POINTER(Rope), u64, u64,
                                                 C.POINTER(Pages), u64]),
+            "ihip_enqueue_paged_read": (i32, [vp, C.POINTER(Pages), u64, i64, u64, u64, i64, i64, i32, u64,
+                                              u64]),
             "ihip_enqueue_paged_attention": (i32, [vp, u64, i64, C.POINTER(Pages), u64, i64, u64,
                                                    u64, i64, i64, i64, u64, C.c_double]),
             "ihip_enqueue_paged_attention_at": (i32, [vp, u64, i64, C.POINTER(Pages), u64, i64, u64,
