@@ -696,6 +696,22 @@ int ihip_enqueue_paged_attention_at(ihip_ctx* ctx, uint64_t q, int64_t q_stride,
                                     uint64_t lengths, uint64_t offsets, int64_t rows, uint64_t y,
                                     int64_t seqs, int64_t heads, int64_t window, uint64_t sinks,
                                     double scale);
+/* the same for a batch in which groups of sequences have their first tokens in common (a
+ * system prompt, a document, samples of one request): sequences members[g] ..
+ * members[g + 1] - 1 (members [groups + 1], int32, ascending; at most seqs groups) hold
+ * the same first shared[g] tokens, in pages that the tables of all of them list, and the
+ * group's first table is read for them, once for all of the group. What comes behind
+ * is read by each sequence from its own table; a sequence shorter than shared[g] sees
+ * its own tokens alone, one outside every group, or alone in its own, all of its
+ * tokens as _paged_attention_at. With a window every sequence reads its own keys. The
+ * results are _paged_attention_at's but for the order of sums. y does not overlap q;
+ * seqs * heads is at most 2^20. Both arrays are read on the device. */
+int ihip_enqueue_paged_attention_shared(ihip_ctx* ctx, uint64_t q, int64_t q_stride,
+                                        const ihip_pages* cache, uint64_t table, int64_t max_pages,
+                                        uint64_t lengths, uint64_t offsets, int64_t rows,
+                                        uint64_t members, uint64_t shared, int64_t groups, uint64_t y,
+                                        int64_t seqs, int64_t heads, int64_t window, uint64_t sinks,
+                                        double scale);
 /* cached tokens read back as contiguous rows, as the caches of
  * ihip_enqueue_attention and ihip_enqueue_qkrope hold them (a prompt's next chunk over
  * a history in pages, a sequence that leaves the pool): row r of k_out and v_out ([rows,

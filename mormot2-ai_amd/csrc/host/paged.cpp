@@ -104,6 +104,89 @@ int check_pool(const char* who, const ihip_pages* p, Pool* out)
   return 0;
 }
 
+// the sequences that share their first tokens (null: none do)
+struct Groups {
+  uint64_t members, shared;
+  int64_t groups;
+};
+
+int paged_attention(const char* who, ihip_ctx* c, uint64_t q, int64_t q_stride, const ihip_pages* cache,
+                    uint64_t table, int64_t max_pages, uint64_t lengths, uint64_t offsets, int64_t rows,
+                    const Groups* groups, uint64_t y, int64_t seqs, int64_t heads, int64_t window,
+                    uint64_t sinks, double scale)
+{
+  Pool p;
+  if (int rc = check_pool(who, cache, &p)) return rc;
+  const int64_t hd = cache->head_dim, kvh = cache->kv_heads;
+  if (!q || !table || !lengths || !y || (groups && (!groups->members || !groups->shared)))
+    return refuse(who, "a missing array");
+  if (seqs > IHIP_PAGED_SEQS) return refuse(who, "more sequences than IHIP_PAGED_SEQS", IHIP_E_NOMEM);
+  if (seqs < 1 || heads < 1 || heads > 65535 || heads % kvh || window < 0 || max_pages < 1 ||
+      max_pages > INT32_MAX / cache->page_size || rows < 1 || rows > INT32_MAX)
+    return refuse(who, "seqs, heads, window, max_pages or rows out of range");
+  if (groups && (groups->groups < 1 || groups->groups > seqs)) return refuse(who, "groups out of range");
+  if (groups && seqs * heads > SHARED_HEADS) return refuse(who, "more than 2^20 heads of sequences", IHIP_E_NOMEM);
+  q_stride = q_stride ? q_stride : heads * hd;
+  if (q_stride < heads * hd) return refuse(who, "a stride below a row");
+  if (q_stride > STRIDE_MOST) return refuse(who, "a stride beyond 2^36");
+  if ((q | y | sinks | lengths | offsets | table | (groups ? groups->members | groups->shared : 0)) % 4) return refuse(who, "arrays aligned to 4 bytes");
+  if (overlaps(y, (__int128)rows * heads * hd * 4, q, q_stride * 4, heads * hd * 4, rows) &&
+      (groups || !(y == q && q_stride == heads * hd)))
+    return refuse(who, groups ? "y overlaps q" : "y overlaps q, and is not q's contiguous rows");
+  // (the kernel's scores are in base 2, in single)
+  const float scale2 = (float)((scale != 0 ? scale : 1.0 / std::sqrt((double)hd)) * 1.4426950408889634);
+  if (!(scale >= 0) || !std::isfinite(scale2)) return refuse(who, "scale is 0 or positive, times log2 e within single");
+  // the kernels take tiles of 128 keys of 16-bit and 8-bit caches, 64 of single ones,
+  // half as many of heads beyond 256
+  const int64_t group = heads / kvh, tiles = (group + 15) / 16;
+  const int64_t tk = (cache->dtype == IHIP_F32 ? 64 : 128) / (hd > 256 ? 2 : 1);
+  const int64_t keys = window > 0 ? std::min(window, max_pages * cache->page_size) : max_pages * cache->page_size;
+  const int64_t units = (keys + tk - 1) / tk * kvh * tiles;
+  if (units > INT32_MAX / seqs) return refuse(who, "more than 2^31 tiles of keys", IHIP_E_NOMEM);
+  if (!c) return no_context(who);
+  OnDevice on(c);
+  struct {
+    const float* q;
+    const char *kc, *vc;
+    const int *table, *lengths, *offsets;
+    float* y;
+    const float* sinks;
+    float* part;
+    int* done;
+    int64_t q_stride, pages, page_stride, slot_stride, head_stride, window;
+    float scale;
+    int32_t seqs, heads, kvh, hd, page_size, max_pages, group, tiles, rows, cus;
+    uint64_t ks, vs;  // (of 8-bit pages' and the groups' kernels alone, as what follows)
+    int64_t s_page, s_slot, s_head;
+    uint64_t members, shared, pieces, lse, plan;  // (of the groups' kernels alone)
+    int32_t groups, pad;
+  } a = {(const float*)q, (const char*)cache->k, (const char*)cache->v, (const int*)table,
+         (const int*)lengths, (const int*)offsets, (float*)y, (const float*)sinks, (float*)c->paged_part,
+         (int*)(c->paged_part + PAGED_PART_BYTES), q_stride, cache->pages, p.page_stride,
+         p.slot_stride, p.head_stride, window,
+         scale2, (int32_t)seqs,
+         (int32_t)heads, (int32_t)kvh, (int32_t)hd, cache->page_size, (int32_t)max_pages, (int32_t)group,
+         (int32_t)tiles, (int32_t)rows, c->cus, q8_scales(cache, 0), q8_scales(cache, 1), p.s_page, p.s_slot, p.s_head,
+         groups ? groups->members : 0, groups ? groups->shared : 0, c->paged_shared, c->paged_shared + SHARED_PIECE_BYTES,
+         c->paged_shared + SHARED_PIECE_BYTES + SHARED_HEADS * 4, groups ? (int32_t)groups->groups : 0, 0};
+  const int d = hd <= 64 ? 64 : hd <= 128 ? 128 : hd <= 256 ? 256 : 512;
+  char name[40];
+  // (a window's keys are few: every sequence reads its own)
+  const bool prefix = groups && window == 0;
+  if (prefix) {
+    const int64_t cols = d <= 128 ? 64 : d == 256 ? 32 : 16;  // shared_ct's
+    snprintf(name, sizeof name, "paged_prefix_%s_%d%s", p.type, d, hd == d ? "" : "_part");
+    int64_t blocks = (int64_t)c->cus * resident_blocks(c, name, 256);
+    blocks = std::min<int64_t>({blocks, PAGED_BLOCKS, (int64_t)(SHARED_PIECE_BYTES / (2 * cols * (hd + 2) * 4)), units * seqs});
+    if (int rc = launch(c, name, dim3((unsigned)blocks), dim3(256), &a)) return rc;
+  }
+  snprintf(name, sizeof name, "paged_%s_%s_%d%s", prefix ? "own" : "attention", p.type, d, hd == d ? "" : "_part");
+  // as many blocks as reside at once, and as there are tiles and pieces for them
+  int64_t blocks = (int64_t)c->cus * resident_blocks(c, name, 256);
+  blocks = std::min<int64_t>({blocks, PAGED_BLOCKS, (int64_t)(PAGED_PART_BYTES / (2 * (16 * hd + 32) * 4)), units * seqs});
+  return launch(c, name, dim3((unsigned)blocks), dim3(256), &a);
+}
+
 }  // namespace
 
 extern "C" {
@@ -230,61 +313,18 @@ int ihip_enqueue_paged_attention_at(ihip_ctx* c, uint64_t q, int64_t q_stride, c
                                     int64_t rows, uint64_t y, int64_t seqs, int64_t heads, int64_t window,
                                     uint64_t sinks, double scale)
 {
-  const char* who = "ihip_enqueue_paged_attention";
-  Pool p;
-  if (int rc = check_pool(who, cache, &p)) return rc;
-  const int64_t hd = cache->head_dim, kvh = cache->kv_heads;
-  if (!q || !table || !lengths || !y) return refuse(who, "a missing array");
-  if (seqs > IHIP_PAGED_SEQS) return refuse(who, "more sequences than IHIP_PAGED_SEQS", IHIP_E_NOMEM);
-  if (seqs < 1 || heads < 1 || heads > 65535 || heads % kvh || window < 0 || max_pages < 1 ||
-      max_pages > INT32_MAX / cache->page_size || rows < 1 || rows > INT32_MAX)
-    return refuse(who, "seqs, heads, window, max_pages or rows out of range");
-  q_stride = q_stride ? q_stride : heads * hd;
-  if (q_stride < heads * hd) return refuse(who, "a stride below a row");
-  if (q_stride > STRIDE_MOST) return refuse(who, "a stride beyond 2^36");
-  if ((q | y | sinks | lengths | offsets | table) % 4) return refuse(who, "arrays aligned to 4 bytes");
-  if (overlaps(y, (__int128)rows * heads * hd * 4, q, q_stride * 4, heads * hd * 4, rows) &&
-      !(y == q && q_stride == heads * hd))
-    return refuse(who, "y overlaps q, and is not q's contiguous rows");
-  // (the kernel's scores are in base 2, in single)
-  const float scale2 = (float)((scale != 0 ? scale : 1.0 / std::sqrt((double)hd)) * 1.4426950408889634);
-  if (!(scale >= 0) || !std::isfinite(scale2)) return refuse(who, "scale is 0 or positive, times log2 e within single");
-  // the kernels take tiles of 128 keys of 16-bit and 8-bit caches, 64 of single ones,
-  // half as many of heads beyond 256
-  const int64_t group = heads / kvh, tiles = (group + 15) / 16;
-  const int64_t tk = (cache->dtype == IHIP_F32 ? 64 : 128) / (hd > 256 ? 2 : 1);
-  const int64_t keys = window > 0 ? std::min(window, max_pages * cache->page_size) : max_pages * cache->page_size;
-  const int64_t units = (keys + tk - 1) / tk * kvh * tiles;
-  if (units > INT32_MAX / seqs) return refuse(who, "more than 2^31 tiles of keys", IHIP_E_NOMEM);
-  if (!c) return no_context(who);
-  OnDevice on(c);
-  struct {
-    const float* q;
-    const char *kc, *vc;
-    const int *table, *lengths, *offsets;
-    float* y;
-    const float* sinks;
-    float* part;
-    int* done;
-    int64_t q_stride, pages, page_stride, slot_stride, head_stride, window;
-    float scale;
-    int32_t seqs, heads, kvh, hd, page_size, max_pages, group, tiles, rows, cus;
-    uint64_t ks, vs;  // (of 8-bit pages' kernel alone, as what follows)
-    int64_t s_page, s_slot, s_head;
-  } a = {(const float*)q, (const char*)cache->k, (const char*)cache->v, (const int*)table,
-         (const int*)lengths, (const int*)offsets, (float*)y, (const float*)sinks, (float*)c->paged_part,
-         (int*)(c->paged_part + PAGED_PART_BYTES), q_stride, cache->pages, p.page_stride,
-         p.slot_stride, p.head_stride, window,
-         scale2, (int32_t)seqs,
-         (int32_t)heads, (int32_t)kvh, (int32_t)hd, cache->page_size, (int32_t)max_pages, (int32_t)group,
-         (int32_t)tiles, (int32_t)rows, c->cus, q8_scales(cache, 0), q8_scales(cache, 1), p.s_page, p.s_slot, p.s_head};
-  const int d = hd <= 64 ? 64 : hd <= 128 ? 128 : hd <= 256 ? 256 : 512;
-  char name[40];
-  snprintf(name, sizeof name, "paged_attention_%s_%d%s", p.type, d, hd == d ? "" : "_part");
-  // as many blocks as reside at once, and as there are tiles and pieces for them
-  int64_t blocks = (int64_t)c->cus * resident_blocks(c, name, 256);
-  blocks = std::min<int64_t>({blocks, PAGED_BLOCKS, (int64_t)(PAGED_PART_BYTES / (2 * (16 * hd + 32) * 4)), units * seqs});
-  return launch(c, name, dim3((unsigned)blocks), dim3(256), &a);
+  return paged_attention("ihip_enqueue_paged_attention", c, q, q_stride, cache, table, max_pages, lengths, offsets, rows,
+                         nullptr, y, seqs, heads, window, sinks, scale);
+}
+
+int ihip_enqueue_paged_attention_shared(ihip_ctx* c, uint64_t q, int64_t q_stride, const ihip_pages* cache,
+                                        uint64_t table, int64_t max_pages, uint64_t lengths, uint64_t offsets,
+                                        int64_t rows, uint64_t members, uint64_t shared, int64_t groups, uint64_t y,
+                                        int64_t seqs, int64_t heads, int64_t window, uint64_t sinks, double scale)
+{
+  const Groups g = {members, shared, groups};
+  return paged_attention("ihip_enqueue_paged_attention_shared", c, q, q_stride, cache, table, max_pages, lengths, offsets,
+                         rows, &g, y, seqs, heads, window, sinks, scale);
 }
 
 int ihip_enqueue_paged_read(ihip_ctx* c, const ihip_pages* cache, uint64_t table, int64_t max_pages,

@@ -2,6 +2,8 @@
 // the kernel that paged.hip instantiates.
 #pragma once
 
+#include <type_traits>
+
 #include "common.h"
 #include "../paged.h"
 
@@ -31,6 +33,17 @@ struct PagedAttn8Args : PagedAttnArgs {
   const float *ks, *vs;
   int64_t s_page, s_slot, s_head;
 };
+
+// groups of sequences whose first tokens are the same (paged_shared.hip): the own tokens'
+// attention joined with that of the prefix, which a launch before has left
+struct PagedSharedArgs : PagedAttn8Args {
+  const int *members, *shared;  // [groups + 1], [groups]: a group's sequences, their common tokens
+  float* pieces;  // [blocks][2][16 CT (hd + 2)]: parts of a prefix that blocks share
+  float* lse;     // [seqs][heads], base 2: of a prefix that one block has finished, into y
+  int* plan;      // SHARED_PLAN's numbers, then [groups][3]: tiles before the group's, keys' tiles, columns' tiles
+  int32_t groups, pad;
+};
+constexpr int SHARED_PLAN = 4;  // all tiles, the blocks that share them
 
 typedef _Float16 half2 __attribute__((ext_vector_type(2)));
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
@@ -128,6 +141,52 @@ __device__ __forceinline__ float quad_sum(float v)
   return v + xpart<32>(v);
 }
 
+template <typename A>
+constexpr bool is_shared = false;
+template <>
+constexpr bool is_shared<PagedSharedArgs> = true;
+
+// the last g of the n with first[g] <= i, first[0] <= i (first ascending; any other
+// array ends within it too)
+__device__ __forceinline__ int find_last(const int* first, int n, int i)
+{
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (first[mid] <= i) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+// a sequence's group, -1 where it has none, and how many of its tokens are read once for
+// the group
+__device__ __forceinline__ int64_t shared_tokens(const PagedSharedArgs& a, int seq, int& g)
+{
+  g = -1;
+  if (a.groups < 1) return 0;
+  const int at = find_last(a.members, a.groups, seq);
+  const int m0 = a.members[at], m1 = a.members[at + 1];
+  if (seq < m0 || seq >= m1) return 0;
+  const int64_t n = paged_common(m0, m1, a.shared[at], a.seqs, a.max_pages, a.page_size);
+  if (n > 0) g = at;
+  return n;
+}
+
+// `all` tiles shared out evenly over B blocks: block i takes first(i) .. first(i + 1) - 1
+struct PieceShare {
+  uint32_t all, B, quot, rem;
+  __device__ __forceinline__ PieceShare(uint32_t a, uint32_t b) : all(a), B(b), quot(a / b), rem(a % b) {}
+  __device__ __forceinline__ uint32_t first(uint32_t i) const { return i * quot + i * rem / B; }
+  __device__ __forceinline__ uint32_t block_of(uint32_t u) const
+  {
+    uint32_t k = (uint32_t)((double)u * B / all);
+    while (k > 0 && first(k) > u) k--;
+    while (first(k + 1) <= u) k++;
+    return k;
+  }
+};
+
 // what a block works on: a sequence, one of its KV heads, 16 of that one's query heads
 struct AttnItem {
   int s, row, kv;   // sequence, its row of q and y, KV head
@@ -182,6 +241,13 @@ struct AttnLds : AttnScales<T> {
   float qs[16];                  // powers of two that the queries were divided by
   int64_t off[4][2][S::KS];      // byte offsets of the steps' keys
   floatx4 x[S::DS > 1 ? 2 : 1][S::DS > 1 ? 4 : 1][S::NT][64];  // the waves' shares of the scores
+};
+
+// a tile's heads' part of a prefix (PagedSharedArgs), in LDS
+struct AttnPrefix {
+  float m[16], l[16];          // its maxima (base 2) and sums
+  int first[16], count[16];    // the blocks of its pieces; count 0: in y and lse
+  int col[16];                 // a head's column in the pieces
 };
 
 // The heads of a piece whose sums are not all finite, again by the formula's own
@@ -353,8 +419,108 @@ __device__ __forceinline__ void paged_attention_t(const A& a)
     lo = hi = 0;
     if (row_of(seq) < 0) return 0u;
     paged_range(a.lengths[seq], a.window, a.max_pages, a.page_size, &lo, &hi);
+    if constexpr (is_shared<A>) {
+      int grp;
+      lo = min(hi, shared_tokens(a, seq, grp));
+    }
     return (uint32_t)((hi - lo + S::TK - 1) / S::TK);
   };
+  // the heads' part of their sequence's prefix; whether there is one
+  auto prefix_of = [&](const AttnItem& it, auto& px) {
+    if constexpr (is_shared<A>) {
+      int grp;
+      if (shared_tokens(a, it.s, grp) == 0) return false;
+      const int pall = a.plan[0], pb = a.plan[1], pct = a.plan[2] * 16;
+      if (pall <= 0) return false;
+      const uint32_t before = a.plan[SHARED_PLAN + 3 * grp], pn = a.plan[SHARED_PLAN + 3 * grp + 1];
+      const int cts = a.plan[SHARED_PLAN + 3 * grp + 2];
+      const int64_t size = (int64_t)pct * (a.hd + 2);
+      const int h = t >> 4;
+      __syncthreads();
+      if (h < it.heads) {
+        const int col = (it.s - a.members[grp]) * a.group + it.head0 - it.kv * a.group + h;
+        const uint32_t u0 = before + (uint32_t)(it.kv * cts + col / pct) * pn;
+        const PieceShare share(pall, pb);
+        const int b0 = share.block_of(u0), b1 = share.block_of(u0 + pn - 1);
+        const int c16 = col % pct;
+        float m = -__builtin_inff(), l = 0.f;
+        if (b0 == b1) {
+          if ((t & 15) == 0) m = a.lse[(int64_t)it.s * a.heads + it.head0 + h];
+          l = m == -__builtin_inff() ? 0.f : 1.f;
+        } else {
+          for (int i = t & 15; i <= b1 - b0; i += 16) {
+            const float* const e = a.pieces + (2 * (int64_t)(b0 + i) + (i == 0)) * size + pct * a.hd + c16;
+            const float pm = e[0], pl = e[pct];
+            if (pl == 0.f) continue;
+            const float m2 = pm > m || pm != pm ? pm : m;
+            l = (m == -__builtin_inff() ? 0.f : l * exp2_fast(m - m2)) + pl * exp2_fast(pm - m2);
+            m = m2;
+          }
+        }
+        auto meet = [&](float om, float ol) {
+          const float m2 = om > m || om != om ? om : m;
+          l = (l == 0.f ? 0.f : l * exp2_fast(m - m2)) + (ol == 0.f ? 0.f : ol * exp2_fast(om - m2));
+          m = m2;
+        };
+        meet(xpart<1>(m), xpart<1>(l));
+        meet(xpart<2>(m), xpart<2>(l));
+        meet(xpart<4>(m), xpart<4>(l));
+        meet(xpart<8>(m), xpart<8>(l));
+        if ((t & 15) == 0) {
+          px.m[h] = m;
+          px.l[h] = l;
+          px.first[h] = b0;
+          px.count[h] = b0 == b1 ? 0 : b1 - b0 + 1;
+          px.col[h] = c16;
+        }
+      }
+      __syncthreads();
+      return true;
+    } else {
+      return false;
+    }
+  };
+  // 4 values of a head, own ones over the maximum m with sum l, joined with the prefix's and
+  // the sink's weight
+  auto with_prefix = [&](const AttnItem& it, auto& px, int h, int d, float m, float l, float (&v)[4]) {
+    if constexpr (is_shared<A>) {
+      const int pct = a.plan[2] * 16;
+      const int64_t size = (int64_t)pct * (a.hd + 2);
+      const float pm = px.m[h], pl = px.l[h];
+      float M = -__builtin_inff();
+      auto top = [&](float x) { M = x > M || x != x ? x : M; };
+      if (l != 0.f) top(m);
+      if (pl != 0.f) top(pm);
+      const float sk = a.sinks ? a.sinks[it.head0 + h] * LOG2E : -__builtin_inff();
+      if (sk != -__builtin_inff()) top(sk);
+      const float fo = l != 0.f ? exp2_fast(m - M) : 0.f, fp = pl != 0.f ? exp2_fast(pm - M) : 0.f;
+      const float L = l * fo + pl * fp + (sk != -__builtin_inff() ? exp2_fast(sk - M) : 0.f);
+      float p[4] = {0.f, 0.f, 0.f, 0.f};
+      if (pl != 0.f) {
+        if (px.count[h] == 0) {
+          const float* const e = a.y + (int64_t)it.row * a.heads * a.hd + (int64_t)(it.head0 + h) * a.hd + d;
+#pragma unroll
+          for (int i = 0; i < 4; i++) p[i] = e[i];
+        } else {
+          const int np = px.count[h];
+#pragma unroll 4
+          for (int i = 0; i < np; i++) {
+            const float* const e = a.pieces + (2 * (int64_t)(px.first[h] + i) + (i == 0)) * size;
+            const float x = e[pct * a.hd + px.col[h]], w2 = x == -__builtin_inff() ? 0.f : exp2_fast(x - pm);
+            const floatx4 o4 = *(const floatx4*)(e + (int64_t)px.col[h] * a.hd + d);
+#pragma unroll
+            for (int k = 0; k < 4; k++) p[k] = __builtin_fmaf(w2, w2 != 0.f ? o4[k] : 0.f, p[k]);
+          }
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const float x = (fo != 0.f ? v[i] * fo : 0.f) + (fp != 0.f ? p[i] * fp : 0.f);
+        v[i] = L != 0.f ? x / L : 0.f;
+      }
+    }
+  };
+  __shared__ typename std::conditional<is_shared<A>, AttnPrefix, int>::type px;
   // all tiles (each wave for itself); rows without a key are zeros
   uint32_t all = 0, n0 = 0, live = 0;  // tiles, those of the lane's first sequence; sequences with any
   int64_t lo0 = 0, hi0 = 0;  // of the first 64 sequences, a lane each
@@ -372,6 +538,27 @@ __device__ __forceinline__ void paged_attention_t(const A& a)
     live += __popcll(__ballot(n != 0));
     for (uint64_t z = __ballot(zero); z; z &= z - 1) {
       float* const y = a.y + (int64_t)row_of(s0 + __builtin_ctzll(z)) * row_out;
+      if constexpr (is_shared<A>) {
+        // no token of its own: the prefix alone, where there is one
+        AttnItem it;
+        it.s = s0 + __builtin_ctzll(z);
+        it.row = row_of(it.s);
+        bool done = true;
+        for (int i = 0; i < (int)per && done; i++) {
+          it.kv = i / a.tiles;
+          it.heads = min(16, a.group - 16 * (i % a.tiles));
+          it.head0 = it.kv * a.group + 16 * (i % a.tiles);
+          done = prefix_of(it, px);
+          if (!done) break;
+          for (int j = 4 * t; j < it.heads * a.hd; j += 1024) {
+            float v[4] = {0.f, 0.f, 0.f, 0.f};
+            with_prefix(it, px, j / a.hd, j % a.hd, 0.f, 0.f, v);
+#pragma unroll
+            for (int e = 0; e < 4; e++) y[(int64_t)it.head0 * a.hd + j + e] = v[e];
+          }
+        }
+        if (done) continue;
+      }
       for (int i = t; i < row_out; i += 256) y[i] = 0.f;
     }
   }
@@ -705,6 +892,7 @@ __device__ __forceinline__ void paged_attention_t(const A& a)
       paged_walk<T, D>(a, it, lo + (int64_t)tile0 * S::TK, min(hi, lo + (int64_t)tile1 * S::TK), s);
 
     float* const y = a.y + (int64_t)it.row * row_out + (int64_t)it.head0 * a.hd;
+    bool pre = false;  // joined with a prefix (where this block ends the item)
     // with the sink: its weight beside the sum's, both against the larger maximum
     auto finish = [&](int h, float m2, float l2, float& f2) {
       f2 = 1.f;
@@ -720,7 +908,19 @@ __device__ __forceinline__ void paged_attention_t(const A& a)
       f2 = l2 != 0.f ? f2 / l2 : 0.f;
     };
     if (tile0 == 0 && tile1 == n) {
-      for (int h = w; h < it.heads; h += 4) {
+      if constexpr (is_shared<A>) {
+        pre = prefix_of(it, px);
+        for (int j = 4 * t; pre && j < it.heads * a.hd; j += 1024) {
+          const int h = j / a.hd, d = j - h * a.hd;
+          float v[4];
+#pragma unroll
+          for (int e = 0; e < 4; e++) v[e] = s.o[h * S::OS + d + e];
+          with_prefix(it, px, h, d, s.m[h], s.l[h], v);
+#pragma unroll
+          for (int e = 0; e < 4; e++) y[j + e] = v[e];
+        }
+      }
+      for (int h = w + (pre ? 16 : 0); h < it.heads; h += 4) {
         float f2;
         finish(h, s.m[h], s.l[h], f2);
         for (int d = lane; d < hd; d += 64) y[h * a.hd + d] = f2 == 0.f ? 0.f : s.o[h * S::OS + d] * f2;
@@ -749,6 +949,8 @@ __device__ __forceinline__ void paged_attention_t(const A& a)
       auto join = [&](uint32_t i0, uint32_t step, uint32_t cnt, bool out) {
         // 4 values of 16 pieces a thread, the first on their way while the weights are formed
         const int total = it.heads * a.hd;
+        if constexpr (is_shared<A>)
+          if (out) pre = prefix_of(it, px);
         uint64_t x[16][2];
         auto fetch = [&](int i, uint32_t j0) {
 #pragma unroll
@@ -810,7 +1012,11 @@ __device__ __forceinline__ void paged_attention_t(const A& a)
               }
             }
           }
-          if (out) {
+          if (out && pre) {
+            with_prefix(it, px, h, i - h * a.hd, s.m[h], s.l[h], v);
+#pragma unroll
+            for (int e = 0; e < 4; e++) y[i + e] = v[e];
+          } else if (out) {
             float f2;
             finish(h, s.m[h], s.l[h], f2);
 #pragma unroll

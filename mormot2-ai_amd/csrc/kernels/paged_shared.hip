@@ -1,0 +1,608 @@
+// paged_shared.hip - attention of one new token of each sequence where groups of
+// sequences share their first tokens: a launch over the prefixes, each read once for
+// all of its group's queries, and one over the sequences' own tokens, which joins them.
+// Built once for each type of pages (IHIP_SHARED_T: 0 single, 1 half, 2 bf16, 3 8-bit).
+#include "paged_attention.h"
+
+using namespace ihip;
+
+// columns (a member's query head each) of a block: 16 CT
+template <int D>
+constexpr int shared_ct = D <= 128 ? 4 : D == 256 ? 2 : 1;
+
+template <int T, int D>
+struct PrefixLds : AttnScales<T> {
+  using S = AttnShape<T, D>;
+  static constexpr int CT = shared_ct<D>;
+  uintx4 q[CT][S::NP * S::DS * S::NF * 64];  // the query tiles as the matrix cores take them
+  float o[16 * S::OS];
+  float m[16], l[16];
+  float wm[4][16], wl[4][16];
+  float qs[CT * 16];
+  int64_t at[CT * 16];  // a column's query and output, from q and y (rows of q_stride and heads * hd): row, -1 none
+  int head[CT * 16];
+  int keys[CT * 16];    // of a column: the prefix's tokens that its sequence has
+  int64_t off[4][2][S::KS];
+  floatx4 x[S::DS > 1 ? 2 : 1][S::DS > 1 ? 4 : 1][S::NT][64];
+};
+
+// a tile of 16 columns by the formula's own steps, where sums are not all finite
+// (paged_walk's reasons)
+template <int T, int D>
+__device__ __forceinline__ void prefix_walk(const PagedSharedArgs& a, const int* table, int kv, int ct, int64_t j0,
+                                            int64_t j1, PrefixLds<T, D>& s)
+{
+  using S = AttnShape<T, D>;
+  constexpr int NV = D / 64;
+  const int t = threadIdx.x, lane = t & 63, w = t >> 6;
+  __shared__ float tmp[4 * D];
+  for (int h = 0; h < 16; h++) {
+    const int col = 16 * ct + h;
+    if (s.at[col] < 0) continue;
+    const float* const qp = a.q + s.at[col] * a.q_stride + (int64_t)s.head[col] * a.hd;
+    float q[NV], acc[NV];
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+      const int d = lane + 64 * i;
+      q[i] = d < a.hd ? qp[d] * a.scale : 0.f;
+      acc[i] = 0.f;
+    }
+    float m = -__builtin_inff(), l = 0.f;
+    const int64_t end = min(j1, (int64_t)s.keys[col]);
+    for (int64_t j = j0 + w; j < end; j += 4) {
+      const int page = table[(uint32_t)j / (uint32_t)a.page_size], in = (int)((uint32_t)j % (uint32_t)a.page_size);
+      const int64_t at = paged_value(page, in, a.pages, a.page_stride, a.slot_stride);
+      if (at < 0) continue;
+      const int64_t row = (at + kv * a.head_stride) * S::ES;
+      float x = 0.f, vscale = 1.f, kscale = 1.f;
+      if constexpr (T == 3) {
+        const int64_t sc = page * a.s_page + (int64_t)in * a.s_slot + kv * a.s_head;
+        kscale = a.ks[sc];
+        vscale = a.vs[sc];
+      }
+#pragma unroll
+      for (int i = 0; i < NV; i++)
+        if (lane + 64 * i < a.hd) x = __builtin_fmaf(q[i], load1<T>(a.kc + row + (lane + 64 * i) * S::ES), x);
+      x = wave_sum(x, 64);
+      if constexpr (T == 3) x *= kscale;
+      if (x == -__builtin_inff()) continue;
+      const float m2 = x > m || x != x ? x : m;
+      const float f = m == -__builtin_inff() ? 0.f : exp2_fast(m - m2), p = exp2_fast(x - m2);
+      l = l * f + p;
+      m = m2;
+#pragma unroll
+      for (int i = 0; i < NV; i++)
+        if (lane + 64 * i < a.hd)
+          acc[i] = __builtin_fmaf(p, load1<T>(a.vc + row + (lane + 64 * i) * S::ES) * (T == 3 ? vscale : 1.f), acc[i] * f);
+    }
+#pragma unroll
+    for (int i = 0; i < NV; i++) tmp[w * D + lane + 64 * i] = acc[i];
+    if (lane == 0) {
+      s.wm[w][0] = m;
+      s.wl[w][0] = l;
+    }
+    __syncthreads();
+    float M = -__builtin_inff(), L = 0.f, f[4];
+    for (int i = 0; i < 4; i++) M = s.wm[i][0] > M || s.wm[i][0] != s.wm[i][0] ? s.wm[i][0] : M;
+    for (int i = 0; i < 4; i++) {
+      f[i] = s.wl[i][0] == 0.f ? 0.f : exp2_fast(s.wm[i][0] - M);
+      L += f[i] * s.wl[i][0];
+    }
+    for (int d = t; d < a.hd; d += 256) {
+      float v = 0.f;
+      for (int i = 0; i < 4; i++)
+        if (s.wl[i][0] != 0.f) v += f[i] * tmp[i * D + d];
+      s.o[h * S::OS + d] = v;
+    }
+    if (t == 0) {
+      s.m[h] = M;
+      s.l[h] = L;
+    }
+    __syncthreads();
+  }
+}
+
+// The queries of a group's members for one KV head are the columns of one problem, which
+// reads the prefix's keys and values once for 16 CT of them: scores K q^T and values V^T
+// P as paged_attention's, a wave's keys and values in registers used for CT tiles of 16
+// columns, the query tiles in LDS. All groups' tiles of keys are one row, shared out
+// evenly over the grid. A block that has the whole of an item (KV head, columns) finishes
+// it into y and lse; parts go to `pieces`, and the launch over the sequences' own tokens
+// joins them.
+template <int T, int D, bool FULL>
+__device__ __forceinline__ void paged_prefix_t(const PagedSharedArgs& a)
+{
+  using S = AttnShape<T, D>;
+  constexpr int CT = shared_ct<D>, COLS = 16 * CT;
+  __shared__ PrefixLds<T, D> s;
+  const int t = threadIdx.x, lane = t & 63, c = lane & 15, g = lane >> 4;
+  const int w = __builtin_amdgcn_readfirstlane(t >> 6);
+  const uint32_t grid = gridDim.x, b = blockIdx.x;
+  const int hd = FULL ? D : a.hd, row_out = a.heads * a.hd;
+
+  // a group's items of a KV head and tiles of keys
+  auto shape_of = [&](int grp, uint32_t& items, int64_t& common) {
+    const int m0 = a.members[grp], m1 = a.members[grp + 1];
+    common = paged_common(m0, m1, a.shared[grp], a.seqs, a.max_pages, a.page_size);
+    items = common > 0 ? ((uint32_t)(m1 - m0) * a.group + COLS - 1) / COLS : 0;
+    return (uint32_t)((common + S::TK - 1) / S::TK);
+  };
+  uint64_t total = 0;
+  for (int g0 = 0; g0 < a.groups; g0 += 64) {
+    uint32_t items = 0, n = 0;
+    int64_t common;
+    if (g0 + lane < a.groups) n = shape_of(g0 + lane, items, common);
+    total += wave_sum((uint64_t)n * items * (uint32_t)a.kvh, 64);
+  }
+  // (groups that overlap, which no caller has, may pass 32 bits)
+  const uint32_t all = total < (1u << 31) ? __builtin_amdgcn_readfirstlane((uint32_t)total) : 0u;
+  const uint32_t B = min(grid, all);
+  if (b == 0) {
+    if (t == 0) {
+      a.plan[0] = (int)all;
+      a.plan[1] = (int)B;
+      a.plan[2] = CT;
+    }
+    if (w == 0) {
+      uint32_t before = 0;
+      for (int g0 = 0; g0 < a.groups; g0 += 64) {
+        uint32_t items = 0, n = 0;
+        int64_t common;
+        if (g0 + lane < a.groups) n = shape_of(g0 + lane, items, common);
+        const uint32_t mine = n * items * a.kvh;
+        uint32_t upto = mine;
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+          const uint32_t o = __shfl_up(upto, d, 64);
+          if (lane >= d) upto += o;
+        }
+        if (g0 + lane < a.groups) {
+          int* const e = a.plan + SHARED_PLAN + 3 * (g0 + lane);
+          e[0] = (int)(before + upto - mine);
+          e[1] = (int)n;
+          e[2] = (int)items;
+        }
+        before += __shfl(upto, 63, 64);
+      }
+    }
+  }
+  if (b >= B) return;
+  const PieceShare share(all, B);
+  uint32_t u = share.first(b);
+  const uint32_t end = share.first(b + 1);
+  // the group of tile u
+  int grp = 0;
+  uint32_t before = 0, n = 0, items = 0;
+  int64_t common = 0;
+  for (;; grp++) {
+    if (grp >= a.groups) return;
+    n = shape_of(grp, items, common);
+    if (before + n * items * a.kvh > u) break;
+    before += n * items * a.kvh;
+  }
+  grp = __builtin_amdgcn_readfirstlane(grp);
+
+  for (;;) {
+    const uint32_t item = (u - before) / n, tile0 = (u - before) - item * n;
+    const uint32_t tile1 = min(n, tile0 + (end - u));
+    const int kv = item / items, col0 = (int)(item - kv * items) * COLS;
+    const int m0 = a.members[grp], cols = (a.members[grp + 1] - m0) * a.group;
+    const char* const kb = a.kc + (int64_t)kv * a.head_stride * S::ES;
+    const char* const vb = a.vc + (int64_t)kv * a.head_stride * S::ES;
+    const float* sb = nullptr;
+    float scale = 0.f;
+    if constexpr (T == 3) sb = (lane < S::KS ? a.ks : a.vs) + (int64_t)kv * a.s_head;
+    const int* const table = a.table + (int64_t)m0 * a.max_pages;
+    const int kg = w / S::DS, dh = w % S::DS;
+    const int64_t wlo = kg * S::KS;
+    const int64_t jend = min(common, (int64_t)tile1 * S::TK);
+    auto entry = [&](uint32_t tile) {
+      const int64_t j = wlo + (int64_t)tile * S::TK + (lane & (S::KS - 1));
+      return j < jend ? table[(uint32_t)j / (uint32_t)a.page_size] : -1;
+    };
+    auto locate = [&](uint32_t tile, int page) {
+      const int64_t j = wlo + (int64_t)tile * S::TK + (lane & (S::KS - 1));
+      const int in = (int)((uint32_t)j % (uint32_t)a.page_size);
+      const int64_t at = paged_value(page, in, a.pages, a.page_stride, a.slot_stride);
+      if (lane < S::KS) s.off[w][tile & 1][lane] = at < 0 ? 0 : at * S::ES;
+      if constexpr (T == 3) scale = at < 0 ? 0.f : sb[page * a.s_page + (int64_t)in * a.s_slot];
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      return (uint32_t)__ballot(at >= 0) & (uint32_t)((1ull << S::KS) - 1);
+    };
+    uint32_t tile = tile0;
+    const int page0 = entry(tile);
+    int page = entry(tile + 1);
+
+    // the columns: a member's row, its head, the keys that it sees
+    if (t < COLS) {
+      const int col = col0 + t, seq = m0 + col / a.group;
+      int64_t at = -1;
+      int keys = 0;
+      if (col < cols) {
+        const int row = a.offsets ? paged_row(a.offsets[seq], a.offsets[seq + 1], a.rows) : paged_row(seq, seq + 1, a.rows);
+        if (row >= 0 && a.lengths[seq] >= 0) {
+          at = row;
+          keys = (int)min((int64_t)a.lengths[seq], common);
+        }
+      }
+      s.at[t] = at;
+      s.head[t] = kv * a.group + col % a.group;
+      s.keys[t] = keys;
+    }
+    __syncthreads();
+    // the query tiles (stage_query's form)
+    if constexpr (T == 1 || T == 3) {
+      for (int ct = 0; ct < CT; ct++) {
+        const int col = 16 * ct + (t >> 4);
+        float top = 0.f;
+        if (s.at[col] >= 0) {
+          const float* const q = a.q + s.at[col] * a.q_stride + (int64_t)s.head[col] * a.hd;
+          for (int d = t & 15; d < a.hd; d += 16) top = fmaxf(top, fabsf(q[d] * a.scale));
+        }
+        top = fmaxf(top, xpart<1>(top));
+        top = fmaxf(top, xpart<2>(top));
+        top = fmaxf(top, xpart<4>(top));
+        top = fmaxf(top, xpart<8>(top));
+        if ((t & 15) == 0) {
+          int e = (int)(float_bits(top) >> 23) - 126;  // top < 2^e
+          if (top == 0.f || !finite(top)) e = 14;
+          s.qs[col] = ldexpf(1.f, max(e - 14, -120));
+        }
+      }
+      __syncthreads();
+    }
+    for (int i = t; i < CT * S::DS * S::NF * 64; i += 256) {
+      const int ct = i / (S::DS * S::NF * 64), j = i % (S::DS * S::NF * 64);
+      const int col = 16 * ct + (j & 15), d0 = S::factor(j >> 6, (j >> 4) & 3);
+      const bool in = s.at[col] >= 0 && d0 < a.hd;
+      const float* const q = a.q + (in ? s.at[col] * a.q_stride + (int64_t)s.head[col] * a.hd + d0 : 0);
+      float f = a.scale, v[S::FL];
+      if constexpr (T == 1 || T == 3) f = 1.f / s.qs[col];
+#pragma unroll
+      for (int e = 0; e < S::FL; e++) {
+        v[e] = in ? q[e] : 0.f;
+        v[e] = T == 1 || T == 3 ? v[e] * a.scale * f : v[e] * f;
+      }
+      if constexpr (T == 0) {
+        s.q[ct][j] = uintx4{float_bits(v[0]), float_bits(v[1]), float_bits(v[2]), float_bits(v[3])};
+      } else {
+        uint32_t part[4][S::NP];
+#pragma unroll
+        for (int e = 0; e < 4; e++) split2<T>(v[2 * e], v[2 * e + 1], part[e]);
+#pragma unroll
+        for (int p = 0; p < S::NP; p++) s.q[ct][p * S::DS * S::NF * 64 + j] = uintx4{part[0][p], part[1][p], part[2][p], part[3][p]};
+      }
+    }
+    __syncthreads();
+    float sscale[CT];
+    int keys[CT], least = INT32_MAX;  // of the lane's columns; the least of all
+#pragma unroll
+    for (int ct = 0; ct < CT; ct++) {
+      sscale[ct] = T == 1 || T == 3 ? s.qs[16 * ct + c] : 1.f;
+      keys[ct] = s.keys[16 * ct + c];
+      if (s.at[16 * ct + c] >= 0) least = min(least, keys[ct]);
+    }
+    least = -wave_max(-least);
+
+    uintx4 kr[S::NT][S::NQ];
+    auto load_keys = [&](uint32_t tile) {
+#pragma unroll
+      for (int i = 0; i < S::NT; i++) {
+        const char* const p = kb + s.off[w][tile & 1][16 * i + c];
+#pragma unroll
+        for (int j = 0; j < S::NQ; j++) {
+          const int d0 = dh * S::DW + j * 4 * S::QL + g * S::QL;
+          const bool in = FULL || d0 < hd;
+          kr[i][j] = *(const uintx4*)(p + (in ? d0 : 0) * S::ES);
+          if (!in) kr[i][j] = uintx4{0, 0, 0, 0};
+        }
+      }
+    };
+
+    floatx4 o[CT][S::NJ][S::VL];
+    float m[CT], l[CT];
+#pragma unroll
+    for (int ct = 0; ct < CT; ct++) {
+      m[ct] = -__builtin_inff();
+      l[ct] = 0.f;
+#pragma unroll
+      for (int i = 0; i < S::NJ; i++)
+#pragma unroll
+        for (int j = 0; j < S::VL; j++) o[ct][i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+    }
+    float vtop = 0x1p-100f, vinv = 0x1p100f;
+    uint32_t steps = 0;
+    if (S::DS > 1) {
+      steps = tile1 - tile0;
+    } else if (wlo + (int64_t)tile0 * S::TK < common) {
+      const uint32_t mine = (uint32_t)((common - wlo + S::TK - 1) / S::TK);
+      steps = min(tile1, mine) - tile0;
+    }
+    uint32_t there = locate(tile, page0);
+    if (steps) load_keys(tile);
+    for (uint32_t i = 0; i < steps; i++, tile++) {
+      constexpr int NV = 4 * S::NT;
+      uintx4 vr[NV][S::NJ];
+#pragma unroll
+      for (int k = 0; k < NV; k++) {
+        const char* const p = vb + s.off[w][tile & 1][16 * (k >> 2) + 4 * g + (k & 3)];
+#pragma unroll
+        for (int j = 0; j < S::NJ; j++) {
+          const int d0 = dh * S::DW + j * 16 * S::VL + c * S::VL;
+          const char* const v = p + (FULL || d0 < hd ? d0 : 0) * S::ES;
+          if constexpr (S::VL * S::ES == 4) {
+            vr[k][j] = uintx4{*(const uint32_t*)v, 0, 0, 0};
+          } else if constexpr (S::VL * S::ES == 16) {
+            vr[k][j] = *(const uintx4*)v;
+          } else {
+            const uintx2 h = *(const uintx2*)v;
+            vr[k][j] = uintx4{h[0], h[1], 0, 0};
+          }
+        }
+      }
+      const uint32_t now = there;
+      floatx4 ksc[T == 3 ? S::NT : 1], vsc[T == 3 ? S::NT : 1];
+      if constexpr (T == 3) {
+        s.sc[w][lane] = scale;
+        if (__any(lane >= 32 && fabsf(scale) >= vtop)) {
+          const uint32_t top = __builtin_amdgcn_readfirstlane(float_bits(wave_max(lane >= 32 ? fabsf(scale) : 0.f)));
+          const float v2 = bits_float(min((top & 0x7f800000u) + 0x00800000u, 0x7f000000u));
+          const float f = vtop / v2;
+          vtop = v2;
+          vinv = 1.f / v2;
+          products_done();
+#pragma unroll
+          for (int ct = 0; ct < CT; ct++)
+#pragma unroll
+            for (int j = 0; j < S::NJ; j++)
+#pragma unroll
+              for (int e = 0; e < S::VL; e++) o[ct][j][e] *= f;
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int k = 0; k < S::NT; k++) {
+          ksc[k] = *(const floatx4*)&s.sc[w][16 * k + 4 * g];
+          vsc[k] = *(const floatx4*)&s.sc[w][32 + 16 * k + 4 * g] * (vinv * S::PS);
+        }
+      }
+      // whether every column sees every key of the wave's step
+      const bool plain = now == (uint32_t)((1ull << S::KS) - 1) && wlo + (int64_t)tile * S::TK + S::KS <= least;
+      const int64_t key0 = wlo + (int64_t)tile * S::TK + 4 * g;
+      there = locate(tile + 1, page);
+      page = entry(tile + 2);
+      floatx4 x[CT][S::NT];
+#pragma unroll
+      for (int ct = 0; ct < CT; ct++)
+#pragma unroll
+        for (int k = 0; k < S::NT; k++) x[ct][k] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int j = 0; j < S::NF; j++) {
+        uintx4 kf[S::NT];
+#pragma unroll
+        for (int k = 0; k < S::NT; k++) {
+          if constexpr (T == 3) {
+            const uintx2 lo = codes4(kr[k][j / 2][2 * (j & 1)] ^ 0x80808080u), hi = codes4(kr[k][j / 2][2 * (j & 1) + 1] ^ 0x80808080u);
+            kf[k] = uintx4{lo[0], lo[1], hi[0], hi[1]};
+          } else {
+            kf[k] = kr[k][j];
+          }
+        }
+#pragma unroll
+        for (int ct = 0; ct < CT; ct++)
+#pragma unroll
+          for (int n2 = 0; n2 < S::NP; n2++) {
+            const uintx4 q = s.q[ct][(n2 * S::DS * S::NF + dh * S::NF + j) * 64 + lane];
+#pragma unroll
+            for (int k = 0; k < S::NT; k++) {
+              if constexpr (T == 0) {
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                  x[ct][k] = __builtin_amdgcn_mfma_f32_16x16x4f32(bits_float(kf[k][e]), bits_float(q[e]), x[ct][k], 0, 0, 0);
+              } else {
+                x[ct][k] = mfma16<T>(kf[k], q, x[ct][k]);
+              }
+            }
+          }
+      }
+      load_keys(tile + 1);
+      products_done();
+      if constexpr (S::DS > 1) {
+        static_assert(S::DS == 1 || CT == 1, "one tile of columns where waves share a head");
+#pragma unroll
+        for (int k = 0; k < S::NT; k++) s.x[tile & 1][w][k][lane] = x[0][k];
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < S::NT; k++) x[0][k] += s.x[tile & 1][w ^ 1][k][lane];
+      }
+      // keys that are not there: values of zero (0 times NaN is NaN)
+      if (T != 3 && now != (uint32_t)((1ull << S::KS) - 1)) {
+#pragma unroll
+        for (int k = 0; k < NV; k++)
+#pragma unroll
+          for (int j = 0; j < S::NJ; j++)
+            if (!(now >> (16 * (k >> 2) + 4 * g + (k & 3)) & 1)) vr[k][j] = uintx4{0, 0, 0, 0};
+      }
+      // the values turned: 8 keys of a dimension side by side
+      uintx4 vt[T == 0 ? 1 : S::NJ][T == 0 ? 1 : S::VL];
+      if constexpr (T != 0) {
+#pragma unroll
+        for (int j = 0; j < S::NJ; j++)
+#pragma unroll
+          for (int e = 0; e < S::VL; e++)
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+              if constexpr (T == 3) {
+                const uint32_t pair = __builtin_amdgcn_perm(vr[2 * k + 1][j][e / 4], vr[2 * k][j][e / 4],
+                                                            e & 2 ? 0x07030602u : 0x05010400u) ^ 0x80808080u;
+                vt[j][e][k] = halves_of(__builtin_amdgcn_perm(0x64646464u, pair, e & 1 ? 0x04030402u : 0x04010400u));
+              } else {
+                vt[j][e][k] = __builtin_amdgcn_perm(vr[2 * k + 1][j][e / 2], vr[2 * k][j][e / 2], e & 1 ? 0x07060302u : 0x05040100u);
+              }
+            }
+      }
+#pragma unroll
+      for (int ct = 0; ct < CT; ct++) {
+        float top = -__builtin_inff(), y[NV];
+#pragma unroll
+        for (int k = 0; k < NV; k++) y[k] = x[ct][k >> 2][k & 3] * (T == 3 ? sscale[ct] * ksc[T == 3 ? k >> 2 : 0][k & 3] : sscale[ct]);
+        if (!plain)
+#pragma unroll
+          for (int k = 0; k < NV; k++) {
+            const bool in = (now >> (16 * (k >> 2) + 4 * g + (k & 3)) & 1) && key0 + 16 * (k >> 2) + (k & 3) < keys[ct];
+            y[k] = in ? y[k] : -__builtin_inff();
+          }
+#pragma unroll
+        for (int k = 0; k < NV; k++) top = fmaxf(top, y[k]);
+        if (__any(top > m[ct])) {
+          top = quad_max(top);
+          const float m2 = fmaxf(top, m[ct]), f = m[ct] == -__builtin_inff() ? 0.f : exp2_fast(m[ct] - m2);
+          m[ct] = m2;
+          l[ct] *= f;
+#pragma unroll
+          for (int j = 0; j < S::NJ; j++)
+#pragma unroll
+            for (int e = 0; e < S::VL; e++) o[ct][j][e] *= f;
+        }
+        const float shift = m[ct] == -__builtin_inff() ? 0.f : m[ct];
+        float p[NV];
+#pragma unroll
+        for (int k = 0; k < NV; k++) {
+          p[k] = exp2_fast(y[k] - shift);
+          l[ct] += p[k];
+        }
+        if constexpr (T == 0) {
+#pragma unroll
+          for (int k = 0; k < NV; k++)
+#pragma unroll
+            for (int j = 0; j < S::NJ; j++)
+#pragma unroll
+              for (int e = 0; e < 4; e++)
+                o[ct][j][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(bits_float(vr[k][j][e]), p[k], o[ct][j][e], 0, 0, 0);
+        } else {
+          uint32_t part[4][S::NP];
+#pragma unroll
+          for (int k = 0; k < 4; k++) {
+            if constexpr (T == 3)
+              split2<T>(p[2 * k] * vsc[k >> 1][2 * k & 3], p[2 * k + 1] * vsc[k >> 1][(2 * k + 1) & 3], part[k]);
+            else
+              split2<T>(p[2 * k] * S::PS, p[2 * k + 1] * S::PS, part[k]);
+          }
+#pragma unroll
+          for (int j = 0; j < S::NJ; j++)
+#pragma unroll
+            for (int e = 0; e < S::VL; e++)
+#pragma unroll
+              for (int n2 = 0; n2 < S::NP; n2++)
+                o[ct][j][e] = mfma16<T>(vt[j][e], uintx4{part[0][n2], part[1][n2], part[2][n2], part[3][n2]}, o[ct][j][e]);
+        }
+      }
+    }
+
+    // the waves' sums meet, 16 columns at a time
+    products_done();
+    const bool whole = tile0 == 0 && tile1 == n;
+    float* const pc = a.pieces + (int64_t)(2 * b + (tile0 ? 0 : 1)) * COLS * (a.hd + 2);
+#pragma unroll
+    for (int ct = 0; ct < CT; ct++) {
+      l[ct] = quad_sum(l[ct]);
+      if (g == 0 && dh == 0) {
+        s.wm[kg][c] = m[ct];
+        s.wl[kg][c] = l[ct];
+      }
+      __syncthreads();
+      float M = s.wm[0][c];
+#pragma unroll
+      for (int i = 1; i < S::KG; i++) M = fmaxf(M, s.wm[i][c]);
+      const float Ms = M == -__builtin_inff() ? 0.f : M;
+      const float f = exp2_fast(m[ct] - Ms) * (1.f / S::PS) * (T == 3 ? vtop : 1.f);
+      bool odd = false;
+      if (w == 0 && g == 0) {
+        float L = 0.f;
+#pragma unroll
+        for (int i = 0; i < S::KG; i++) L += s.wl[i][c] * exp2_fast(s.wm[i][c] - Ms);
+        s.m[c] = M;
+        s.l[c] = L;
+        odd = s.at[16 * ct + c] >= 0 && !finite(L);
+      }
+      for (int r4 = 0; r4 < S::KG; r4++) {
+        if (kg == r4) {
+#pragma unroll
+          for (int j = 0; j < S::NJ; j++)
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+#pragma unroll
+              for (int e = 0; e < S::VL; e += 4) {
+                floatx4* const d = (floatx4*)&s.o[c * S::OS + dh * S::DW + j * 16 * S::VL + S::VL * (4 * g + r) + e];
+                floatx4 v = {o[ct][j][e][r] * f, o[ct][j][e + 1][r] * f, o[ct][j][e + 2][r] * f, o[ct][j][e + 3][r] * f};
+                if (r4) v += *d;
+                *d = v;
+              }
+        }
+        __syncthreads();
+      }
+      for (int h = w; h < 16; h += 4)
+        if (s.at[16 * ct + h] >= 0)
+          for (int d = lane; d < hd; d += 64) odd |= !finite(s.o[h * S::OS + d]);
+      if (__syncthreads_or(odd))
+        prefix_walk<T, D>(a, table, kv, ct, (int64_t)tile0 * S::TK, jend, s);
+      for (int h = w; h < 16; h += 4) {
+        const int col = 16 * ct + h;
+        if (s.at[col] < 0) continue;
+        const float M2 = s.m[h], L2 = s.l[h];
+        if (whole) {
+          const float inv = L2 != 0.f ? 1.f / L2 : 0.f;
+          float* const y = a.y + s.at[col] * row_out + (int64_t)s.head[col] * a.hd;
+          for (int d = lane; d < hd; d += 64) y[d] = L2 == 0.f ? 0.f : s.o[h * S::OS + d] * inv;
+          if (lane == 0)
+            a.lse[(int64_t)(m0 + (col0 + col) / a.group) * a.heads + s.head[col]] = L2 == 0.f ? -__builtin_inff() : M2 + __builtin_amdgcn_logf(L2);
+        } else {
+          for (int d = lane; d < hd; d += 64) pc[col * a.hd + d] = s.o[h * S::OS + d];
+          if (lane == 0) {
+            pc[COLS * a.hd + col] = L2 == 0.f ? -__builtin_inff() : M2;
+            pc[COLS * a.hd + COLS + col] = L2;
+          }
+        }
+      }
+      __syncthreads();
+    }
+    u += tile1 - tile0;
+    if (u >= end) return;
+    if (tile1 == n && item + 1 == items * a.kvh) {  // the next group with a prefix
+      before = u;
+      do {
+        if (++grp >= a.groups) return;
+        n = shape_of(grp, items, common);
+      } while (n == 0);
+    }
+  }
+}
+
+#define PAGED_SHARED2(NAME, T, D, SUFFIX, FULL)                                                                   \
+  extern "C" __global__ __launch_bounds__(256) void paged_prefix_##NAME##_##D##SUFFIX(PagedSharedArgs a)          \
+  {                                                                                                               \
+    paged_prefix_t<T, D, FULL>(a);                                                                                \
+  }                                                                                                               \
+  extern "C" __global__ __launch_bounds__(256) void paged_own_##NAME##_##D##SUFFIX(PagedSharedArgs a)             \
+  {                                                                                                               \
+    paged_attention_t<T, D, FULL>(a);                                                                             \
+  }
+#define PAGED_SHARED1(NAME, T)                  \
+  PAGED_SHARED2(NAME, T, 64, , true)            \
+  PAGED_SHARED2(NAME, T, 64, _part, false)      \
+  PAGED_SHARED2(NAME, T, 128, , true)           \
+  PAGED_SHARED2(NAME, T, 128, _part, false)     \
+  PAGED_SHARED2(NAME, T, 256, , true)           \
+  PAGED_SHARED2(NAME, T, 256, _part, false)     \
+  PAGED_SHARED2(NAME, T, 512, , true)           \
+  PAGED_SHARED2(NAME, T, 512, _part, false)
+#if IHIP_SHARED_T == 0
+PAGED_SHARED1(f32, 0)
+#elif IHIP_SHARED_T == 1
+PAGED_SHARED1(f16, 1)
+#elif IHIP_SHARED_T == 2
+PAGED_SHARED1(bf16, 2)
+#else
+PAGED_SHARED1(q8, 3)
+#endif

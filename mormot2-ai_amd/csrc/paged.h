@@ -22,6 +22,16 @@ IHIP_HD void paged_range(int32_t length, int64_t window, int64_t max_pages, int3
   *lo = window > 0 && n > window ? n - window : 0;
 }
 
+// how many tokens a group of the sequences [first, end) of `seqs` reads together: those of
+// its `shared` that its tables hold, none where fewer than two sequences are its
+IHIP_HD int64_t paged_common(int32_t first, int32_t end, int32_t shared, int32_t seqs, int64_t max_pages,
+                             int32_t page_size)
+{
+  if (first < 0 || end > seqs || end <= first || end - first < 2 || shared <= 0) return 0;
+  const int64_t most = max_pages * page_size;
+  return shared < most ? shared : most;
+}
+
 // the row of q and y of a sequence whose rows of the step are [first, end): the
 // last of them, or -1 where it has none or its last is not among the `rows`
 IHIP_HD int32_t paged_row(int32_t first, int32_t end, int32_t rows)

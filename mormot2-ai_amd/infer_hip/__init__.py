@@ -182,6 +182,9 @@ def lib():
             "ihip_enqueue_paged_qkrope": (i32, [vp, u64, i64, u64, i64, u64, i64, i64, i64, u64,
                                                 u64, C.c_double, C.POINTER(Rope), u64, u64,
                                                 C.POINTER(Pages), u64]),
+            "ihip_enqueue_paged_attention_shared": (i32, [vp, u64, i64, C.POINTER(Pages), u64, i64, u64, u64,
+                                                          i64, u64, u64, i64, u64, i64, i64, i64, u64,
+                                                          C.c_double]),
             "ihip_enqueue_paged_read": (i32, [vp, C.POINTER(Pages), u64, i64, u64, u64, i64, i64, i32, u64,
                                               u64]),
             "ihip_enqueue_paged_attention": (i32, [vp, u64, i64, C.POINTER(Pages), u64, i64, u64,
