@@ -724,6 +724,19 @@ int ihip_enqueue_paged_attention_shared(ihip_ctx* ctx, uint64_t q, int64_t q_str
 int ihip_enqueue_paged_read(ihip_ctx* ctx, const ihip_pages* cache, uint64_t table, int64_t max_pages,
                             uint64_t first, uint64_t offsets, int64_t seqs, int64_t rows, int out_type,
                             uint64_t k_out, uint64_t v_out);
+/* a draw for every row of logits (TInferSampler.Next, sampler.pas:269-435, with its
+ * filters and their order, for rows with settings and random numbers of their own):
+ * settings [rows] of ihip_sampling on the device (the seed is not read), uniform [rows]
+ * doubles in [0, 1), logits [rows, vocab] (vocab up to 2^22, rows to 2^24), `stride`
+ * floats from a row to the next (0: vocab). ids [rows] (int32) receives the tokens, probs
+ * [rows] (or 0) the probability that each had among those that its filters left (1 of a
+ * greedy row). A temperature of 0 or below (or below 1e-30) is greedy: the largest logit,
+ * the lowest id on a tie, NaN skipped; so is a row whose largest logit is infinite. Logits
+ * of -infinity and NaN are never drawn. Settings
+ * that ihip_sampler_create refuses give id -1 and probability 0, for that row alone. */
+int ihip_enqueue_sample_rows(ihip_ctx* ctx, uint64_t logits, int64_t rows, int64_t vocab,
+                             int64_t stride, uint64_t settings, uint64_t uniform, uint64_t ids,
+                             uint64_t probs);
 /* what a row of logits says of its tokens: logits [rows, vocab] (vocab up to
  * 2^22, rows to 2^24), `stride` floats from a row to the next (0: vocab);
  * - logprobs [rows] (or 0): log softmax of token ids[r] (int32), NaN for an id

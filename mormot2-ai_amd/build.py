@@ -23,7 +23,8 @@ LINEAR_FMTS = ["q8_0", "q4_0", "mxfp4", "q5_0", "q5_1", "q4_k", "q6_k", "f32", "
 # gemm.hip (the MFMA prefill GEMM) once per quantized weight type
 GEMM_FMTS = ["q8_0", "q4_0", "mxfp4", "q5_0", "q5_1", "q4_k", "q6_k", "f32", "bf16", "f16"]
 KERNELS = ([("ops", "ops", []), ("deltanet", "deltanet", []), ("paged", "paged", []),
-            ("paged_q8", "paged_q8", []), ("logprobs", "logprobs", [])] +
+            ("paged_q8", "paged_q8", []), ("sample_rows", "sample_rows", []),
+            ("logprobs", "logprobs", [])] +
            [("paged_shared_" + f, "paged_shared", ["-DIHIP_SHARED_T=%d" % i])
             for i, f in enumerate(["f32", "f16", "bf16", "q8"])] +
            [("linear_" + f, "linear", ["-DIHIP_ONLY_FMT_" + f.upper()]) for f in LINEAR_FMTS] +

@@ -106,6 +106,7 @@ struct ihip_ctx {
   uint64_t paged_plan = 0;  // the step plan between ihip_enqueue_paged_slots' two launches, a counter behind it
   uint64_t paged_part = 0;  // paged_attention's shared pieces and counters (zero between launches)
   uint64_t paged_shared = 0;  // parts of shared prefixes, their sums' logarithms, and the plan of them
+  uint64_t sample_rows = 0;  // ihip_enqueue_sample_rows' parts of the rows
   uint64_t logprobs_part = 0;  // the same of ihip_enqueue_logprobs
   uint64_t scratch_planes = 0, scratch_planes_bytes = 0;  // e4m3 activation planes (gemm_mxfp4_f8)
   // the device address of static_scratch.hip's array on this device
@@ -169,6 +170,8 @@ constexpr uint64_t SHARED_BYTES = SHARED_PIECE_BYTES + SHARED_HEADS * 4 + (4 + 3
 // doubles and IHIP_LOGPROBS_TOP alternatives each), and a counter of 32 bytes a row
 constexpr int64_t LOGPROBS_BLOCKS = 1024;
 constexpr uint64_t LOGPROBS_PART_BYTES = LOGPROBS_BLOCKS * (3 + IHIP_LOGPROBS_TOP) * 8;
+// sample_rows: the parts' and chunks' results of as many rows as one launch takes
+constexpr uint64_t SAMPLE_ROWS_BYTES = 24u << 20;
 constexpr uint64_t PAGED_PLAN_BYTES = (5 * IHIP_PAGED_SEQS + 8) * 4;
 
 struct LinearCall {

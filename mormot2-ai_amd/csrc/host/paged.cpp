@@ -368,6 +368,67 @@ int ihip_enqueue_paged_read(ihip_ctx* c, const ihip_pages* cache, uint64_t table
   return launch(c, name, dim3((unsigned)std::min<int64_t>((turns + 3) / 4, 64 * c->cus)), dim3(256), &a);
 }
 
+int ihip_enqueue_sample_rows(ihip_ctx* c, uint64_t logits, int64_t rows, int64_t vocab, int64_t stride,
+                             uint64_t settings, uint64_t uniform, uint64_t ids, uint64_t probs)
+{
+  const char* who = "ihip_enqueue_sample_rows";
+  if (!logits || !settings || !uniform || !ids) return refuse(who, "a missing array");
+  if (rows < 1 || rows > (int64_t)1 << 24 || vocab < 1 || vocab > 1 << 22)
+    return refuse(who, "rows or vocab out of range");
+  stride = stride ? stride : vocab;
+  if (stride < vocab) return refuse(who, "a stride below a row");
+  if (stride > STRIDE_MOST) return refuse(who, "a stride beyond 2^36");
+  if ((logits | ids | probs) % 4) return refuse(who, "arrays aligned to 4 bytes");
+  if ((settings | uniform) % 8) return refuse(who, "settings and random numbers are doubles, aligned to 8 bytes");
+  if (!c) return no_context(who);
+  OnDevice on(c);
+  // parts of 8192 tokens, of 2048 where they would leave the chip's CUs empty
+  const int64_t per = rows * ((vocab + 8191) / 8192) < 2 * c->cus ? 2048 : 8192;
+  const int64_t parts = (vocab + per - 1) / per, chunks = (vocab + 255) / 256;
+  // a row's results: a double, two words and 32 octaves a part, a word a chunk
+  const int64_t bytes = parts * (8 + 8 + 32 * 4) + chunks * 4;
+  const int64_t most = std::min<int64_t>({rows, 65535, (int64_t)(SAMPLE_ROWS_BYTES / bytes)});
+  struct {
+    const float* x;
+    int64_t stride;
+    const ihip_sampling* settings;
+    const double* uniform;
+    int* ids;
+    float* probs;
+    float* best;
+    int* best_id;
+    double* sum;
+    uint32_t* octaves;
+    float* chunk;
+    int32_t rows, vocab, parts, chunks, wide, per;
+  } a = {};
+  a.stride = stride;
+  a.sum = (double*)c->sample_rows;
+  a.best = (float*)(a.sum + most * parts);
+  a.best_id = (int*)(a.best + most * parts);
+  a.octaves = (uint32_t*)(a.best_id + most * parts);
+  a.chunk = (float*)(a.octaves + most * parts * 32);
+  a.vocab = (int32_t)vocab;
+  a.parts = (int32_t)parts;
+  a.chunks = (int32_t)chunks;
+  a.wide = logits % 16 == 0 && stride % 4 == 0;
+  a.per = (int32_t)per;
+  for (int64_t r = 0; r < rows; r += most) {
+    const int64_t n = std::min<int64_t>(rows - r, most);
+    a.x = (const float*)logits + r * stride;
+    a.settings = (const ihip_sampling*)settings + r;
+    a.uniform = (const double*)uniform + r;
+    a.ids = (int*)ids + r;
+    a.probs = probs ? (float*)probs + r : nullptr;
+    a.rows = (int32_t)n;
+    int rc = launch(c, per == 2048 ? "sample_rows_part_2048" : "sample_rows_part_8192", dim3((unsigned)parts, (unsigned)n),
+                    dim3(256), &a);
+    if (!rc) rc = launch(c, "sample_rows_pick", dim3((unsigned)n), dim3(1024), &a);
+    if (rc) return rc;
+  }
+  return 0;
+}
+
 int ihip_enqueue_logprobs(ihip_ctx* c, uint64_t logits, int64_t rows, int64_t vocab, int64_t stride,
                           uint64_t ids, uint64_t logprobs, uint64_t entropy, int64_t k,
                           uint64_t top_ids, uint64_t top_logprobs)

@@ -220,6 +220,7 @@ int ihip_create(int device, ihip_ctx** out)
   for (auto [to, bytes, counters] : {std::tuple(&c->paged_plan, PAGED_PLAN_BYTES, (int64_t)128),
                                      std::tuple(&c->paged_part, PAGED_PART_BYTES, PAGED_BLOCKS * 128),
                                      std::tuple(&c->paged_shared, SHARED_BYTES, (int64_t)128),
+                                     std::tuple(&c->sample_rows, SAMPLE_ROWS_BYTES, (int64_t)128),
                                      std::tuple(&c->logprobs_part, LOGPROBS_PART_BYTES, LOGPROBS_BLOCKS * 32)}) {
     void* q = nullptr;
     if (hipMalloc(&q, bytes + counters) != hipSuccess) {
@@ -254,7 +255,7 @@ void ihip_destroy(ihip_ctx* c)
   for (auto a : c->allocations) (void)hipFree((void*)a);
   for (uint64_t b : {c->scratch_x, c->scratch_y, c->scratch_q, c->scratch_bad, c->scratch_attn,
                      c->scratch_argmax, c->scratch_split, c->scratch_planes, c->paged_plan, c->paged_part,
-                     c->paged_shared, c->logprobs_part})
+                     c->paged_shared, c->sample_rows, c->logprobs_part})
     if (b) (void)hipFree((void*)b);
   for (auto ev : c->events)
     if (ev) (void)hipEventDestroy(ev);

@@ -185,6 +185,7 @@ def lib():
             "ihip_enqueue_paged_attention_shared": (i32, [vp, u64, i64, C.POINTER(Pages), u64, i64, u64, u64,
                                                           i64, u64, u64, i64, u64, i64, i64, i64, u64,
                                                           C.c_double]),
+            "ihip_enqueue_sample_rows": (i32, [vp, u64, i64, i64, i64, u64, u64, u64, u64]),
             "ihip_enqueue_paged_read": (i32, [vp, C.POINTER(Pages), u64, i64, u64, u64, i64, i64, i32, u64,
                                               u64]),
             "ihip_enqueue_paged_attention": (i32, [vp, u64, i64, C.POINTER(Pages), u64, i64, u64,
