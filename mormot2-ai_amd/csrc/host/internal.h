@@ -12,6 +12,7 @@
 
 #include "../../../include/mormot_ai_hip.h"
 #include "../layout.h"
+#include "../sample_rows.h"
 
 namespace ihip {
 
@@ -170,8 +171,10 @@ constexpr uint64_t SHARED_BYTES = SHARED_PIECE_BYTES + SHARED_HEADS * 4 + (4 + 3
 // doubles and IHIP_LOGPROBS_TOP alternatives each), and a counter of 32 bytes a row
 constexpr int64_t LOGPROBS_BLOCKS = 1024;
 constexpr uint64_t LOGPROBS_PART_BYTES = LOGPROBS_BLOCKS * (3 + IHIP_LOGPROBS_TOP) * 8;
-// sample_rows: the parts' and chunks' results of as many rows as one launch takes
+// sample_rows: the parts' and chunks' results of as many rows as one launch takes, behind
+// the bins of some, and the list of those
 constexpr uint64_t SAMPLE_ROWS_BYTES = 24u << 20;
+constexpr int64_t SAMPLE_ROWS_COUNTERS = (1 + SAMPLE_HEAVY) * 4;
 constexpr uint64_t PAGED_PLAN_BYTES = (5 * IHIP_PAGED_SEQS + 8) * 4;
 
 struct LinearCall {

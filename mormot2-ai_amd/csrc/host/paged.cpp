@@ -9,6 +9,7 @@
 #include <string>
 
 #include "internal.h"
+#include "../sample_rows.h"
 
 using namespace ihip;
 
@@ -382,11 +383,12 @@ int ihip_enqueue_sample_rows(ihip_ctx* c, uint64_t logits, int64_t rows, int64_t
   if ((settings | uniform) % 8) return refuse(who, "settings and random numbers are doubles, aligned to 8 bytes");
   if (!c) return no_context(who);
   OnDevice on(c);
-  // parts of 8192 tokens, of 2048 where they would leave the chip's CUs empty
-  const int64_t per = rows * ((vocab + 8191) / 8192) < 2 * c->cus ? 2048 : 8192;
+  // parts of 8192 tokens, of 4096 or 2048 where they would leave the chip's CUs empty
+  const int64_t most_parts = rows * ((vocab + 8191) / 8192);
+  const int64_t per = most_parts < 2 * c->cus ? 2048 : most_parts < 8 * c->cus ? 4096 : 8192;
   const int64_t parts = (vocab + per - 1) / per, chunks = (vocab + 255) / 256;
-  // a row's results: a double, two words and 32 octaves a part, a word a chunk
-  const int64_t bytes = parts * (8 + 8 + 32 * 4) + chunks * 4;
+  // a row's results: a double, two words and 32 octaves a part, a word a chunk, its sums
+  const int64_t bytes = parts * (8 + 8 + 32 * 4) + chunks * 4 + 24;
   const int64_t most = std::min<int64_t>({rows, 65535, (int64_t)(SAMPLE_ROWS_BYTES / bytes)});
   struct {
     const float* x;
@@ -400,10 +402,17 @@ int ihip_enqueue_sample_rows(ihip_ctx* c, uint64_t logits, int64_t rows, int64_t
     double* sum;
     uint32_t* octaves;
     float* chunk;
+    uint64_t row;
+    int* heavy;
+    uint64_t bins, found;
     int32_t rows, vocab, parts, chunks, wide, per;
   } a = {};
   a.stride = stride;
-  a.sum = (double*)c->sample_rows;
+  a.bins = c->sample_rows;
+  a.found = a.bins + SAMPLE_HEAVY * SAMPLE_BINS * 8;
+  a.row = a.bins + SAMPLE_HEAVY_BYTES;
+  a.sum = (double*)(a.row + 24 * most);
+  a.heavy = (int*)(c->sample_rows + SAMPLE_HEAVY_BYTES + SAMPLE_ROWS_BYTES);
   a.best = (float*)(a.sum + most * parts);
   a.best_id = (int*)(a.best + most * parts);
   a.octaves = (uint32_t*)(a.best_id + most * parts);
@@ -421,9 +430,12 @@ int ihip_enqueue_sample_rows(ihip_ctx* c, uint64_t logits, int64_t rows, int64_t
     a.ids = (int*)ids + r;
     a.probs = probs ? (float*)probs + r : nullptr;
     a.rows = (int32_t)n;
-    int rc = launch(c, per == 2048 ? "sample_rows_part_2048" : "sample_rows_part_8192", dim3((unsigned)parts, (unsigned)n),
+    int rc = launch(c, per == 2048 ? "sample_rows_part_2048" : per == 4096 ? "sample_rows_part_4096" : "sample_rows_part_8192", dim3((unsigned)parts, (unsigned)n),
                     dim3(256), &a);
-    if (!rc) rc = launch(c, "sample_rows_pick", dim3((unsigned)n), dim3(1024), &a);
+    if (!rc) rc = launch(c, "sample_rows_finish", dim3((unsigned)n), dim3(256), &a);
+    for (const char* heavy : {"sample_rows_bins", "sample_rows_find"})
+      if (!rc) rc = launch(c, heavy, dim3((unsigned)c->cus), dim3(256), &a);
+    if (!rc) rc = launch(c, a.wide ? "sample_rows_pick_wide" : "sample_rows_pick", dim3((unsigned)n), dim3(512), &a);
     if (rc) return rc;
   }
   return 0;

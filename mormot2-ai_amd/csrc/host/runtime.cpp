@@ -220,7 +220,7 @@ int ihip_create(int device, ihip_ctx** out)
   for (auto [to, bytes, counters] : {std::tuple(&c->paged_plan, PAGED_PLAN_BYTES, (int64_t)128),
                                      std::tuple(&c->paged_part, PAGED_PART_BYTES, PAGED_BLOCKS * 128),
                                      std::tuple(&c->paged_shared, SHARED_BYTES, (int64_t)128),
-                                     std::tuple(&c->sample_rows, SAMPLE_ROWS_BYTES, (int64_t)128),
+                                     std::tuple(&c->sample_rows, SAMPLE_HEAVY_BYTES + SAMPLE_ROWS_BYTES, SAMPLE_ROWS_COUNTERS),
                                      std::tuple(&c->logprobs_part, LOGPROBS_PART_BYTES, LOGPROBS_BLOCKS * 32)}) {
     void* q = nullptr;
     if (hipMalloc(&q, bytes + counters) != hipSuccess) {
