@@ -142,7 +142,8 @@ int paged_attention(const char* who, ihip_ctx* c, uint64_t q, int64_t q_stride, 
   const int64_t group = heads / kvh, tiles = (group + 15) / 16;
   const int64_t tk = (cache->dtype == IHIP_F32 ? 64 : 128) / (hd > 256 ? 2 : 1);
   const int64_t keys = window > 0 ? std::min(window, max_pages * cache->page_size) : max_pages * cache->page_size;
-  const int64_t units = (keys + tk - 1) / tk * kvh * tiles;
+  // (8-bit pages' and the groups' kernels count three more an item)
+  const int64_t units = ((keys + tk - 1) / tk + (cache->dtype == IHIP_Q8_HEAD || groups ? 3 : 0)) * kvh * tiles;
   if (units > INT32_MAX / seqs) return refuse(who, "more than 2^31 tiles of keys", IHIP_E_NOMEM);
   if (!c) return no_context(who);
   OnDevice on(c);

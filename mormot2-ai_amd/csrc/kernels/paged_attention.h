@@ -521,8 +521,14 @@ __device__ __forceinline__ void paged_attention_t(const A& a)
     }
   };
   __shared__ typename std::conditional<is_shared<A>, AttnPrefix, int>::type px;
+  // What an item (a sequence's KV head) costs beside its tiles of keys, in tiles: its query,
+  // the waves' meeting, the prefix. The blocks share out tiles and these, so that one
+  // with many short items has as much to do (three prompts' 480 items of 1 to 8 tiles, on
+  // one block a CU: 140 us without, the others through at 50).
+  constexpr uint32_t OV = T == 3 || is_shared<A> ? 3 : 0;
   // all tiles (each wave for itself); rows without a key are zeros
   uint32_t all = 0, n0 = 0, live = 0;  // tiles, those of the lane's first sequence; sequences with any
+  uint32_t longest = 0;
   int64_t lo0 = 0, hi0 = 0;  // of the first 64 sequences, a lane each
   for (int s0 = 0; s0 < a.seqs; s0 += 64) {
     const int seq = s0 + lane;
@@ -534,7 +540,8 @@ __device__ __forceinline__ void paged_attention_t(const A& a)
       if (s0 == 0) n0 = n, lo0 = lo, hi0 = hi;
       zero = n == 0 && a.lengths[seq] >= 0 && row_of(seq) >= 0 && (uint32_t)seq % grid == b;
     }
-    all += n * per;
+    if (n) all += (n + OV) * per;
+    if (OV) longest = max(longest, n);
     live += __popcll(__ballot(n != 0));
     for (uint64_t z = __ballot(zero); z; z &= z - 1) {
       float* const y = a.y + (int64_t)row_of(s0 + __builtin_ctzll(z)) * row_out;
@@ -568,20 +575,29 @@ __device__ __forceinline__ void paged_attention_t(const A& a)
   // other's latencies: 64 sequences of 8192, 8 KV heads of 64, two blocks a CU 222 us,
   // one 196; 16384 of 128 731, 718; of 200 sequences up to 4000, 16 tiles an item, the
   // starts and ends of pieces need the second block: 301, one 313), else all.
-  const uint32_t B = all >= 32 * grid && all / 24 >= live * per ? min(grid, (uint32_t)a.cus) : min(grid, all);
+  // Many items of few tiles go to a block each and whole, in turn: what a block with two
+  // parts of them spends is their starts and ends, not their tiles.
+  const bool whole = OV && live * per * 4 >= grid && wave_max((int)longest) <= 8;
+  const uint32_t B = whole ? min(grid, live * per) : T != 3 && all >= 32 * grid && all / 24 >= live * per ? min(grid, (uint32_t)a.cus) : min(grid, all);
   if (b >= B) return;
   const uint32_t quot = all / B, rem = all % B;
   auto first = [&](uint32_t i) { return i * quot + i * rem / B; };
   uint32_t u = first(b);
-  const uint32_t end = first(b + 1);
-  // the sequence of tile u
+  uint32_t end = first(b + 1);
+  for (uint32_t turn = b;; turn += B) {
+  if (OV && whole) {
+    if (turn >= live * per) return;
+    u = turn;
+  }
+  // the sequence of tile u (or of item u of those that are whole)
   int seq = 0;
   uint32_t before = 0, n = 0;  // tiles before the sequence, tiles of a KV head's item
   int64_t lo = 0, hi = 0;
   for (int s0 = 0;; s0 += 64) {
     uint32_t m = s0 == 0 ? n0 : 0;
-    if (s0 > 0 && s0 + lane < a.seqs) m = tiles_of(s0 + lane, lo0, hi0);
+    if ((s0 > 0 || (OV && whole && turn != b && a.seqs > 64)) && s0 + lane < a.seqs) m = tiles_of(s0 + lane, lo0, hi0);
     const uint32_t items = m;
+    if (OV && m) m = whole ? 1 : m + OV;
     m *= per;
     uint32_t upto = m;
 #pragma unroll
@@ -602,9 +618,18 @@ __device__ __forceinline__ void paged_attention_t(const A& a)
     before += __builtin_amdgcn_readlane(upto, 63);
   }
 
+  if (OV && whole) {
+    u = (u - before) * (n + OV);
+    end = u + n + OV;
+    before = 0;
+  }
+
   for (;;) {
-    const uint32_t item = (u - before) / n, tile0 = (u - before) - item * n;
-    const uint32_t tile1 = min(n, tile0 + (end - u));
+    // (of an item the first OV are nothing but its cost; its tiles lie behind them)
+    const uint32_t item = (u - before) / (n + OV), at = (u - before) - item * (n + OV);
+    const uint32_t tile0 = at > OV ? at - OV : 0, upto = min(n + OV, at + (end - u));
+    const uint32_t tile1 = upto > OV ? upto - OV : 0;
+    if (OV && tile1 == tile0) return;  // (the block's range ends before the item's first tile)
     AttnItem it;
     it.s = seq;
     it.row = row_of(seq);
@@ -942,7 +967,7 @@ __device__ __forceinline__ void paged_attention_t(const A& a)
         while (first(k + 1) <= i) k++;
         return k;
       };
-      const uint32_t u0 = before + item * n, b0 = block_of(u0), np = block_of(u0 + n - 1) - b0 + 1;
+      const uint32_t u0 = before + item * (n + OV) + OV, b0 = block_of(u0), np = block_of(u0 + n - 1) - b0 + 1;
       auto piece = [&](uint32_t i) { return a.part + (int64_t)(2 * (b0 + i) + (i == 0)) * ps; };
       // pieces i0, i0 + step, .. (cnt of them, at most 64) joined in that order: into
       // the output, or into the first of them
@@ -1041,13 +1066,17 @@ __device__ __forceinline__ void paged_attention_t(const A& a)
       }
       __syncthreads();
     }
-    u += tile1 - tile0;
-    if (u >= end) return;
+    u += upto - at;
+    if (u >= end) {
+      if (OV && whole) break;
+      return;
+    }
     if (tile1 == n && item + 1 == per) {  // the next sequence with a key
       before = u;
       do n = tiles_of(++seq, lo, hi);
       while (n == 0);
     }
+  }
   }
 }
 

@@ -5,7 +5,7 @@
 using namespace ihip;
 
 #define PAGED_ATTENTION_Q8(D)                                                                         \
-  extern "C" __global__ __launch_bounds__(256) void paged_attention_q8_##D(PagedAttn8Args a)          \
+  extern "C" __global__ __launch_bounds__(256, D <= 256 ? 2 : 1) void paged_attention_q8_##D(PagedAttn8Args a)          \
   {                                                                                                   \
     paged_attention_t<3, D, true>(a);                                                                 \
   }                                                                                                   \

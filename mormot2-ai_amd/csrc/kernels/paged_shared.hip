@@ -584,7 +584,7 @@ __device__ __forceinline__ void paged_prefix_t(const PagedSharedArgs& a)
   {                                                                                                               \
     paged_prefix_t<T, D, FULL>(a);                                                                                \
   }                                                                                                               \
-  extern "C" __global__ __launch_bounds__(256) void paged_own_##NAME##_##D##SUFFIX(PagedSharedArgs a)             \
+  extern "C" __global__ __launch_bounds__(256, D <= 256 ? 2 : 1) void paged_own_##NAME##_##D##SUFFIX(PagedSharedArgs a)             \
   {                                                                                                               \
     paged_attention_t<T, D, FULL>(a);                                                                             \
   }
