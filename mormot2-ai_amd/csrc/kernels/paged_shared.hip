@@ -6,19 +6,24 @@
 
 using namespace ihip;
 
-// columns (a member's query head each) of a block: 16 CT
+// columns (a member's query head each) of a block: 16 CT, as many as leave two blocks a CU
+// their registers (heads of 128: 32 chats behind 4096 tokens 26 us with two, 33 with four
+// and one block a CU, 53 with four that spill; of 256: three prompts of 9001 tokens 84 us
+// with one, 95 with two; of 64: 128 sequences behind 30011 240 us with four, 245 with
+// two and three blocks a CU, 310 with two and four)
 template <int D>
-constexpr int shared_ct = D <= 128 ? 4 : D == 256 ? 2 : 1;
+constexpr int shared_ct = D <= 64 ? 4 : D <= 128 ? 2 : 1;
 
 template <int T, int D>
 struct PrefixLds : AttnScales<T> {
   using S = AttnShape<T, D>;
   static constexpr int CT = shared_ct<D>;
-  uintx4 q[CT][S::NP * S::DS * S::NF * 64];  // the query tiles as the matrix cores take them
-  float o[16 * S::OS];
-  float m[16], l[16];
-  float wm[4][16], wl[4][16];
-  float qs[CT * 16];
+  union {
+    uintx4 q[CT][S::NP * S::DS * S::NF * 64];  // the query tiles as the matrix cores take them
+    float o[S::KG][16 * S::OS];                // behind the keys: 16 columns' sums, of the waves of each group of keys
+  };
+  float wm[4][CT * 16], wl[4][CT * 16];
+  uint32_t top[CT * 16];  // a column's largest magnitude, as bits
   int64_t at[CT * 16];  // a column's query and output, from q and y (rows of q_stride and heads * hd): row, -1 none
   int head[CT * 16];
   int keys[CT * 16];    // of a column: the prefix's tokens that its sequence has
@@ -78,25 +83,27 @@ __device__ __forceinline__ void prefix_walk(const PagedSharedArgs& a, const int*
 #pragma unroll
     for (int i = 0; i < NV; i++) tmp[w * D + lane + 64 * i] = acc[i];
     if (lane == 0) {
-      s.wm[w][0] = m;
-      s.wl[w][0] = l;
+      s.wm[w][col] = m;
+      s.wl[w][col] = l;
     }
     __syncthreads();
     float M = -__builtin_inff(), L = 0.f, f[4];
-    for (int i = 0; i < 4; i++) M = s.wm[i][0] > M || s.wm[i][0] != s.wm[i][0] ? s.wm[i][0] : M;
+    for (int i = 0; i < 4; i++) M = s.wm[i][col] > M || s.wm[i][col] != s.wm[i][col] ? s.wm[i][col] : M;
     for (int i = 0; i < 4; i++) {
-      f[i] = s.wl[i][0] == 0.f ? 0.f : exp2_fast(s.wm[i][0] - M);
-      L += f[i] * s.wl[i][0];
+      f[i] = s.wl[i][col] == 0.f ? 0.f : exp2_fast(s.wm[i][col] - M);
+      L += f[i] * s.wl[i][col];
     }
     for (int d = t; d < a.hd; d += 256) {
       float v = 0.f;
       for (int i = 0; i < 4; i++)
-        if (s.wl[i][0] != 0.f) v += f[i] * tmp[i * D + d];
-      s.o[h * S::OS + d] = v;
+        if (s.wl[i][col] != 0.f) v += f[i] * tmp[i * D + d];
+      s.o[0][h * S::OS + d] = v;
     }
-    if (t == 0) {
-      s.m[h] = M;
-      s.l[h] = L;
+    __syncthreads();
+    // (as if one group of keys had them all)
+    if (t < S::KG) {
+      s.wm[t][col] = t == 0 ? M : -__builtin_inff();
+      s.wl[t][col] = t == 0 ? L : 0.f;
     }
     __syncthreads();
   }
@@ -229,41 +236,44 @@ __device__ __forceinline__ void paged_prefix_t(const PagedSharedArgs& a)
       s.at[t] = at;
       s.head[t] = kv * a.group + col % a.group;
       s.keys[t] = keys;
+      s.top[t] = 0;
     }
     __syncthreads();
-    // the query tiles (stage_query's form)
+    // the query tiles (stage_query's form), a thread's factors on their way at once
+    constexpr int TILE = S::DS * S::NF * 64, R = CT * TILE / 256;
+    float qv[R][S::FL];
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+      const int i = t + 256 * r, col = 16 * (i / TILE) + (i & 15), d0 = S::factor((i % TILE) >> 6, (i >> 4) & 3);
+      const bool in = s.at[col] >= 0 && d0 < a.hd;
+      const float* const q = a.q + (in ? s.at[col] * a.q_stride + (int64_t)s.head[col] * a.hd + d0 : 0);
+#pragma unroll
+      for (int e = 0; e < S::FL; e++) qv[r][e] = in ? q[e] : 0.f;
+    }
     if constexpr (T == 1 || T == 3) {
-      for (int ct = 0; ct < CT; ct++) {
-        const int col = 16 * ct + (t >> 4);
-        float top = 0.f;
-        if (s.at[col] >= 0) {
-          const float* const q = a.q + s.at[col] * a.q_stride + (int64_t)s.head[col] * a.hd;
-          for (int d = t & 15; d < a.hd; d += 16) top = fmaxf(top, fabsf(q[d] * a.scale));
-        }
-        top = fmaxf(top, xpart<1>(top));
-        top = fmaxf(top, xpart<2>(top));
-        top = fmaxf(top, xpart<4>(top));
-        top = fmaxf(top, xpart<8>(top));
-        if ((t & 15) == 0) {
-          int e = (int)(float_bits(top) >> 23) - 126;  // top < 2^e
-          if (top == 0.f || !finite(top)) e = 14;
-          s.qs[col] = ldexpf(1.f, max(e - 14, -120));
-        }
+#pragma unroll
+      for (int r = 0; r < R; r++) {
+        const int i = t + 256 * r, col = 16 * (i / TILE) + (i & 15);
+        uint32_t top = 0;
+#pragma unroll
+        for (int e = 0; e < S::FL; e++) top = max(top, float_bits(fabsf(qv[r][e] * a.scale)));
+        atomicMax(&s.top[col], top);
       }
       __syncthreads();
     }
-    for (int i = t; i < CT * S::DS * S::NF * 64; i += 256) {
-      const int ct = i / (S::DS * S::NF * 64), j = i % (S::DS * S::NF * 64);
-      const int col = 16 * ct + (j & 15), d0 = S::factor(j >> 6, (j >> 4) & 3);
-      const bool in = s.at[col] >= 0 && d0 < a.hd;
-      const float* const q = a.q + (in ? s.at[col] * a.q_stride + (int64_t)s.head[col] * a.hd + d0 : 0);
-      float f = a.scale, v[S::FL];
-      if constexpr (T == 1 || T == 3) f = 1.f / s.qs[col];
+    // the power of two that a column's queries are divided by: the largest below 2^14
+    auto divisor = [&](int col) {
+      const uint32_t top = s.top[col];
+      const int e = top == 0 || top >= 0x7f800000u ? 14 : (int)(top >> 23) - 126;
+      return ldexpf(1.f, max(e - 14, -120));
+    };
 #pragma unroll
-      for (int e = 0; e < S::FL; e++) {
-        v[e] = in ? q[e] : 0.f;
-        v[e] = T == 1 || T == 3 ? v[e] * a.scale * f : v[e] * f;
-      }
+    for (int r = 0; r < R; r++) {
+      const int i = t + 256 * r, ct = i / TILE, j = i % TILE;
+      float f = a.scale, v[S::FL];
+      if constexpr (T == 1 || T == 3) f = 1.f / divisor(16 * ct + (i & 15));
+#pragma unroll
+      for (int e = 0; e < S::FL; e++) v[e] = T == 1 || T == 3 ? qv[r][e] * a.scale * f : qv[r][e] * f;
       if constexpr (T == 0) {
         s.q[ct][j] = uintx4{float_bits(v[0]), float_bits(v[1]), float_bits(v[2]), float_bits(v[3])};
       } else {
@@ -271,7 +281,7 @@ __device__ __forceinline__ void paged_prefix_t(const PagedSharedArgs& a)
 #pragma unroll
         for (int e = 0; e < 4; e++) split2<T>(v[2 * e], v[2 * e + 1], part[e]);
 #pragma unroll
-        for (int p = 0; p < S::NP; p++) s.q[ct][p * S::DS * S::NF * 64 + j] = uintx4{part[0][p], part[1][p], part[2][p], part[3][p]};
+        for (int p = 0; p < S::NP; p++) s.q[ct][p * TILE + j] = uintx4{part[0][p], part[1][p], part[2][p], part[3][p]};
       }
     }
     __syncthreads();
@@ -279,7 +289,7 @@ __device__ __forceinline__ void paged_prefix_t(const PagedSharedArgs& a)
     int keys[CT], least = INT32_MAX;  // of the lane's columns; the least of all
 #pragma unroll
     for (int ct = 0; ct < CT; ct++) {
-      sscale[ct] = T == 1 || T == 3 ? s.qs[16 * ct + c] : 1.f;
+      sscale[ct] = T == 1 || T == 3 ? divisor(16 * ct + c) : 1.f;
       keys[ct] = s.keys[16 * ct + c];
       if (s.at[16 * ct + c] >= 0) least = min(least, keys[ct]);
     }
@@ -442,22 +452,35 @@ __device__ __forceinline__ void paged_prefix_t(const PagedSharedArgs& a)
               }
             }
       }
+      // the scores' scale, what a column does not see, and whether a maximum rises
+      float top[CT];
+      bool rises = false;
 #pragma unroll
       for (int ct = 0; ct < CT; ct++) {
-        float top = -__builtin_inff(), y[NV];
+        top[ct] = -__builtin_inff();
 #pragma unroll
-        for (int k = 0; k < NV; k++) y[k] = x[ct][k >> 2][k & 3] * (T == 3 ? sscale[ct] * ksc[T == 3 ? k >> 2 : 0][k & 3] : sscale[ct]);
-        if (!plain)
+        for (int k = 0; k < NV; k++)
+          x[ct][k >> 2][k & 3] *= T == 3 ? sscale[ct] * ksc[T == 3 ? k >> 2 : 0][k & 3] : sscale[ct];
+      }
+      if (!plain) {
+#pragma unroll
+        for (int ct = 0; ct < CT; ct++)
 #pragma unroll
           for (int k = 0; k < NV; k++) {
             const bool in = (now >> (16 * (k >> 2) + 4 * g + (k & 3)) & 1) && key0 + 16 * (k >> 2) + (k & 3) < keys[ct];
-            y[k] = in ? y[k] : -__builtin_inff();
+            x[ct][k >> 2][k & 3] = in ? x[ct][k >> 2][k & 3] : -__builtin_inff();
           }
+      }
 #pragma unroll
-        for (int k = 0; k < NV; k++) top = fmaxf(top, y[k]);
-        if (__any(top > m[ct])) {
-          top = quad_max(top);
-          const float m2 = fmaxf(top, m[ct]), f = m[ct] == -__builtin_inff() ? 0.f : exp2_fast(m[ct] - m2);
+      for (int ct = 0; ct < CT; ct++) {
+#pragma unroll
+        for (int k = 0; k < NV; k++) top[ct] = fmaxf(top[ct], x[ct][k >> 2][k & 3]);
+        rises |= top[ct] > m[ct];
+      }
+      if (__any(rises)) {
+#pragma unroll
+        for (int ct = 0; ct < CT; ct++) {
+          const float m2 = fmaxf(quad_max(top[ct]), m[ct]), f = m[ct] == -__builtin_inff() ? 0.f : exp2_fast(m[ct] - m2);
           m[ct] = m2;
           l[ct] *= f;
 #pragma unroll
@@ -465,11 +488,16 @@ __device__ __forceinline__ void paged_prefix_t(const PagedSharedArgs& a)
 #pragma unroll
             for (int e = 0; e < S::VL; e++) o[ct][j][e] *= f;
         }
+      }
+      // Weights and value products, without a branch: a tile's products run while the next
+      // one's weights are formed.
+#pragma unroll
+      for (int ct = 0; ct < CT; ct++) {
         const float shift = m[ct] == -__builtin_inff() ? 0.f : m[ct];
         float p[NV];
 #pragma unroll
         for (int k = 0; k < NV; k++) {
-          p[k] = exp2_fast(y[k] - shift);
+          p[k] = exp2_fast(x[ct][k >> 2][k & 3] - shift);
           l[ct] += p[k];
         }
         if constexpr (T == 0) {
@@ -490,17 +518,18 @@ __device__ __forceinline__ void paged_prefix_t(const PagedSharedArgs& a)
               split2<T>(p[2 * k] * S::PS, p[2 * k + 1] * S::PS, part[k]);
           }
 #pragma unroll
-          for (int j = 0; j < S::NJ; j++)
+          for (int n2 = 0; n2 < S::NP; n2++)
 #pragma unroll
-            for (int e = 0; e < S::VL; e++)
+            for (int j = 0; j < S::NJ; j++)
 #pragma unroll
-              for (int n2 = 0; n2 < S::NP; n2++)
+              for (int e = 0; e < S::VL; e++)
                 o[ct][j][e] = mfma16<T>(vt[j][e], uintx4{part[0][n2], part[1][n2], part[2][n2], part[3][n2]}, o[ct][j][e]);
         }
       }
     }
 
-    // the waves' sums meet, 16 columns at a time
+    // the waves' sums meet, 16 columns at a time: each group of keys' into LDS, where the
+    // query was, then added up by all threads, 4 values of a column each time
     products_done();
     const bool whole = tile0 == 0 && tile1 == n;
     float* const pc = a.pieces + (int64_t)(2 * b + (tile0 ? 0 : 1)) * COLS * (a.hd + 2);
@@ -508,65 +537,102 @@ __device__ __forceinline__ void paged_prefix_t(const PagedSharedArgs& a)
     for (int ct = 0; ct < CT; ct++) {
       l[ct] = quad_sum(l[ct]);
       if (g == 0 && dh == 0) {
-        s.wm[kg][c] = m[ct];
-        s.wl[kg][c] = l[ct];
+        s.wm[kg][16 * ct + c] = m[ct];
+        s.wl[kg][16 * ct + c] = l[ct];
       }
-      __syncthreads();
-      float M = s.wm[0][c];
-#pragma unroll
-      for (int i = 1; i < S::KG; i++) M = fmaxf(M, s.wm[i][c]);
-      const float Ms = M == -__builtin_inff() ? 0.f : M;
-      const float f = exp2_fast(m[ct] - Ms) * (1.f / S::PS) * (T == 3 ? vtop : 1.f);
-      bool odd = false;
-      if (w == 0 && g == 0) {
-        float L = 0.f;
-#pragma unroll
-        for (int i = 0; i < S::KG; i++) L += s.wl[i][c] * exp2_fast(s.wm[i][c] - Ms);
-        s.m[c] = M;
-        s.l[c] = L;
-        odd = s.at[16 * ct + c] >= 0 && !finite(L);
-      }
-      for (int r4 = 0; r4 < S::KG; r4++) {
-        if (kg == r4) {
-#pragma unroll
-          for (int j = 0; j < S::NJ; j++)
-#pragma unroll
-            for (int r = 0; r < 4; r++)
-#pragma unroll
-              for (int e = 0; e < S::VL; e += 4) {
-                floatx4* const d = (floatx4*)&s.o[c * S::OS + dh * S::DW + j * 16 * S::VL + S::VL * (4 * g + r) + e];
-                floatx4 v = {o[ct][j][e][r] * f, o[ct][j][e + 1][r] * f, o[ct][j][e + 2][r] * f, o[ct][j][e + 3][r] * f};
-                if (r4) v += *d;
-                *d = v;
-              }
-        }
-        __syncthreads();
-      }
-      for (int h = w; h < 16; h += 4)
-        if (s.at[16 * ct + h] >= 0)
-          for (int d = lane; d < hd; d += 64) odd |= !finite(s.o[h * S::OS + d]);
-      if (__syncthreads_or(odd))
-        prefix_walk<T, D>(a, table, kv, ct, (int64_t)tile0 * S::TK, jend, s);
-      for (int h = w; h < 16; h += 4) {
-        const int col = 16 * ct + h;
-        if (s.at[col] < 0) continue;
-        const float M2 = s.m[h], L2 = s.l[h];
-        if (whole) {
-          const float inv = L2 != 0.f ? 1.f / L2 : 0.f;
-          float* const y = a.y + s.at[col] * row_out + (int64_t)s.head[col] * a.hd;
-          for (int d = lane; d < hd; d += 64) y[d] = L2 == 0.f ? 0.f : s.o[h * S::OS + d] * inv;
-          if (lane == 0)
-            a.lse[(int64_t)(m0 + (col0 + col) / a.group) * a.heads + s.head[col]] = L2 == 0.f ? -__builtin_inff() : M2 + __builtin_amdgcn_logf(L2);
-        } else {
-          for (int d = lane; d < hd; d += 64) pc[col * a.hd + d] = s.o[h * S::OS + d];
-          if (lane == 0) {
-            pc[COLS * a.hd + col] = L2 == 0.f ? -__builtin_inff() : M2;
-            pc[COLS * a.hd + COLS + col] = L2;
-          }
-        }
-      }
-      __syncthreads();
     }
+    __syncthreads();
+    constexpr int V4 = D / 64;  // of a thread: 4 values each of the 16 columns'
+    // a column's maximum and sum
+    auto sums = [&](int col, float& M2, float& L2) {
+      M2 = s.wm[0][col];
+      L2 = 0.f;
+#pragma unroll
+      for (int i = 1; i < S::KG; i++) M2 = s.wm[i][col] > M2 || s.wm[i][col] != s.wm[i][col] ? s.wm[i][col] : M2;
+      const float ms = M2 == -__builtin_inff() ? 0.f : M2;
+#pragma unroll
+      for (int i = 0; i < S::KG; i++) L2 += s.wl[i][col] == 0.f ? 0.f : s.wl[i][col] * exp2_fast(s.wm[i][col] - ms);
+    };
+    // 16 columns' results: to y and lse, or to the pieces
+    auto put = [&](int ct, const floatx4 (&v)[V4]) {
+      if (t < 16 && s.at[16 * ct + t] >= 0) {
+        const int col = 16 * ct + t;
+        float M2, L2;
+        sums(col, M2, L2);
+        const float m2 = L2 == 0.f ? -__builtin_inff() : M2;
+        if (whole) {
+          a.lse[(int64_t)(m0 + (col0 + col) / a.group) * a.heads + s.head[col]] = L2 == 0.f ? m2 : M2 + __builtin_amdgcn_logf(L2);
+        } else {
+          pc[COLS * a.hd + col] = m2;
+          pc[COLS * a.hd + COLS + col] = L2;
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < V4; k++) {
+        const int i = 4 * t + 1024 * k, h = i / hd, d = i - h * hd, col = 16 * ct + h;
+        if (i >= 16 * hd || s.at[col] < 0) continue;
+        if (whole) {
+          float M3, L3;
+          sums(col, M3, L3);
+          const float inv = L3 != 0.f ? 1.f / L3 : 0.f;
+          float* const y = a.y + s.at[col] * row_out + (int64_t)s.head[col] * a.hd + d;
+#pragma unroll
+          for (int e = 0; e < 4; e++) y[e] = L3 == 0.f ? 0.f : v[k][e] * inv;
+        } else {
+          *(floatx4*)(pc + col * a.hd + d) = v[k];
+        }
+      }
+    };
+    uint32_t bad = 0;
+#pragma unroll
+    for (int ct = 0; ct < CT; ct++) {
+      float M = s.wm[0][16 * ct + c];
+#pragma unroll
+      for (int i = 1; i < S::KG; i++) M = fmaxf(M, s.wm[i][16 * ct + c]);
+      const float f = exp2_fast(m[ct] - (M == -__builtin_inff() ? 0.f : M)) * (1.f / S::PS) * (T == 3 ? vtop : 1.f);
+#pragma unroll
+      for (int j = 0; j < S::NJ; j++)
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+#pragma unroll
+          for (int e = 0; e < S::VL; e += 4)
+            *(floatx4*)&s.o[kg][c * S::OS + dh * S::DW + j * 16 * S::VL + S::VL * (4 * g + r) + e] =
+                floatx4{o[ct][j][e][r] * f, o[ct][j][e + 1][r] * f, o[ct][j][e + 2][r] * f, o[ct][j][e + 3][r] * f};
+      __syncthreads();
+      floatx4 v[V4];
+      bool odd = false;
+#pragma unroll
+      for (int k = 0; k < V4; k++) {
+        const int i = 4 * t + 1024 * k;
+        v[k] = floatx4{0.f, 0.f, 0.f, 0.f};
+        if (i >= 16 * hd) continue;
+        const int h = i / hd, d = i - h * hd;
+#pragma unroll
+        for (int p = 0; p < S::KG; p++) v[k] += *(const floatx4*)&s.o[p][h * S::OS + d];
+        odd |= s.at[16 * ct + h] >= 0 && !(finite(v[k][0]) && finite(v[k][1]) && finite(v[k][2]) && finite(v[k][3]));
+      }
+      float M2, L2;
+      if (t < 16) {
+        sums(16 * ct + t, M2, L2);
+        odd |= s.at[16 * ct + t] >= 0 && !finite(L2);
+      }
+      bad |= (uint32_t)__syncthreads_or(odd) << ct;
+      put(ct, v);
+    }
+    // (again by the formula's steps, where sums are not all finite)
+    for (; bad; bad &= bad - 1) {
+      const int ct = __builtin_ctz(bad);
+      __syncthreads();
+      prefix_walk<T, D>(a, table, kv, ct, (int64_t)tile0 * S::TK, jend, s);
+      floatx4 v[V4];
+#pragma unroll
+      for (int k = 0; k < V4; k++) {
+        const int i = min(4 * t + 1024 * k, 16 * hd - 4);
+        v[k] = *(const floatx4*)&s.o[0][i / hd * S::OS + i % hd];
+      }
+      put(ct, v);
+    }
+    __syncthreads();
     u += tile1 - tile0;
     if (u >= end) return;
     if (tile1 == n && item + 1 == items * a.kvh) {  // the next group with a prefix
@@ -580,7 +646,7 @@ __device__ __forceinline__ void paged_prefix_t(const PagedSharedArgs& a)
 }
 
 #define PAGED_SHARED2(NAME, T, D, SUFFIX, FULL)                                                                   \
-  extern "C" __global__ __launch_bounds__(256) void paged_prefix_##NAME##_##D##SUFFIX(PagedSharedArgs a)          \
+  extern "C" __global__ __launch_bounds__(256, D <= 256 ? 2 : 1) void paged_prefix_##NAME##_##D##SUFFIX(PagedSharedArgs a)          \
   {                                                                                                               \
     paged_prefix_t<T, D, FULL>(a);                                                                                \
   }                                                                                                               \
