@@ -6,18 +6,21 @@
 
 using namespace ihip;
 
-// columns (a member's query head each) of a block: 16 CT, as many as leave two blocks a CU
-// their registers (heads of 128: 32 chats behind 4096 tokens 26 us with two, 33 with four
-// and one block a CU, 53 with four that spill; of 256: three prompts of 9001 tokens 84 us
-// with one, 95 with two; of 64: 128 sequences behind 30011 240 us with four, 245 with
-// two and three blocks a CU, 310 with two and four)
-template <int D>
-constexpr int shared_ct = D <= 64 ? 4 : D <= 128 ? 2 : 1;
+// Columns (a member's query head each) of a block: 16 CT. As many as leave two blocks a CU
+// their registers: heads of 128 two tiles (32 chats behind 4096 tokens 26 us; four tiles
+// and one block a CU 33, four that spill 53), of 64 four (128 sequences behind 30011
+// 240 us; two and three blocks a CU 245, two and four 310), of 256 in 8-bit pages one (three
+// prompts of 9001 80 us; two and one block 95). Others of 256 have two and one block
+// (halves 113 us; one and two that spill 135).
+template <int T, int D>
+constexpr int shared_ct = D <= 64 ? 4 : D <= 128 ? 2 : D == 256 && T != 3 ? 2 : 1;
+template <int T, int D>
+constexpr int shared_blocks = D <= 128 || (D == 256 && T == 3) ? 2 : 1;
 
 template <int T, int D>
 struct PrefixLds : AttnScales<T> {
   using S = AttnShape<T, D>;
-  static constexpr int CT = shared_ct<D>;
+  static constexpr int CT = shared_ct<T, D>;
   union {
     uintx4 q[CT][S::NP * S::DS * S::NF * 64];  // the query tiles as the matrix cores take them
     float o[S::KG][16 * S::OS];                // behind the keys: 16 columns' sums, of the waves of each group of keys
@@ -120,7 +123,7 @@ template <int T, int D, bool FULL>
 __device__ __forceinline__ void paged_prefix_t(const PagedSharedArgs& a)
 {
   using S = AttnShape<T, D>;
-  constexpr int CT = shared_ct<D>, COLS = 16 * CT;
+  constexpr int CT = shared_ct<T, D>, COLS = 16 * CT;
   __shared__ PrefixLds<T, D> s;
   const int t = threadIdx.x, lane = t & 63, c = lane & 15, g = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(t >> 6);
@@ -434,23 +437,29 @@ __device__ __forceinline__ void paged_prefix_t(const PagedSharedArgs& a)
           for (int j = 0; j < S::NJ; j++)
             if (!(now >> (16 * (k >> 2) + 4 * g + (k & 3)) & 1)) vr[k][j] = uintx4{0, 0, 0, 0};
       }
-      // the values turned: 8 keys of a dimension side by side
-      uintx4 vt[T == 0 ? 1 : S::NJ][T == 0 ? 1 : S::VL];
-      if constexpr (T != 0) {
+      // the values turned: 8 keys of a dimension side by side (once for all tiles of columns;
+      // for one, where its products are, as they take as many registers as the values)
+      auto turned = [&](int j, int e) {
+        uintx4 v;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+          if constexpr (T == 3) {
+            const uint32_t pair = __builtin_amdgcn_perm(vr[2 * k + 1][j][e / 4], vr[2 * k][j][e / 4],
+                                                        e & 2 ? 0x07030602u : 0x05010400u) ^ 0x80808080u;
+            v[k] = halves_of(__builtin_amdgcn_perm(0x64646464u, pair, e & 1 ? 0x04030402u : 0x04010400u));
+          } else {
+            v[k] = __builtin_amdgcn_perm(vr[2 * k + 1][j][e / 2], vr[2 * k][j][e / 2], e & 1 ? 0x07060302u : 0x05040100u);
+          }
+        }
+        return v;
+      };
+      constexpr bool ONCE = T != 0 && CT > 1;
+      uintx4 vt[ONCE ? S::NJ : 1][ONCE ? S::VL : 1];
+      if constexpr (ONCE) {
 #pragma unroll
         for (int j = 0; j < S::NJ; j++)
 #pragma unroll
-          for (int e = 0; e < S::VL; e++)
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-              if constexpr (T == 3) {
-                const uint32_t pair = __builtin_amdgcn_perm(vr[2 * k + 1][j][e / 4], vr[2 * k][j][e / 4],
-                                                            e & 2 ? 0x07030602u : 0x05010400u) ^ 0x80808080u;
-                vt[j][e][k] = halves_of(__builtin_amdgcn_perm(0x64646464u, pair, e & 1 ? 0x04030402u : 0x04010400u));
-              } else {
-                vt[j][e][k] = __builtin_amdgcn_perm(vr[2 * k + 1][j][e / 2], vr[2 * k][j][e / 2], e & 1 ? 0x07060302u : 0x05040100u);
-              }
-            }
+          for (int e = 0; e < S::VL; e++) vt[j][e] = turned(j, e);
       }
       // the scores' scale, what a column does not see, and whether a maximum rises
       float top[CT];
@@ -518,12 +527,16 @@ __device__ __forceinline__ void paged_prefix_t(const PagedSharedArgs& a)
               split2<T>(p[2 * k] * S::PS, p[2 * k + 1] * S::PS, part[k]);
           }
 #pragma unroll
-          for (int n2 = 0; n2 < S::NP; n2++)
+          for (int j = 0; j < S::NJ; j++)
 #pragma unroll
-            for (int j = 0; j < S::NJ; j++)
+            for (int e = 0; e < S::VL; e++) {
+              uintx4 v;
+              if constexpr (ONCE) v = vt[ONCE ? j : 0][ONCE ? e : 0];
+              else v = turned(j, e);
 #pragma unroll
-              for (int e = 0; e < S::VL; e++)
-                o[ct][j][e] = mfma16<T>(vt[j][e], uintx4{part[0][n2], part[1][n2], part[2][n2], part[3][n2]}, o[ct][j][e]);
+              for (int n2 = 0; n2 < S::NP; n2++)
+                o[ct][j][e] = mfma16<T>(v, uintx4{part[0][n2], part[1][n2], part[2][n2], part[3][n2]}, o[ct][j][e]);
+            }
         }
       }
     }
@@ -646,11 +659,11 @@ __device__ __forceinline__ void paged_prefix_t(const PagedSharedArgs& a)
 }
 
 #define PAGED_SHARED2(NAME, T, D, SUFFIX, FULL)                                                                   \
-  extern "C" __global__ __launch_bounds__(256, D <= 256 ? 2 : 1) void paged_prefix_##NAME##_##D##SUFFIX(PagedSharedArgs a)          \
+  extern "C" __global__ __launch_bounds__(256, (shared_blocks<T, D>)) void paged_prefix_##NAME##_##D##SUFFIX(PagedSharedArgs a)          \
   {                                                                                                               \
     paged_prefix_t<T, D, FULL>(a);                                                                                \
   }                                                                                                               \
-  extern "C" __global__ __launch_bounds__(256, D <= 256 ? 2 : 1) void paged_own_##NAME##_##D##SUFFIX(PagedSharedArgs a)             \
+  extern "C" __global__ __launch_bounds__(256, (shared_blocks<T, D>)) void paged_own_##NAME##_##D##SUFFIX(PagedSharedArgs a)             \
   {                                                                                                               \
     paged_attention_t<T, D, FULL>(a);                                                                             \
   }
