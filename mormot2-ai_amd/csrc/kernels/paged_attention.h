@@ -122,6 +122,15 @@ __device__ __forceinline__ void products_done()
   __builtin_amdgcn_sched_barrier(0);
 }
 
+// a block's barrier for what it has in LDS: loads and stores of memory stay on their way
+// (__syncthreads waits for them)
+__device__ __forceinline__ void lds_barrier()
+{
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
 __device__ __forceinline__ uint64_t lane_value(uint64_t v, int lane)
 {
   return (uint64_t)__builtin_amdgcn_readlane((uint32_t)(v >> 32), lane) << 32 |
@@ -503,13 +512,23 @@ __device__ __forceinline__ void paged_attention_t(const A& a)
           for (int i = 0; i < 4; i++) p[i] = e[i];
         } else {
           const int np = px.count[h];
-#pragma unroll 4
-          for (int i = 0; i < np; i++) {
-            const float* const e = a.pieces + (2 * (int64_t)(px.first[h] + i) + (i == 0)) * size;
-            const float x = e[pct * a.hd + px.col[h]], w2 = x == -__builtin_inff() ? 0.f : exp2_fast(x - pm);
-            const floatx4 o4 = *(const floatx4*)(e + (int64_t)px.col[h] * a.hd + d);
+          // (4 pieces' loads on their way at once)
+          for (int i0 = 0; i0 < np; i0 += 4) {
+            float x[4];
+            floatx4 o4[4];
 #pragma unroll
-            for (int k = 0; k < 4; k++) p[k] = __builtin_fmaf(w2, w2 != 0.f ? o4[k] : 0.f, p[k]);
+            for (int k = 0; k < 4; k++) {
+              const int i = min(i0 + k, np - 1);
+              const float* const e = a.pieces + (2 * (int64_t)(px.first[h] + i) + (i == 0)) * size;
+              x[k] = e[pct * a.hd + px.col[h]];
+              o4[k] = *(const floatx4*)(e + (int64_t)px.col[h] * a.hd + d);
+            }
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+              const float w2 = i0 + k >= np || x[k] == -__builtin_inff() ? 0.f : exp2_fast(x[k] - pm);
+#pragma unroll
+              for (int j = 0; j < 4; j++) p[j] = __builtin_fmaf(w2, w2 != 0.f ? o4[k][j] : 0.f, p[j]);
+            }
           }
         }
       }

@@ -10,8 +10,8 @@ using namespace ihip;
 // their registers: heads of 128 two tiles (32 chats behind 4096 tokens 26 us; four tiles
 // and one block a CU 33, four that spill 53), of 64 four (128 sequences behind 30011
 // 240 us; two and three blocks a CU 245, two and four 310), of 256 in 8-bit pages one (three
-// prompts of 9001 80 us; two and one block 95). Others of 256 have two and one block
-// (halves 113 us; one and two that spill 135).
+// prompts of 9001 75 us; two and one block 95 where one took 80). Others of 256 have two and
+// one block (halves 97 us; one and two that spill 135 where two took 111).
 template <int T, int D>
 constexpr int shared_ct = D <= 64 ? 4 : D <= 128 ? 2 : D == 256 && T != 3 ? 2 : 1;
 template <int T, int D>
@@ -23,9 +23,11 @@ struct PrefixLds : AttnScales<T> {
   static constexpr int CT = shared_ct<T, D>;
   union {
     uintx4 q[CT][S::NP * S::DS * S::NF * 64];  // the query tiles as the matrix cores take them
-    float o[S::KG][16 * S::OS];                // behind the keys: 16 columns' sums, of the waves of each group of keys
+    float o[CT][S::KG][16 * S::OS];            // behind the keys: a tile's sums, of the waves of each group of keys
   };
   float wm[4][CT * 16], wl[4][CT * 16];
+  int odd;                 // whether sums are not all finite
+  float m[CT * 16], l[CT * 16];  // the columns' maxima and sums
   uint32_t top[CT * 16];  // a column's largest magnitude, as bits
   int64_t at[CT * 16];  // a column's query and output, from q and y (rows of q_stride and heads * hd): row, -1 none
   int head[CT * 16];
@@ -100,7 +102,7 @@ __device__ __forceinline__ void prefix_walk(const PagedSharedArgs& a, const int*
       float v = 0.f;
       for (int i = 0; i < 4; i++)
         if (s.wl[i][col] != 0.f) v += f[i] * tmp[i * D + d];
-      s.o[0][h * S::OS + d] = v;
+      s.o[ct][0][h * S::OS + d] = v;
     }
     __syncthreads();
     // (as if one group of keys had them all)
@@ -224,6 +226,21 @@ __device__ __forceinline__ void paged_prefix_t(const PagedSharedArgs& a)
     const int page0 = entry(tile);
     int page = entry(tile + 1);
 
+    uintx4 kr[S::NT][S::NQ];
+    auto load_keys = [&](uint32_t tile) {
+#pragma unroll
+      for (int i = 0; i < S::NT; i++) {
+        const char* const p = kb + s.off[w][tile & 1][16 * i + c];
+#pragma unroll
+        for (int j = 0; j < S::NQ; j++) {
+          const int d0 = dh * S::DW + j * 4 * S::QL + g * S::QL;
+          const bool in = FULL || d0 < hd;
+          kr[i][j] = *(const uintx4*)(p + (in ? d0 : 0) * S::ES);
+          if (!in) kr[i][j] = uintx4{0, 0, 0, 0};
+        }
+      }
+    };
+
     // the columns: a member's row, its head, the keys that it sees
     if (t < COLS) {
       const int col = col0 + t, seq = m0 + col / a.group;
@@ -241,7 +258,7 @@ __device__ __forceinline__ void paged_prefix_t(const PagedSharedArgs& a)
       s.keys[t] = keys;
       s.top[t] = 0;
     }
-    __syncthreads();
+    lds_barrier();
     // the query tiles (stage_query's form), a thread's factors on their way at once
     constexpr int TILE = S::DS * S::NF * 64, R = CT * TILE / 256;
     float qv[R][S::FL];
@@ -253,6 +270,16 @@ __device__ __forceinline__ void paged_prefix_t(const PagedSharedArgs& a)
 #pragma unroll
       for (int e = 0; e < S::FL; e++) qv[r][e] = in ? q[e] : 0.f;
     }
+    // (the first keys, on their way behind the queries)
+    uint32_t steps = 0;
+    if (S::DS > 1) {
+      steps = tile1 - tile0;
+    } else if (wlo + (int64_t)tile0 * S::TK < common) {
+      const uint32_t mine = (uint32_t)((common - wlo + S::TK - 1) / S::TK);
+      steps = min(tile1, mine) - tile0;
+    }
+    uint32_t there = locate(tile, page0);
+    if (steps) load_keys(tile);
     if constexpr (T == 1 || T == 3) {
 #pragma unroll
       for (int r = 0; r < R; r++) {
@@ -262,7 +289,7 @@ __device__ __forceinline__ void paged_prefix_t(const PagedSharedArgs& a)
         for (int e = 0; e < S::FL; e++) top = max(top, float_bits(fabsf(qv[r][e] * a.scale)));
         atomicMax(&s.top[col], top);
       }
-      __syncthreads();
+      lds_barrier();
     }
     // the power of two that a column's queries are divided by: the largest below 2^14
     auto divisor = [&](int col) {
@@ -287,7 +314,7 @@ __device__ __forceinline__ void paged_prefix_t(const PagedSharedArgs& a)
         for (int p = 0; p < S::NP; p++) s.q[ct][p * TILE + j] = uintx4{part[0][p], part[1][p], part[2][p], part[3][p]};
       }
     }
-    __syncthreads();
+    lds_barrier();
     float sscale[CT];
     int keys[CT], least = INT32_MAX;  // of the lane's columns; the least of all
 #pragma unroll
@@ -297,21 +324,6 @@ __device__ __forceinline__ void paged_prefix_t(const PagedSharedArgs& a)
       if (s.at[16 * ct + c] >= 0) least = min(least, keys[ct]);
     }
     least = -wave_max(-least);
-
-    uintx4 kr[S::NT][S::NQ];
-    auto load_keys = [&](uint32_t tile) {
-#pragma unroll
-      for (int i = 0; i < S::NT; i++) {
-        const char* const p = kb + s.off[w][tile & 1][16 * i + c];
-#pragma unroll
-        for (int j = 0; j < S::NQ; j++) {
-          const int d0 = dh * S::DW + j * 4 * S::QL + g * S::QL;
-          const bool in = FULL || d0 < hd;
-          kr[i][j] = *(const uintx4*)(p + (in ? d0 : 0) * S::ES);
-          if (!in) kr[i][j] = uintx4{0, 0, 0, 0};
-        }
-      }
-    };
 
     floatx4 o[CT][S::NJ][S::VL];
     float m[CT], l[CT];
@@ -325,15 +337,6 @@ __device__ __forceinline__ void paged_prefix_t(const PagedSharedArgs& a)
         for (int j = 0; j < S::VL; j++) o[ct][i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
     }
     float vtop = 0x1p-100f, vinv = 0x1p100f;
-    uint32_t steps = 0;
-    if (S::DS > 1) {
-      steps = tile1 - tile0;
-    } else if (wlo + (int64_t)tile0 * S::TK < common) {
-      const uint32_t mine = (uint32_t)((common - wlo + S::TK - 1) / S::TK);
-      steps = min(tile1, mine) - tile0;
-    }
-    uint32_t there = locate(tile, page0);
-    if (steps) load_keys(tile);
     for (uint32_t i = 0; i < steps; i++, tile++) {
       constexpr int NV = 4 * S::NT;
       uintx4 vr[NV][S::NJ];
@@ -425,7 +428,7 @@ __device__ __forceinline__ void paged_prefix_t(const PagedSharedArgs& a)
         static_assert(S::DS == 1 || CT == 1, "one tile of columns where waves share a head");
 #pragma unroll
         for (int k = 0; k < S::NT; k++) s.x[tile & 1][w][k][lane] = x[0][k];
-        __syncthreads();
+        lds_barrier();
 #pragma unroll
         for (int k = 0; k < S::NT; k++) x[0][k] += s.x[tile & 1][w ^ 1][k][lane];
       }
@@ -541,8 +544,9 @@ __device__ __forceinline__ void paged_prefix_t(const PagedSharedArgs& a)
       }
     }
 
-    // the waves' sums meet, 16 columns at a time: each group of keys' into LDS, where the
-    // query was, then added up by all threads, 4 values of a column each time
+    // the waves' sums meet: each group of keys' into LDS, where the query was, then added
+    // up by all threads, 4 values of a column each time (loops that are not unrolled: the
+    // code runs once a block, and fetching it is what it costs)
     products_done();
     const bool whole = tile0 == 0 && tile1 == n;
     float* const pc = a.pieces + (int64_t)(2 * b + (tile0 ? 0 : 1)) * COLS * (a.hd + 2);
@@ -554,49 +558,7 @@ __device__ __forceinline__ void paged_prefix_t(const PagedSharedArgs& a)
         s.wl[kg][16 * ct + c] = l[ct];
       }
     }
-    __syncthreads();
-    constexpr int V4 = D / 64;  // of a thread: 4 values each of the 16 columns'
-    // a column's maximum and sum
-    auto sums = [&](int col, float& M2, float& L2) {
-      M2 = s.wm[0][col];
-      L2 = 0.f;
-#pragma unroll
-      for (int i = 1; i < S::KG; i++) M2 = s.wm[i][col] > M2 || s.wm[i][col] != s.wm[i][col] ? s.wm[i][col] : M2;
-      const float ms = M2 == -__builtin_inff() ? 0.f : M2;
-#pragma unroll
-      for (int i = 0; i < S::KG; i++) L2 += s.wl[i][col] == 0.f ? 0.f : s.wl[i][col] * exp2_fast(s.wm[i][col] - ms);
-    };
-    // 16 columns' results: to y and lse, or to the pieces
-    auto put = [&](int ct, const floatx4 (&v)[V4]) {
-      if (t < 16 && s.at[16 * ct + t] >= 0) {
-        const int col = 16 * ct + t;
-        float M2, L2;
-        sums(col, M2, L2);
-        const float m2 = L2 == 0.f ? -__builtin_inff() : M2;
-        if (whole) {
-          a.lse[(int64_t)(m0 + (col0 + col) / a.group) * a.heads + s.head[col]] = L2 == 0.f ? m2 : M2 + __builtin_amdgcn_logf(L2);
-        } else {
-          pc[COLS * a.hd + col] = m2;
-          pc[COLS * a.hd + COLS + col] = L2;
-        }
-      }
-#pragma unroll
-      for (int k = 0; k < V4; k++) {
-        const int i = 4 * t + 1024 * k, h = i / hd, d = i - h * hd, col = 16 * ct + h;
-        if (i >= 16 * hd || s.at[col] < 0) continue;
-        if (whole) {
-          float M3, L3;
-          sums(col, M3, L3);
-          const float inv = L3 != 0.f ? 1.f / L3 : 0.f;
-          float* const y = a.y + s.at[col] * row_out + (int64_t)s.head[col] * a.hd + d;
-#pragma unroll
-          for (int e = 0; e < 4; e++) y[e] = L3 == 0.f ? 0.f : v[k][e] * inv;
-        } else {
-          *(floatx4*)(pc + col * a.hd + d) = v[k];
-        }
-      }
-    };
-    uint32_t bad = 0;
+    lds_barrier();
 #pragma unroll
     for (int ct = 0; ct < CT; ct++) {
       float M = s.wm[0][16 * ct + c];
@@ -609,43 +571,72 @@ __device__ __forceinline__ void paged_prefix_t(const PagedSharedArgs& a)
         for (int r = 0; r < 4; r++)
 #pragma unroll
           for (int e = 0; e < S::VL; e += 4)
-            *(floatx4*)&s.o[kg][c * S::OS + dh * S::DW + j * 16 * S::VL + S::VL * (4 * g + r) + e] =
+            *(floatx4*)&s.o[ct][kg][c * S::OS + dh * S::DW + j * 16 * S::VL + S::VL * (4 * g + r) + e] =
                 floatx4{o[ct][j][e][r] * f, o[ct][j][e + 1][r] * f, o[ct][j][e + 2][r] * f, o[ct][j][e + 3][r] * f};
-      __syncthreads();
-      floatx4 v[V4];
-      bool odd = false;
+    }
+    // (a tile's columns that are walked have theirs as one group of keys')
+    auto sums = [&](int col) {
+      float M2 = s.wm[0][col], L2 = 0.f;
 #pragma unroll
-      for (int k = 0; k < V4; k++) {
-        const int i = 4 * t + 1024 * k;
-        v[k] = floatx4{0.f, 0.f, 0.f, 0.f};
-        if (i >= 16 * hd) continue;
-        const int h = i / hd, d = i - h * hd;
+      for (int i = 1; i < S::KG; i++) M2 = s.wm[i][col] > M2 || s.wm[i][col] != s.wm[i][col] ? s.wm[i][col] : M2;
+      const float ms = M2 == -__builtin_inff() ? 0.f : M2;
 #pragma unroll
-        for (int p = 0; p < S::KG; p++) v[k] += *(const floatx4*)&s.o[p][h * S::OS + d];
-        odd |= s.at[16 * ct + h] >= 0 && !(finite(v[k][0]) && finite(v[k][1]) && finite(v[k][2]) && finite(v[k][3]));
-      }
-      float M2, L2;
-      if (t < 16) {
-        sums(16 * ct + t, M2, L2);
-        odd |= s.at[16 * ct + t] >= 0 && !finite(L2);
-      }
-      bad |= (uint32_t)__syncthreads_or(odd) << ct;
-      put(ct, v);
+      for (int i = 0; i < S::KG; i++) L2 += s.wl[i][col] == 0.f ? 0.f : s.wl[i][col] * exp2_fast(s.wm[i][col] - ms);
+      s.m[col] = L2 == 0.f ? -__builtin_inff() : M2;
+      s.l[col] = L2;
+      return L2;
+    };
+    bool odd = false;
+    if (t == 0) s.odd = 0;
+    if (t < COLS) odd = s.at[t] >= 0 && !finite(sums(t));
+    lds_barrier();
+    auto value = [&](int ct, int i) {
+      const float* const e = &s.o[ct][0][i / hd * S::OS + i % hd];
+      floatx4 v = *(const floatx4*)e;
+#pragma unroll
+      for (int p = 1; p < S::KG; p++) v += *(const floatx4*)(e + p * 16 * S::OS);
+      return v;
+    };
+#pragma unroll 1
+    for (int i = 4 * t; i < CT * 16 * hd; i += 1024) {
+      const floatx4 v = value(i / (16 * hd), i % (16 * hd));
+      odd |= s.at[i / hd] >= 0 && !(finite(v[0]) && finite(v[1]) && finite(v[2]) && finite(v[3]));
     }
     // (again by the formula's steps, where sums are not all finite)
-    for (; bad; bad &= bad - 1) {
-      const int ct = __builtin_ctz(bad);
-      __syncthreads();
-      prefix_walk<T, D>(a, table, kv, ct, (int64_t)tile0 * S::TK, jend, s);
-      floatx4 v[V4];
-#pragma unroll
-      for (int k = 0; k < V4; k++) {
-        const int i = min(4 * t + 1024 * k, 16 * hd - 4);
-        v[k] = *(const floatx4*)&s.o[0][i / hd * S::OS + i % hd];
+    if (__any(odd) && lane == 0) s.odd = 1;
+    lds_barrier();
+    const bool walked = s.odd != 0;
+    if (walked) {
+      for (int ct = 0; ct < CT; ct++) {
+        prefix_walk<T, D>(a, table, kv, ct, (int64_t)tile0 * S::TK, jend, s);
+        if (t < 16) sums(16 * ct + t);
       }
-      put(ct, v);
+      __syncthreads();
     }
-    __syncthreads();
+    // the columns' results: to y and lse, or to the pieces
+    if (t < COLS && s.at[t] >= 0) {
+      if (whole) {
+        a.lse[(int64_t)(m0 + (col0 + t) / a.group) * a.heads + s.head[t]] = s.l[t] == 0.f ? s.m[t] : s.m[t] + __builtin_amdgcn_logf(s.l[t]);
+      } else {
+        pc[COLS * a.hd + t] = s.m[t];
+        pc[COLS * a.hd + COLS + t] = s.l[t];
+      }
+    }
+#pragma unroll 1
+    for (int i = 4 * t; i < CT * 16 * hd; i += 1024) {
+      const int col = i / hd, d = i - col * hd, ct = col >> 4;
+      if (s.at[col] < 0) continue;
+      const floatx4 v = walked ? *(const floatx4*)&s.o[ct][0][(col & 15) * S::OS + d] : value(ct, i % (16 * hd));
+      if (whole) {
+        const float L = s.l[col], inv = L != 0.f ? 1.f / L : 0.f;
+        float* const y = a.y + s.at[col] * row_out + (int64_t)s.head[col] * a.hd + d;
+#pragma unroll
+        for (int e = 0; e < 4; e++) y[e] = L == 0.f ? 0.f : v[e] * inv;
+      } else {
+        *(floatx4*)(pc + col * a.hd + d) = v;
+      }
+    }
+    lds_barrier();
     u += tile1 - tile0;
     if (u >= end) return;
     if (tile1 == n && item + 1 == items * a.kvh) {  // the next group with a prefix
