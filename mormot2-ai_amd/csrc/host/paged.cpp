@@ -382,6 +382,12 @@ int ihip_enqueue_sample_rows(ihip_ctx* c, uint64_t logits, int64_t rows, int64_t
   if (stride > STRIDE_MOST) return refuse(who, "a stride beyond 2^36");
   if ((logits | ids | probs) % 4) return refuse(who, "arrays aligned to 4 bytes");
   if ((settings | uniform) % 8) return refuse(who, "settings and random numbers are doubles, aligned to 8 bytes");
+  // (a row's token is written while others are read)
+  for (uint64_t o : {ids, probs})
+    if (o && (overlaps(o, (__int128)rows * 4, logits, (__int128)stride * 4, (__int128)vocab * 4, rows) ||
+              overlaps(o, (__int128)rows * 4, settings, sizeof(ihip_sampling), sizeof(ihip_sampling), rows) ||
+              overlaps(o, (__int128)rows * 4, uniform, 8, 8, rows) || (o == probs && overlaps(probs, (__int128)rows * 4, ids, 4, 4, rows))))
+      return refuse(who, "ids or probs overlap another array");
   if (!c) return no_context(who);
   OnDevice on(c);
   // parts of 8192 tokens, of 4096 or 2048 where they would leave the chip's CUs empty

@@ -6,6 +6,7 @@ import os
 import pytest
 
 import infer_hip as H
+import oracle_lib as O
 from code_objects import OBJDUMP, build_of, products_wait
 from test_paged import A, pages, refused
 
@@ -39,6 +40,19 @@ def test_refused():
     refused(lambda: call(y=A + 3 * 4 * 64 * 4), -1, "no context")
     refused(lambda: call(), -1, "no context")
     refused(lambda: call(window=100), -1, "no context")
+
+
+def test_common_tokens():
+    f = O.lib().orc_paged_common
+    f.restype, f.argtypes = C.c_int64, [C.c_int32] * 4 + [C.c_int64, C.c_int32]
+    most = 2 ** 31 - 1
+    assert f(0, 2, 5, 3, 4, 16) == 5 and f(1, 3, 64, 3, 4, 16) == 64
+    assert f(1, 3, 65, 3, 4, 16) == 64 and f(0, 3, most, 3, 4, 16) == 64  # the tables' width
+    assert f(0, 3, most, 3, most, 1) == most
+    # one sequence, none, a group that ends before it begins or outside the batch, no tokens
+    for first, end, shared in ((0, 1, 5), (2, 2, 5), (2, 1, 5), (-1, 2, 5), (-2 ** 31, most, 5), (most, -2 ** 31, 5),
+                               (1, 4, 5), (0, most, 5), (0, 2, 0), (0, 2, -1), (0, 2, -2 ** 31)):
+        assert f(first, end, shared, 3, 4, 16) == 0
 
 
 @pytest.mark.parametrize("name", ["f32", "f16", "bf16", "q8"])

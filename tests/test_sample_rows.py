@@ -10,7 +10,7 @@ from test_paged import A, refused
 
 
 def call(**kw):
-    a = dict(ctx=None, x=A, rows=3, vocab=1000, stride=0, settings=A, uniform=A, ids=A, probs=A)
+    a = dict(ctx=None, x=A, rows=3, vocab=1000, stride=0, settings=2 * A, uniform=3 * A, ids=4 * A, probs=5 * A)
     a.update(kw)
     return H.lib().ihip_enqueue_sample_rows(*a.values())
 
@@ -28,6 +28,27 @@ def test_refused():
         refused(lambda: call(**{name: A + 4}), -1, "8 bytes")
     refused(lambda: call(), -1, "no context")
     refused(lambda: call(probs=0), -1, "no context")
+
+
+def test_overlaps_are_refused():
+    # of 3 rows: 12 bytes of ids and of probs, logits 1000 floats every 1100, 40 bytes of settings, 8 of uniform
+    for name in ("ids", "probs"):
+        for at in (A - 8, A, A + 4 * 999, A + 4 * 1100 - 8, A + 4 * (2200 + 999), 2 * A - 8, 2 * A + 116, 3 * A - 8, 3 * A + 20):
+            refused(lambda: call(stride=1100, **{name: at}), -1, "overlap")
+        for at in (A - 12, A + 4 * 1000, A + 4 * 1100 - 12, A + 4 * (2200 + 1000), 2 * A - 12, 2 * A + 120, 3 * A - 12, 3 * A + 24):
+            refused(lambda: call(stride=1100, **{name: at}), -1, "no context")
+    for at in (4 * A - 8, 4 * A, 4 * A + 8):
+        refused(lambda: call(probs=at), -1, "overlap")
+    for at in (4 * A - 12, 4 * A + 12):
+        refused(lambda: call(probs=at), -1, "no context")
+
+
+@pytest.mark.parametrize("vocab", [1, 2, 3, 4, 1023, 1024, 1025, 1 << 21, (1 << 21) + 1, 1 << 22])
+def test_weights_fit(vocab):
+    """A vocabulary's weights (at most 1 each) add up below 2^62, and one is below 2^52."""
+    bits = O.lib().orc_sample_weight_bits(vocab)
+    assert vocab << bits < 1 << 62 and bits <= 51
+    assert bits == 51 or vocab << bits + 2 > 1 << 62
 
 
 def splitmix(seed):
