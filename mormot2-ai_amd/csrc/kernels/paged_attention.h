@@ -1,5 +1,5 @@
-// paged_attention.h - attention of one new token of each sequence over its pages:
-// the kernel that paged.hip instantiates.
+// paged_attention.h - attention of one new token of each sequence over its pages: the
+// kernel that paged.hip, paged_q8.hip and paged_shared.hip (own tokens) instantiate.
 #pragma once
 
 #include <type_traits>

@@ -264,3 +264,44 @@ def test_captured_and_replayed(ctx, dev):
             ok = np.isfinite(tol).all((1, 2))
             assert ok.sum() >= 5
             assert_close(got[ok], want[ok], tol[ok])
+
+
+@pytest.mark.parametrize("dtype", ["f16", "q8"])
+def test_past_32_bits(ctx, dev, dtype):
+    """A prefix and own tokens more than 2^31 values into the pool, in pages that lie apart."""
+    rng = np.random.default_rng(15)
+    hd, heads, kvh, ps, pages = 128, 4, 1, 16, 4
+    stride, es = (1 << 30) + 128 * 16 * 5, 1 if dtype == "q8" else 2
+    n = stride * (pages - 1) + ps * hd
+    shape, values = (pages, ps, kvh, hd), []
+    held = [ctx.alloc(n * es) for _ in range(2)] + ([ctx.alloc(n // hd * 4 + 4) for _ in range(2)] if dtype == "q8" else [])
+    try:
+        if dtype == "q8":
+            raw = [rng.integers(-127, 128, shape).astype(np.int8) for _ in range(2)]
+            raw += [(rng.random(shape[:3]) / 73).astype(np.float32) for _ in range(2)]
+            values = [c.astype(np.float64) * s[..., None] for c, s in zip(raw[:2], raw[2:])]
+        else:
+            raw = [R.pack(rng.standard_normal(shape), dtype) for _ in range(2)]
+            values = [R.unpack(a, dtype) for a in raw]
+        for i, a in enumerate(raw):
+            for p in range(pages):
+                page = np.ascontiguousarray(a[p])
+                step = stride * es if i < 2 else stride // hd * 4
+                H.check(H.lib().ihip_upload(ctx.h, held[i].ptr + p * step, page.ctypes.data, page.nbytes))
+        pool = H.Pages(k=held[0].ptr, v=held[1].ptr, pages=pages, page_stride=stride, page_size=ps, kv_heads=kvh, head_dim=hd,
+                       dtype=H.Q8_HEAD if dtype == "q8" else H.F16, k_scale=held[2].ptr if dtype == "q8" else 0,
+                       v_scale=held[3].ptr if dtype == "q8" else 0)
+        table, lengths = np.array([[3, 1, 0], [3, 1, 2]], np.int32), np.array([45, 41], np.int32)
+        q = rng.standard_normal((2, heads, hd)).astype(np.float32)
+        y = dev.out(q.nbytes)
+        H.check(H.lib().ihip_enqueue_paged_attention_shared(
+            ctx.h, dev(q), 0, C.byref(pool), dev(table), 3, dev(lengths), 0, 2, dev(np.array([0, 2], np.int32)),
+            dev(np.array([30], np.int32)), 1, y.ptr, 2, heads, 0, 0, 0.0))
+        want, tol = R.attention(q.astype(np.float64), *values, table, lengths, ps)
+        # (8-bit pages' small weights are off by 2^-39 of the largest scale more)
+        assert_close(y.download(np.float32, q.size).reshape(q.shape), want,
+                     tol + (2.0 ** -39 * 45 * 128 / 73 if dtype == "q8" else 0))
+    finally:
+        ctx.sync()
+        for b in held:
+            b.free()
