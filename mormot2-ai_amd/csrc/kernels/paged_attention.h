@@ -168,20 +168,6 @@ __device__ __forceinline__ int find_last(const int* first, int n, int i)
   return lo;
 }
 
-// a sequence's group, -1 where it has none, and how many of its tokens are read once for
-// the group
-__device__ __forceinline__ int64_t shared_tokens(const PagedSharedArgs& a, int seq, int& g)
-{
-  g = -1;
-  if (a.groups < 1) return 0;
-  const int at = find_last(a.members, a.groups, seq);
-  const int m0 = a.members[at], m1 = a.members[at + 1];
-  if (seq < m0 || seq >= m1) return 0;
-  const int64_t n = paged_common(m0, m1, a.shared[at], a.seqs, a.max_pages, a.page_size);
-  if (n > 0) g = at;
-  return n;
-}
-
 // `all` tiles shared out evenly over B blocks: block i takes first(i) .. first(i + 1) - 1
 struct PieceShare {
   uint32_t all, B, quot, rem;
@@ -257,7 +243,28 @@ struct AttnPrefix {
   float m[16], l[16];          // its maxima (base 2) and sums
   int first[16], count[16];    // the blocks of its pieces; count 0: in y and lse
   int col[16];                 // a head's column in the pieces
+  int members[64], shared[64]; // the groups, of 3 to 63 (of fewer the search reads no more)
 };
+
+// a sequence's group, -1 where it has none, and how many of its tokens are read once for
+// the group
+__device__ __forceinline__ int64_t shared_tokens(const PagedSharedArgs& a, const AttnPrefix& px, int seq, int& g)
+{
+  g = -1;
+  if (a.groups < 1) return 0;
+  int at, m0, m1, n0;
+  if (a.groups > 2 && a.groups < 64) {
+    at = find_last(px.members, a.groups, seq);
+    m0 = px.members[at], m1 = px.members[at + 1], n0 = px.shared[at];
+  } else {
+    at = find_last(a.members, a.groups, seq);
+    m0 = a.members[at], m1 = a.members[at + 1], n0 = a.shared[at];
+  }
+  if (seq < m0 || seq >= m1) return 0;
+  const int64_t n = paged_common(m0, m1, n0, a.seqs, a.max_pages, a.page_size);
+  if (n > 0) g = at;
+  return n;
+}
 
 // The heads of a piece whose sums are not all finite, again by the formula's own
 // steps in single: the matrix cores' parts turn an infinity into NaN (0 times it
@@ -420,6 +427,16 @@ __device__ __forceinline__ void paged_attention_t(const A& a)
   const uint32_t grid = gridDim.x, b = blockIdx.x, per = a.kvh * a.tiles;
   const int hd = FULL ? D : a.hd, row_out = a.heads * a.hd;
 
+  __shared__ typename std::conditional<is_shared<A>, AttnPrefix, int>::type px;
+  if constexpr (is_shared<A>) {
+    // the groups into LDS, where a sequence's is searched (each wave for itself, the same)
+    if (a.groups > 2 && a.groups < 64) {
+      px.members[lane] = lane <= a.groups ? a.members[lane] : 0;
+      px.shared[lane] = lane < a.groups ? a.shared[lane] : 0;
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+    }
+  }
   // a sequence's row, -1 where it has none in this step
   auto row_of = [&](int seq) {
     return a.offsets ? paged_row(a.offsets[seq], a.offsets[seq + 1], a.rows) : paged_row(seq, seq + 1, a.rows);
@@ -430,22 +447,22 @@ __device__ __forceinline__ void paged_attention_t(const A& a)
     paged_range(a.lengths[seq], a.window, a.max_pages, a.page_size, &lo, &hi);
     if constexpr (is_shared<A>) {
       int grp;
-      lo = min(hi, shared_tokens(a, seq, grp));
+      lo = min(hi, shared_tokens(a, px, seq, grp));
     }
     return (uint32_t)((hi - lo + S::TK - 1) / S::TK);
   };
   // the heads' part of their sequence's prefix; whether there is one
-  auto prefix_of = [&](const AttnItem& it, auto& px) {
+  auto prefix_of = [&](const AttnItem& it) {
     if constexpr (is_shared<A>) {
       int grp;
-      if (shared_tokens(a, it.s, grp) == 0) return false;
+      if (shared_tokens(a, px, it.s, grp) == 0) return false;
       const int pall = a.plan[0], pb = a.plan[1], pct = a.plan[2] * 16;
       if (pall <= 0) return false;
       const uint32_t before = a.plan[SHARED_PLAN + 3 * grp], pn = a.plan[SHARED_PLAN + 3 * grp + 1];
       const int cts = a.plan[SHARED_PLAN + 3 * grp + 2];
       const int64_t size = (int64_t)pct * (a.hd + 2);
       const int h = t >> 4;
-      __syncthreads();
+      lds_barrier();
       if (h < it.heads) {
         const int col = (it.s - a.members[grp]) * a.group + it.head0 - it.kv * a.group + h;
         const uint32_t u0 = before + (uint32_t)(it.kv * cts + col / pct) * pn;
@@ -483,7 +500,7 @@ __device__ __forceinline__ void paged_attention_t(const A& a)
           px.col[h] = c16;
         }
       }
-      __syncthreads();
+      lds_barrier();
       return true;
     } else {
       return false;
@@ -491,7 +508,7 @@ __device__ __forceinline__ void paged_attention_t(const A& a)
   };
   // 4 values of a head, own ones over the maximum m with sum l, joined with the prefix's and
   // the sink's weight
-  auto with_prefix = [&](const AttnItem& it, auto& px, int h, int d, float m, float l, float (&v)[4]) {
+  auto with_prefix = [&](const AttnItem& it, int h, int d, float m, float l, float (&v)[4]) {
     if constexpr (is_shared<A>) {
       const int pct = a.plan[2] * 16;
       const int64_t size = (int64_t)pct * (a.hd + 2);
@@ -539,7 +556,6 @@ __device__ __forceinline__ void paged_attention_t(const A& a)
       }
     }
   };
-  __shared__ typename std::conditional<is_shared<A>, AttnPrefix, int>::type px;
   // What an item (a sequence's KV head) costs beside its tiles of keys, in tiles: its query,
   // the waves' meeting, the prefix. The blocks share out tiles and these, so that one
   // with many short items has as much to do (three prompts' 480 items of 1 to 8 tiles, on
@@ -574,11 +590,11 @@ __device__ __forceinline__ void paged_attention_t(const A& a)
           it.kv = i / a.tiles;
           it.heads = min(16, a.group - 16 * (i % a.tiles));
           it.head0 = it.kv * a.group + 16 * (i % a.tiles);
-          done = prefix_of(it, px);
+          done = prefix_of(it);
           if (!done) break;
           for (int j = 4 * t; j < it.heads * a.hd; j += 1024) {
             float v[4] = {0.f, 0.f, 0.f, 0.f};
-            with_prefix(it, px, j / a.hd, j % a.hd, 0.f, 0.f, v);
+            with_prefix(it, j / a.hd, j % a.hd, 0.f, 0.f, v);
 #pragma unroll
             for (int e = 0; e < 4; e++) y[(int64_t)it.head0 * a.hd + j + e] = v[e];
           }
@@ -726,6 +742,9 @@ __device__ __forceinline__ void paged_attention_t(const A& a)
     // read the pool's first row.
     uint32_t there = locate(tile, page0);
     if (steps) load_keys(tile);
+    // (what the item's heads have of a prefix, looked up while the first keys are on their way)
+    bool pre = false;
+    if constexpr (is_shared<A>) pre = prefix_of(it);
     for (uint32_t i = 0; i < steps; i++, tile++) {
       // the step's values, on their way while its scores are formed
       constexpr int NV = 4 * S::NT;  // keys of a lane: 16 q + 4 g + r
@@ -936,7 +955,6 @@ __device__ __forceinline__ void paged_attention_t(const A& a)
       paged_walk<T, D>(a, it, lo + (int64_t)tile0 * S::TK, min(hi, lo + (int64_t)tile1 * S::TK), s);
 
     float* const y = a.y + (int64_t)it.row * row_out + (int64_t)it.head0 * a.hd;
-    bool pre = false;  // joined with a prefix (where this block ends the item)
     // with the sink: its weight beside the sum's, both against the larger maximum
     auto finish = [&](int h, float m2, float l2, float& f2) {
       f2 = 1.f;
@@ -953,13 +971,12 @@ __device__ __forceinline__ void paged_attention_t(const A& a)
     };
     if (tile0 == 0 && tile1 == n) {
       if constexpr (is_shared<A>) {
-        pre = prefix_of(it, px);
         for (int j = 4 * t; pre && j < it.heads * a.hd; j += 1024) {
           const int h = j / a.hd, d = j - h * a.hd;
           float v[4];
 #pragma unroll
           for (int e = 0; e < 4; e++) v[e] = s.o[h * S::OS + d + e];
-          with_prefix(it, px, h, d, s.m[h], s.l[h], v);
+          with_prefix(it, h, d, s.m[h], s.l[h], v);
 #pragma unroll
           for (int e = 0; e < 4; e++) y[j + e] = v[e];
         }
@@ -993,8 +1010,6 @@ __device__ __forceinline__ void paged_attention_t(const A& a)
       auto join = [&](uint32_t i0, uint32_t step, uint32_t cnt, bool out) {
         // 4 values of 16 pieces a thread, the first on their way while the weights are formed
         const int total = it.heads * a.hd;
-        if constexpr (is_shared<A>)
-          if (out) pre = prefix_of(it, px);
         uint64_t x[16][2];
         auto fetch = [&](int i, uint32_t j0) {
 #pragma unroll
@@ -1057,7 +1072,7 @@ __device__ __forceinline__ void paged_attention_t(const A& a)
             }
           }
           if (out && pre) {
-            with_prefix(it, px, h, i - h * a.hd, s.m[h], s.l[h], v);
+            with_prefix(it, h, i - h * a.hd, s.m[h], s.l[h], v);
 #pragma unroll
             for (int e = 0; e < 4; e++) y[i + e] = v[e];
           } else if (out) {
