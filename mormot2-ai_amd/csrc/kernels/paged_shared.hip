@@ -10,7 +10,7 @@ using namespace ihip;
 // their registers: heads of 128 two tiles (32 chats behind 4096 tokens 26 us; four tiles
 // and one block a CU 33, four that spill 53), of 64 four (128 sequences behind 30011
 // 240 us; two and three blocks a CU 245, two and four 310), of 256 in 8-bit pages one (three
-// prompts of 9001 75 us; two and one block 95 where one took 80). Others of 256 have two and
+// prompts of 9001 68 us; two and one block 95 where one took 80). Others of 256 have two and
 // one block (halves 97 us; one and two that spill 135 where two took 111).
 template <int T, int D>
 constexpr int shared_ct = D <= 64 ? 4 : D <= 128 ? 2 : D == 256 && T != 3 ? 2 : 1;
@@ -129,7 +129,7 @@ __device__ __forceinline__ void paged_prefix_t(const PagedSharedArgs& a)
   __shared__ PrefixLds<T, D> s;
   const int t = threadIdx.x, lane = t & 63, c = lane & 15, g = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(t >> 6);
-  const uint32_t grid = gridDim.x, b = blockIdx.x;
+  const uint32_t grid = gridDim.x;
   const int hd = FULL ? D : a.hd, row_out = a.heads * a.hd;
 
   // a group's items of a KV head and tiles of keys
@@ -149,6 +149,10 @@ __device__ __forceinline__ void paged_prefix_t(const PagedSharedArgs& a)
   // (groups that overlap, which no caller has, may pass 32 bits)
   const uint32_t all = total < (1u << 31) ? __builtin_amdgcn_readfirstlane((uint32_t)total) : 0u;
   const uint32_t B = min(grid, all);
+  // blocks that follow each other take the columns behind the same keys: onto one XCD (block
+  // i runs on XCD i mod 8), whose L2 then has them (three prompts of 9001, 8-bit heads of 256:
+  // 339 MiB fetched and 75 us, so 280 and 68)
+  const uint32_t x = blockIdx.x, b = B == grid && grid % 8 == 0 ? x % 8 * (grid / 8) + x / 8 : x;
   if (b == 0) {
     if (t == 0) {
       a.plan[0] = (int)all;
