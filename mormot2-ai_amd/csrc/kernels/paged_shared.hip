@@ -120,7 +120,10 @@ __device__ __forceinline__ void prefix_walk(const PagedSharedArgs& a, const int*
 // columns, the query tiles in LDS. All groups' tiles of keys are one row, shared out
 // evenly over the grid. A block that has the whole of an item (KV head, columns) finishes
 // it into y and lse; parts go to `pieces`, and the launch over the sequences' own tokens
-// joins them.
+// joins them. Bound by issue where a group is large (128 sequences behind 30011 tokens, 64
+// heads of 64 over 8 in bf16 235 us: vector work 69%, matrix cores 40% of the SIMDs' time, of
+// weights in three parts), by loads' latency where its columns are few (the sizes at
+// shared_ct).
 template <int T, int D, bool FULL>
 __device__ __forceinline__ void paged_prefix_t(const PagedSharedArgs& a)
 {
