@@ -391,6 +391,59 @@ __device__ __forceinline__ void stage_query(const PagedAttnArgs& a, const AttnIt
   __syncthreads();
 }
 
+// The same with all of a thread's factors on their way at once (8-bit pages and groups);
+// gives the power of two of the lane's head
+template <int T, int D>
+__device__ __forceinline__ float stage_query_once(const PagedAttnArgs& a, const AttnItem& it, AttnLds<T, D>& s)
+{
+  using S = AttnShape<T, D>;
+  constexpr int TILE = S::DS * S::NF * 64, R = (TILE + 255) / 256;
+  const int t = threadIdx.x, c = t & 15;
+  const float* const q = a.q + it.row * a.q_stride + (int64_t)(it.head0 + min(c, it.heads - 1)) * a.hd;
+  float v[R][S::FL];
+#pragma unroll
+  for (int r = 0; r < R; r++) {
+    const int i = t + 256 * r, d0 = S::factor(i >> 6, (i >> 4) & 3);
+    const bool in = i < TILE && c < it.heads && d0 < a.hd;
+#pragma unroll
+    for (int j = 0; j < S::FL; j++) v[r][j] = in ? q[d0 + j] : 0.f;
+  }
+  float power = 1.f;
+  if constexpr (T == 1 || T == 3) {
+    float top = 0.f;
+#pragma unroll
+    for (int r = 0; r < R; r++)
+#pragma unroll
+      for (int j = 0; j < S::FL; j++) top = fmaxf(top, fabsf(v[r][j] * a.scale));
+    top = quad_max(top);
+    if ((t & 63) < 16) s.wm[t >> 6][c] = top;
+    lds_barrier();
+    top = fmaxf(fmaxf(s.wm[0][c], s.wm[1][c]), fmaxf(s.wm[2][c], s.wm[3][c]));
+    int e = (int)(float_bits(top) >> 23) - 126;  // top < 2^e
+    if (top == 0.f || !finite(top)) e = 14;
+    power = ldexpf(1.f, max(e - 14, -120));
+  }
+#pragma unroll
+  for (int r = 0; r < R; r++) {
+    const int i = t + 256 * r;
+    if (i >= TILE) break;
+    const float f = T == 1 || T == 3 ? 1.f / power : a.scale;
+#pragma unroll
+    for (int j = 0; j < S::FL; j++) v[r][j] = T == 1 || T == 3 ? v[r][j] * a.scale * f : v[r][j] * f;
+    if constexpr (T == 0) {
+      s.q[i] = uintx4{float_bits(v[r][0]), float_bits(v[r][1]), float_bits(v[r][2]), float_bits(v[r][3])};
+    } else {
+      uint32_t part[4][S::NP];
+#pragma unroll
+      for (int j = 0; j < 4; j++) split2<T>(v[r][2 * j], v[r][2 * j + 1], part[j]);
+#pragma unroll
+      for (int n = 0; n < S::NP; n++) s.q[n * TILE + i] = uintx4{part[0][n], part[1][n], part[2][n], part[3][n]};
+    }
+  }
+  lds_barrier();
+  return power;
+}
+
 // Attention of one token of each sequence. The work of all sequences and KV heads
 // is one row of tiles of TK keys, shared out evenly over the grid's blocks
 // (ragged lengths leave no block idle, and a captured grid fits the lengths of
@@ -443,12 +496,18 @@ __device__ __forceinline__ void paged_attention_t(const A& a)
   };
   auto tiles_of = [&](int seq, int64_t& lo, int64_t& hi) {
     lo = hi = 0;
+    if constexpr (is_shared<A>) {
+      // (a sequence without a token of its own has a tile without keys, for its prefix)
+      const int length = a.lengths[seq], row = row_of(seq);
+      int grp;
+      const int64_t common = shared_tokens(a, px, seq, grp);
+      if (row < 0 || length < 0) return 0u;
+      paged_range(length, a.window, a.max_pages, a.page_size, &lo, &hi);
+      lo = min(hi, common);
+      return max(1u, (uint32_t)((hi - lo + S::TK - 1) / S::TK));
+    }
     if (row_of(seq) < 0) return 0u;
     paged_range(a.lengths[seq], a.window, a.max_pages, a.page_size, &lo, &hi);
-    if constexpr (is_shared<A>) {
-      int grp;
-      lo = min(hi, shared_tokens(a, px, seq, grp));
-    }
     return (uint32_t)((hi - lo + S::TK - 1) / S::TK);
   };
   // the heads' part of their sequence's prefix; whether there is one
@@ -573,34 +632,13 @@ __device__ __forceinline__ void paged_attention_t(const A& a)
       int64_t lo, hi;
       n = tiles_of(seq, lo, hi);
       if (s0 == 0) n0 = n, lo0 = lo, hi0 = hi;
-      zero = n == 0 && a.lengths[seq] >= 0 && row_of(seq) >= 0 && (uint32_t)seq % grid == b;
+      zero = !is_shared<A> && n == 0 && a.lengths[seq] >= 0 && row_of(seq) >= 0 && (uint32_t)seq % grid == b;
     }
     if (n) all += (n + OV) * per;
     if (OV) longest = max(longest, n);
     live += __popcll(__ballot(n != 0));
     for (uint64_t z = __ballot(zero); z; z &= z - 1) {
       float* const y = a.y + (int64_t)row_of(s0 + __builtin_ctzll(z)) * row_out;
-      if constexpr (is_shared<A>) {
-        // no token of its own: the prefix alone, where there is one
-        AttnItem it;
-        it.s = s0 + __builtin_ctzll(z);
-        it.row = row_of(it.s);
-        bool done = true;
-        for (int i = 0; i < (int)per && done; i++) {
-          it.kv = i / a.tiles;
-          it.heads = min(16, a.group - 16 * (i % a.tiles));
-          it.head0 = it.kv * a.group + 16 * (i % a.tiles);
-          done = prefix_of(it);
-          if (!done) break;
-          for (int j = 4 * t; j < it.heads * a.hd; j += 1024) {
-            float v[4] = {0.f, 0.f, 0.f, 0.f};
-            with_prefix(it, j / a.hd, j % a.hd, 0.f, 0.f, v);
-#pragma unroll
-            for (int e = 0; e < 4; e++) y[(int64_t)it.head0 * a.hd + j + e] = v[e];
-          }
-        }
-        if (done) continue;
-      }
       for (int i = t; i < row_out; i += 256) y[i] = 0.f;
     }
   }
@@ -701,8 +739,13 @@ __device__ __forceinline__ void paged_attention_t(const A& a)
     uint32_t tile = tile0;
     const int page0 = entry(tile);
     int page = entry(tile + 1);
-    stage_query<T, D>(a, it, s);
-    const float sscale = T == 1 || T == 3 ? s.qs[c] : 1.f;
+    float sscale = 1.f;
+    if constexpr (OV != 0) {
+      sscale = stage_query_once<T, D>(a, it, s);
+    } else {
+      stage_query<T, D>(a, it, s);
+      if constexpr (T == 1 || T == 3) sscale = s.qs[c];
+    }
 
     uintx4 kr[S::NT][S::NQ];
     auto load_keys = [&](uint32_t tile) {

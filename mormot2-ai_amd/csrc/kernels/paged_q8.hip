@@ -5,7 +5,7 @@
 using namespace ihip;
 
 // HBM bound: 64 sequences of 100 to 16384 keys, 16 heads of 128 over 8, 1.12 GB: 237 us, 4.7
-// TB/s; one of 1152 keys is a chain of round trips (13.4 us). The codes become halves and
+// TB/s; one of 1152 keys is a chain of round trips (12.9 us). The codes become halves and
 // the values are turned in registers, as much vector work as a step's loads take, which two
 // blocks a CU cover for heads of 128 (one 272 us); heads of 64 and of 256 keep all in the
 // registers of one block a CU (194 us, two 209; 445 us, two that spill 492), and so do sizes
