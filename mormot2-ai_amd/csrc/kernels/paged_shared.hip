@@ -143,10 +143,13 @@ __device__ __forceinline__ void paged_prefix_t(const PagedSharedArgs& a)
     return (uint32_t)((common + S::TK - 1) / S::TK);
   };
   uint64_t total = 0;
+  uint32_t n0 = 0, items0 = 0;  // of the first 64 groups, a lane each
+  int64_t common0 = 0;
   for (int g0 = 0; g0 < a.groups; g0 += 64) {
     uint32_t items = 0, n = 0;
-    int64_t common;
+    int64_t common = 0;
     if (g0 + lane < a.groups) n = shape_of(g0 + lane, items, common);
+    if (g0 == 0) n0 = n, items0 = items, common0 = common;
     total += wave_sum((uint64_t)n * items * (uint32_t)a.kvh, 64);
   }
   // (groups that overlap, which no caller has, may pass 32 bits)
@@ -156,50 +159,49 @@ __device__ __forceinline__ void paged_prefix_t(const PagedSharedArgs& a)
   // i runs on XCD i mod 8), whose L2 then has them (three prompts of 9001, 8-bit heads of 256:
   // 339 MiB fetched and 75 us, so 280 and 68)
   const uint32_t x = blockIdx.x, b = B == grid && grid % 8 == 0 ? x % 8 * (grid / 8) + x / 8 : x;
-  if (b == 0) {
-    if (t == 0) {
-      a.plan[0] = (int)all;
-      a.plan[1] = (int)B;
-      a.plan[2] = CT;
-    }
-    if (w == 0) {
-      uint32_t before = 0;
-      for (int g0 = 0; g0 < a.groups; g0 += 64) {
-        uint32_t items = 0, n = 0;
-        int64_t common;
-        if (g0 + lane < a.groups) n = shape_of(g0 + lane, items, common);
-        const uint32_t mine = n * items * a.kvh;
-        uint32_t upto = mine;
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) {
-          const uint32_t o = __shfl_up(upto, d, 64);
-          if (lane >= d) upto += o;
-        }
-        if (g0 + lane < a.groups) {
-          int* const e = a.plan + SHARED_PLAN + 3 * (g0 + lane);
-          e[0] = (int)(before + upto - mine);
-          e[1] = (int)n;
-          e[2] = (int)items;
-        }
-        before += __shfl(upto, 63, 64);
-      }
-    }
+  if (b == 0 && t == 0) {
+    a.plan[0] = (int)all;
+    a.plan[1] = (int)B;
+    a.plan[2] = CT;
   }
-  if (b >= B) return;
-  const PieceShare share(all, B);
-  uint32_t u = share.first(b);
-  const uint32_t end = share.first(b + 1);
-  // the group of tile u
-  int grp = 0;
+  if (b >= B && b) return;
+  const PieceShare share(max(all, 1u), max(B, 1u));
+  uint32_t u = B ? share.first(b) : UINT32_MAX;
+  const uint32_t end = B ? share.first(b + 1) : 0u;
+  // the group of tile u (and the plan, by the first block)
+  int grp = -1;
   uint32_t before = 0, n = 0, items = 0;
   int64_t common = 0;
-  for (;; grp++) {
-    if (grp >= a.groups) return;
-    n = shape_of(grp, items, common);
-    if (before + n * items * a.kvh > u) break;
-    before += n * items * a.kvh;
+  uint32_t upto_all = 0;
+  for (int g0 = 0; g0 < a.groups; g0 += 64) {
+    if (g0 && g0 + lane < a.groups) n0 = shape_of(g0 + lane, items0, common0);
+    else if (g0) n0 = items0 = 0;
+    const uint32_t mine = n0 * items0 * a.kvh;
+    uint32_t upto = mine;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      const uint32_t o = __shfl_up(upto, d, 64);
+      if (lane >= d) upto += o;
+    }
+    if (b == 0 && w == 0 && g0 + lane < a.groups) {
+      int* const e = a.plan + SHARED_PLAN + 3 * (g0 + lane);
+      e[0] = (int)(upto_all + upto - mine);
+      e[1] = (int)n0;
+      e[2] = (int)items0;
+    }
+    const uint64_t there = __ballot(upto_all + upto > u);
+    if (there && grp < 0) {
+      const int f = __builtin_ctzll(there);
+      grp = __builtin_amdgcn_readfirstlane(g0 + f);
+      before = upto_all + __builtin_amdgcn_readlane(upto - mine, f);
+      n = __builtin_amdgcn_readlane(n0, f);
+      items = __builtin_amdgcn_readlane(items0, f);
+      common = (int64_t)lane_value((uint64_t)common0, f);
+      if (b) break;
+    }
+    upto_all += __builtin_amdgcn_readlane(upto, 63);
   }
-  grp = __builtin_amdgcn_readfirstlane(grp);
+  if (grp < 0) return;  // (no tile)
 
   for (;;) {
     const uint32_t item = (u - before) / n, tile0 = (u - before) - item * n;
