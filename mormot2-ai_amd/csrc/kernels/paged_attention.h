@@ -351,7 +351,7 @@ __device__ __forceinline__ void stage_query(const PagedAttnArgs& a, const AttnIt
   using S = AttnShape<T, D>;
   const int t = threadIdx.x;
   const float* const q = a.q + it.row * a.q_stride + (int64_t)it.head0 * a.hd;
-  if constexpr (T == 1 || T == 3) {
+  if constexpr (T == 1) {
     const int c = t >> 4;
     float top = 0.f;
     if (c < it.heads)
@@ -372,11 +372,11 @@ __device__ __forceinline__ void stage_query(const PagedAttnArgs& a, const AttnIt
     float v[S::FL];
     const bool in = c < it.heads && d0 < a.hd;
     float f = a.scale;
-    if constexpr (T == 1 || T == 3) f = 1.f / s.qs[c];
+    if constexpr (T == 1) f = 1.f / s.qs[c];
 #pragma unroll
     for (int j = 0; j < S::FL; j++) {
       v[j] = in ? q[c * a.hd + d0 + j] : 0.f;
-      v[j] = T == 1 || T == 3 ? v[j] * a.scale * f : v[j] * f;
+      v[j] = T == 1 ? v[j] * a.scale * f : v[j] * f;
     }
     if constexpr (T == 0) {
       s.q[i] = uintx4{float_bits(v[0]), float_bits(v[1]), float_bits(v[2]), float_bits(v[3])};
@@ -744,7 +744,7 @@ __device__ __forceinline__ void paged_attention_t(const A& a)
       sscale = stage_query_once<T, D>(a, it, s);
     } else {
       stage_query<T, D>(a, it, s);
-      if constexpr (T == 1 || T == 3) sscale = s.qs[c];
+      if constexpr (T == 1) sscale = s.qs[c];
     }
 
     uintx4 kr[S::NT][S::NQ];
