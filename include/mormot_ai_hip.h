@@ -732,9 +732,9 @@ int ihip_enqueue_paged_read(ihip_ctx* ctx, const ihip_pages* cache, uint64_t tab
  * [rows] (or 0) the probability that each had among those that its filters left (1 of a
  * greedy row). A temperature of 0 or below (or below 1e-30) is greedy: the largest logit,
  * the lowest id on a tie, NaN skipped; so is a row whose largest logit is infinite. Logits
- * of -infinity and NaN are never drawn. Settings
- * that ihip_sampler_create refuses give id -1 and probability 0, for that row alone. ids
- * and probs that overlap each other or another array are refused. */
+ * of -infinity and NaN are never drawn, nor is a token whose weight is below 2^-1000 of
+ * the best one's. Settings that ihip_sampler_create refuses give id -1 and probability 0,
+ * for that row alone. ids and probs that overlap each other or another array are refused. */
 int ihip_enqueue_sample_rows(ihip_ctx* ctx, uint64_t logits, int64_t rows, int64_t vocab,
                              int64_t stride, uint64_t settings, uint64_t uniform, uint64_t ids,
                              uint64_t probs);

@@ -447,48 +447,67 @@ extern "C" __global__ __launch_bounds__(256) void sample_rows_finish(SampleRowsA
     }
     if (part / pq == t) base = before;
     __syncthreads();
-    // the group of its tokens, by a wave's lanes, then the group's tokens, two a thread
+    // The group of its tokens, by a wave's lanes, then the group's tokens, two a thread. (Tokens
+    // without a weight are in its group's sum, as 2^-1000 of the part's best each: a group
+    // that turns out to have no other is passed over, and the next one whose sums pass the
+    // target is taken, or, where none does, for roundings, the last one before.)
     const float pm = a.best[p0 + part];
+    double mine = 0, upto = 0;
+    uint64_t ahead = 0, behind = 0;
     if (w == 0) {
       const double* const g = (const double*)(a.octaves + (p0 + part) * OCT);
-      const double mine = lane < a.per / GROUP ? g[lane] * weight_of(pm) : 0.0, upto = base + wave_scan(mine);
-      const uint64_t there = __ballot(mine > 0 && target < upto), any = __ballot(mine > 0);
-      const int at = there ? __builtin_ctzll(there) : any ? 63 - __builtin_clzll(any) : 0;
-      if (lane == at) {
-        sums[0] = upto - mine;
-        slot = at;
+      mine = lane < a.per / GROUP ? g[lane] * weight_of(pm) : 0.0;
+      upto = base + wave_scan(mine);
+      ahead = __ballot(mine > 0 && target < upto);
+      behind = __ballot(mine > 0) & ~ahead;
+    }
+    for (;;) {
+      if (w == 0) {
+        const int at = ahead ? __builtin_ctzll(ahead) : behind ? 63 - __builtin_clzll(behind) : -1;
+        if (lane == max(at, 0)) {
+          sums[0] = upto - mine;
+          slot = at;
+          found = INT32_MAX;
+          seen = -1;
+        }
+        if (ahead) ahead &= ahead - 1;
+        else if (behind) behind &= ~(1ull << at);
       }
+      __syncthreads();
+      const int group = slot;
+      if (group < 0) {  // (not reached: the part's best has a weight)
+        if (t == 0) answer(best, 1.0 / all);
+        return;
+      }
+      const int i0 = part * a.per + group * GROUP + 2 * t;
+      const double start = sums[0];
+      double wt[2], group_all;
+#pragma unroll
+      for (int e = 0; e < 2; e++) wt[e] = i0 + e < a.vocab ? weight_of(x[i0 + e]) : 0.0;
+      double run = start + scan_threads<NT>(wt[0] + wt[1], sums, group_all);
+      int first = INT32_MAX, last = -1;
+#pragma unroll
+      for (int e = 0; e < 2; e++) {
+        run = run + wt[e];
+        if (wt[e] > 0) last = i0 + e;  // (the last one, where roundings leave none)
+        if (wt[e] > 0 && target < run) first = min(first, i0 + e);
+      }
+      last = wave_max(last);
+      first = -wave_max(-first);
       if (lane == 0) {
-        found = INT32_MAX;
-        seen = -1;
+        atomicMax(&seen, last);
+        atomicMin(&found, first);
       }
+      __syncthreads();
+      if (group_all > 0) {
+        if (t == 0) {
+          const int i = found != INT32_MAX ? found : seen;
+          answer(i, weight_of(x[i]) / all);
+        }
+        return;
+      }
+      __syncthreads();
     }
-    __syncthreads();
-    const int i0 = part * a.per + slot * GROUP + 2 * t;
-    const double start = sums[0];
-    double wt[2], group_all;
-#pragma unroll
-    for (int e = 0; e < 2; e++) wt[e] = i0 + e < a.vocab ? weight_of(x[i0 + e]) : 0.0;
-    double run = start + scan_threads<NT>(wt[0] + wt[1], sums, group_all);
-    int first = INT32_MAX, last = -1;
-#pragma unroll
-    for (int e = 0; e < 2; e++) {
-      run = run + wt[e];
-      if (wt[e] > 0) last = i0 + e;  // (the last one, where roundings leave none)
-      if (wt[e] > 0 && target < run) first = min(first, i0 + e);
-    }
-    last = wave_max(last);
-    first = -wave_max(-first);
-    if (lane == 0) {
-      atomicMax(&seen, last);
-      atomicMin(&found, first);
-    }
-    __syncthreads();
-    if (t == 0) {
-      const int i = found != INT32_MAX ? found : seen >= 0 ? seen : best;
-      answer(i, weight_of(x[i]) / all);
-    }
-    return;
   }
 
   // the octave below the best weight that surely holds k tokens, or top_p of the sum
