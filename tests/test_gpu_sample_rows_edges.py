@@ -1,5 +1,5 @@
-"""Draws of rows whose first or last tokens cannot be drawn (constrained decoding),
-against the definition in 64 bits."""
+"""Draws of rows whose first or last tokens cannot be drawn (constrained decoding), and of more
+rows with bins than one launch has places for, against the definition in 64 bits."""
 import numpy as np
 import pytest
 
@@ -63,3 +63,22 @@ def test_weights_that_are_none(ctx, dev):
     ids, probs = b.read()
     assert ids.tolist() == [1500, 1500, 2048]
     assert probs[2] == 1
+
+
+def test_more_rows_with_bins_than_places(ctx, dev):
+    """Every row has more candidates than are sorted; 512 of a launch have bins formed by the whole
+    grid, which ones by chance, and the others form theirs alone: all the same, from run to run,
+    and the next call's are counted from 0 again."""
+    rng = np.random.default_rng(6)
+    rows, vocab = 620, 5003
+    x = (rng.standard_normal((rows, vocab)) * 2.5).astype(np.float32)
+    b = Rows(dev, x, [(30.0, 0, 0.5, 0.0)] * rows, rng.random(rows))
+    b.check(ctx)
+    ids, probs = b.read()
+    for _ in range(2):
+        b.enqueue(ctx)
+        again = b.read()
+        assert np.array_equal(again[0], ids) and np.array_equal(again[1].view(np.uint32), probs.view(np.uint32))
+    few = Rows(dev, x[:5], [(30.0, 0, 0.5, 0.0)] * 5, b.u[:5])
+    few.check(ctx)
+    assert np.array_equal(few.read()[0], ids[:5])
