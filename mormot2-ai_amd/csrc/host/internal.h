@@ -106,7 +106,7 @@ struct ihip_ctx {
   uint64_t scratch_attn = 0, scratch_attn_bytes = 0;
   uint64_t paged_plan = 0;  // the step plan between ihip_enqueue_paged_slots' two launches, a counter behind it
   uint64_t paged_part = 0;  // paged_attention's shared pieces and counters (zero between launches)
-  uint64_t paged_shared = 0;  // parts of shared prefixes, their sums' logarithms, and the plan of them
+  uint64_t paged_shared = 0;  // parts of shared prefixes, their maxima and sums, and the plan of them
   uint64_t sample_rows = 0;  // ihip_enqueue_sample_rows' parts of the rows
   uint64_t logprobs_part = 0;  // the same of ihip_enqueue_logprobs
   uint64_t scratch_planes = 0, scratch_planes_bytes = 0;  // e4m3 activation planes (gemm_mxfp4_f8)
@@ -162,11 +162,11 @@ constexpr int64_t PAGED_ROWS_HERE = 4096;
 constexpr int64_t PAGED_BLOCKS = 1024;
 constexpr uint64_t PAGED_PART_BYTES = 17u << 20;
 // paged attention of groups that share their first tokens: the parts of prefixes that
-// blocks share (two a block), a logarithm for each head of a sequence, and the plan
+// blocks share (two a block), a maximum and a sum for each head of a sequence, and the plan
 // (paged_attention.h) of up to IHIP_PAGED_SEQS groups
 constexpr uint64_t SHARED_PIECE_BYTES = 36u << 20;
 constexpr int64_t SHARED_HEADS = 1 << 20;
-constexpr uint64_t SHARED_BYTES = SHARED_PIECE_BYTES + SHARED_HEADS * 4 + (4 + 3 * IHIP_PAGED_SEQS) * 4;
+constexpr uint64_t SHARED_BYTES = SHARED_PIECE_BYTES + SHARED_HEADS * 8 + (4 + 3 * IHIP_PAGED_SEQS) * 4;
 // logprobs: blocks up to which rows are split into parts, the parts' results (3
 // doubles and IHIP_LOGPROBS_TOP alternatives each), and a counter of 32 bytes a row
 constexpr int64_t LOGPROBS_BLOCKS = 1024;

@@ -160,7 +160,7 @@ int paged_attention(const char* who, ihip_ctx* c, uint64_t q, int64_t q_stride, 
     int32_t seqs, heads, kvh, hd, page_size, max_pages, group, tiles, rows, cus;
     uint64_t ks, vs;  // (of 8-bit pages' and the groups' kernels alone, as what follows)
     int64_t s_page, s_slot, s_head;
-    uint64_t members, shared, pieces, lse, plan;  // (of the groups' kernels alone)
+    uint64_t members, shared, pieces, sums, plan;  // (of the groups' kernels alone)
     int32_t groups, pad;
   } a = {(const float*)q, (const char*)cache->k, (const char*)cache->v, (const int*)table,
          (const int*)lengths, (const int*)offsets, (float*)y, (const float*)sinks, (float*)c->paged_part,
@@ -170,7 +170,7 @@ int paged_attention(const char* who, ihip_ctx* c, uint64_t q, int64_t q_stride, 
          (int32_t)heads, (int32_t)kvh, (int32_t)hd, cache->page_size, (int32_t)max_pages, (int32_t)group,
          (int32_t)tiles, (int32_t)rows, c->cus, q8_scales(cache, 0), q8_scales(cache, 1), p.s_page, p.s_slot, p.s_head,
          groups ? groups->members : 0, groups ? groups->shared : 0, c->paged_shared, c->paged_shared + SHARED_PIECE_BYTES,
-         c->paged_shared + SHARED_PIECE_BYTES + SHARED_HEADS * 4, groups ? (int32_t)groups->groups : 0, 0};
+         c->paged_shared + SHARED_PIECE_BYTES + SHARED_HEADS * 8, groups ? (int32_t)groups->groups : 0, 0};
   const int d = hd <= 64 ? 64 : hd <= 128 ? 128 : hd <= 256 ? 256 : 512;
   char name[40];
   // (a window's keys are few: every sequence reads its own)

@@ -39,7 +39,7 @@ struct PagedAttn8Args : PagedAttnArgs {
 struct PagedSharedArgs : PagedAttn8Args {
   const int *members, *shared;  // [groups + 1], [groups]: a group's sequences, their common tokens
   float* pieces;  // [blocks][2][16 CT (hd + 2)]: parts of a prefix that blocks share
-  float* lse;     // [seqs][heads], base 2: of a prefix that one block has finished, into y
+  float* sums;    // [seqs][heads][2], the maximum (base 2) and sum of a prefix that is one block's, its values in y
   int* plan;      // SHARED_PLAN's numbers, then [groups][3]: tiles before the group's, keys' tiles, columns' tiles
   int32_t groups, pad;
 };
@@ -241,7 +241,7 @@ struct AttnLds : AttnScales<T> {
 // a tile's heads' part of a prefix (PagedSharedArgs), in LDS
 struct AttnPrefix {
   float m[16], l[16];          // its maxima (base 2) and sums
-  int first[16], count[16];    // the blocks of its pieces; count 0: in y and lse
+  int first[16], count[16];    // the blocks of its pieces; count 0: in y and sums
   int col[16];                 // a head's column in the pieces
   int members[64], shared[64]; // the groups, of 3 to 63 (of fewer the search reads no more)
 };
@@ -530,8 +530,11 @@ __device__ __forceinline__ void paged_attention_t(const A& a)
         const int c16 = col % pct;
         float m = -__builtin_inff(), l = 0.f;
         if (b0 == b1) {
-          if ((t & 15) == 0) m = a.lse[(int64_t)it.s * a.heads + it.head0 + h];
-          l = m == -__builtin_inff() ? 0.f : 1.f;
+          if ((t & 15) == 0) {
+            const float* const e = a.sums + 2 * ((int64_t)it.s * a.heads + it.head0 + h);
+            m = e[0];
+            l = e[1];
+          }
         } else {
           for (int i = t & 15; i <= b1 - b0; i += 16) {
             const float* const e = a.pieces + (2 * (int64_t)(b0 + i) + (i == 0)) * size + pct * a.hd + c16;

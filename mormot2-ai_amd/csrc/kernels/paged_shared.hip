@@ -118,8 +118,8 @@ __device__ __forceinline__ void prefix_walk(const PagedSharedArgs& a, const int*
 // reads the prefix's keys and values once for 16 CT of them: scores K q^T and values V^T
 // P as paged_attention's, a wave's keys and values in registers used for CT tiles of 16
 // columns, the query tiles in LDS. All groups' tiles of keys are one row, shared out
-// evenly over the grid. A block that has the whole of an item (KV head, columns) finishes
-// it into y and lse; parts go to `pieces`, and the launch over the sequences' own tokens
+// evenly over the grid. A block that has the whole of an item (KV head, columns) leaves
+// it in y and sums; parts go to `pieces`, and the launch over the sequences' own tokens
 // joins them. Bound by issue where a group is large (128 sequences behind 30011 tokens, 64
 // heads of 64 over 8 in bf16 235 us: vector work 69%, matrix cores 40% of the SIMDs' time, of
 // weights in three parts), by loads' latency where its columns are few (the sizes at
@@ -622,10 +622,13 @@ __device__ __forceinline__ void paged_prefix_t(const PagedSharedArgs& a)
       }
       __syncthreads();
     }
-    // the columns' results: to y and lse, or to the pieces
+    // the columns' results: to y and sums, or to the pieces
     if (t < COLS && s.at[t] >= 0) {
       if (whole) {
-        a.lse[(int64_t)(m0 + (col0 + t) / a.group) * a.heads + s.head[t]] = s.l[t] == 0.f ? s.m[t] : s.m[t] + __builtin_amdgcn_logf(s.l[t]);
+        // (the maximum and the sum apart: one logarithm loses half a step of a large maximum)
+        float* const e = a.sums + 2 * ((int64_t)(m0 + (col0 + t) / a.group) * a.heads + s.head[t]);
+        e[0] = s.m[t];
+        e[1] = s.l[t];
       } else {
         pc[COLS * a.hd + t] = s.m[t];
         pc[COLS * a.hd + COLS + t] = s.l[t];
@@ -637,10 +640,9 @@ __device__ __forceinline__ void paged_prefix_t(const PagedSharedArgs& a)
       if (s.at[col] < 0) continue;
       const floatx4 v = walked ? *(const floatx4*)&s.o[ct][0][(col & 15) * S::OS + d] : value(ct, i % (16 * hd));
       if (whole) {
-        const float L = s.l[col], inv = L != 0.f ? 1.f / L : 0.f;
         float* const y = a.y + s.at[col] * row_out + (int64_t)s.head[col] * a.hd + d;
 #pragma unroll
-        for (int e = 0; e < 4; e++) y[e] = L == 0.f ? 0.f : v[e] * inv;
+        for (int e = 0; e < 4; e++) y[e] = v[e];
       } else {
         *(floatx4*)(pc + col * a.hd + d) = v;
       }
