@@ -679,9 +679,10 @@ int ihip_enqueue_paged_qkrope(ihip_ctx* ctx, uint64_t q, int64_t q_stride, uint6
  * sqrt(head_dim)); table [seqs, max_pages], q rows of q_stride floats (0: heads *
  * head_dim); y may be q's own contiguous rows, and is refused where it overlaps
  * them in another way. A key whose table entry is outside the pool is not there,
- * one whose score is -infinity has weight 0, and so has a sink of -infinity. A
- * sequence with no key (length 0), or whose keys have no weight, gives zeros, one
- * with lengths[s] < 0 leaves its row of y as it was.
+ * one whose score is -infinity has weight 0, and so has a sink of -infinity; a sink
+ * of +infinity has all of the weight, which gives zeros. A sequence with no key
+ * (length 0), or whose keys have no weight, gives zeros, one with lengths[s] < 0
+ * leaves its row of y as it was.
  * (ihip_enqueue_attention over a paged cache) */
 int ihip_enqueue_paged_attention(ihip_ctx* ctx, uint64_t q, int64_t q_stride,
                                  const ihip_pages* cache, uint64_t table, int64_t max_pages,

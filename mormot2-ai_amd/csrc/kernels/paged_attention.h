@@ -579,10 +579,12 @@ __device__ __forceinline__ void paged_attention_t(const A& a)
       auto top = [&](float x) { M = x > M || x != x ? x : M; };
       if (l != 0.f) top(m);
       if (pl != 0.f) top(pm);
+      // (a sink above all of them has weight 1, an infinite one too, as in finish)
       const float sk = a.sinks ? a.sinks[it.head0 + h] * LOG2E : -__builtin_inff();
-      if (sk != -__builtin_inff()) top(sk);
+      const bool sink = sk > M;
+      if (sink) M = sk;
       const float fo = l != 0.f ? exp2_fast(m - M) : 0.f, fp = pl != 0.f ? exp2_fast(pm - M) : 0.f;
-      const float L = l * fo + pl * fp + (sk != -__builtin_inff() ? exp2_fast(sk - M) : 0.f);
+      const float L = l * fo + pl * fp + (sink ? 1.f : sk != -__builtin_inff() ? exp2_fast(sk - M) : 0.f);
       float p[4] = {0.f, 0.f, 0.f, 0.f};
       if (pl != 0.f) {
         if (px.count[h] == 0) {
@@ -614,7 +616,7 @@ __device__ __forceinline__ void paged_attention_t(const A& a)
 #pragma unroll
       for (int i = 0; i < 4; i++) {
         const float x = (fo != 0.f ? v[i] * fo : 0.f) + (fp != 0.f ? p[i] * fp : 0.f);
-        v[i] = L != 0.f ? x / L : 0.f;
+        v[i] = L != 0.f && (l != 0.f || pl != 0.f) ? x / L : 0.f;
       }
     }
   };
@@ -1004,6 +1006,10 @@ __device__ __forceinline__ void paged_attention_t(const A& a)
     // with the sink: its weight beside the sum's, both against the larger maximum
     auto finish = [&](int h, float m2, float l2, float& f2) {
       f2 = 1.f;
+      if (is_shared<A> && l2 == 0.f) {  // (no key has a weight: zeros, whatever the sink)
+        f2 = 0.f;
+        return;
+      }
       if (a.sinks) {
         const float sk = a.sinks[it.head0 + h] * LOG2E;
         if (sk > m2) {

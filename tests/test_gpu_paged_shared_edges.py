@@ -1,4 +1,5 @@
-"""Attention of groups that share their first tokens, beside that without groups: large scores, for prefixes that one block finishes and that blocks share."""
+"""Attention of groups that share their first tokens, beside that without groups: large scores and
+sinks that are infinite, for prefixes that one block finishes and that blocks share."""
 import ctypes as C
 
 import numpy as np
@@ -55,3 +56,29 @@ def test_large_scores_of_all_keys(ctx, dev, dtype, hd, prefix):
     want = np.array([(prefix - o) / (prefix + o) for o in own])[:, None, None] * np.ones_like(got)
     assert_close(got, want, 2 * R.U * np.abs(want) + 1e-12)
     assert_close(alone(ctx, dev, b), want, 2 * R.U * np.abs(want) + 1e-12)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("prefix", [30, 1900])
+def test_sinks_of_infinity(ctx, dev, dtype, prefix):
+    """A sink of +infinity, or one that its scaling makes so, has all of the weight, one of -infinity
+    none, a NaN is one: in a group as without it. A sequence without a key gives zeros."""
+    rng = np.random.default_rng(prefix)
+    b = Batch(rng, dtype, 128, 8, 2, 16, [(6, prefix, -(-prefix // 16) * 16)],
+              [prefix, prefix + 1, prefix + 40, 5, 0, prefix + 300], alone=2, behind=1)
+    b.lengths[0] = 0  # (outside the group too)
+    big = np.finfo(np.float32).max
+    b.sinks = np.array([np.inf, -np.inf, 0.5, big, -big, np.nan, -2.0, 1.0], np.float32)
+    b.upload(dev)
+    b.enqueue(ctx)
+    got, without = b.read(), alone(ctx, dev, b)
+    off = b.sinks.copy()
+    off[[0, 3, 4, 5]] = -np.inf
+    b.sinks = off
+    want, tol = b.want()
+    want[:, [0, 3]], tol[:, [0, 3]] = 0, 0
+    live = b.lengths > 0
+    ok = [0, 1, 2, 3, 4, 6, 7]
+    for y in (got, without):
+        assert_close(y[:, ok], want[:, ok], tol[:, ok])
+        assert np.isnan(y[live, 5]).all() and (y[b.lengths == 0] == 0).all()
