@@ -9,6 +9,7 @@
 #include <string>
 
 #include "internal.h"
+#include "../paged.h"
 #include "../sample_rows.h"
 
 using namespace ihip;
@@ -176,7 +177,7 @@ int paged_attention(const char* who, ihip_ctx* c, uint64_t q, int64_t q_stride, 
   // (a window's keys are few: every sequence reads its own)
   const bool prefix = groups && window == 0;
   if (prefix) {
-    const int64_t cols = d <= 64 ? 64 : d <= 128 || (d == 256 && cache->dtype != IHIP_Q8_HEAD) ? 32 : 16;  // shared_ct's
+    const int64_t cols = 16 * PAGED_SHARED_TILES(d, cache->dtype == IHIP_Q8_HEAD);
     snprintf(name, sizeof name, "paged_prefix_%s_%d%s", p.type, d, hd == d ? "" : "_part");
     int64_t blocks = (int64_t)c->cus * resident_blocks(c, name, 256);
     blocks = std::min<int64_t>({blocks, PAGED_BLOCKS, (int64_t)(SHARED_PIECE_BYTES / (2 * cols * (hd + 2) * 4)), units * seqs});

@@ -13,7 +13,7 @@ using namespace ihip;
 // prompts of 9001 68 us; two and one block 95 where one took 80). Others of 256 have two and
 // one block (halves 97 us; one and two that spill 135 where two took 111).
 template <int T, int D>
-constexpr int shared_ct = D <= 64 ? 4 : D <= 128 ? 2 : D == 256 && T != 3 ? 2 : 1;
+constexpr int shared_ct = PAGED_SHARED_TILES(D, T == 3);
 template <int T, int D>
 constexpr int shared_blocks = D <= 128 || (D == 256 && T == 3) ? 2 : 1;
 

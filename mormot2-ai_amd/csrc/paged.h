@@ -32,6 +32,10 @@ IHIP_HD int64_t paged_common(int32_t first, int32_t end, int32_t shared, int32_t
   return shared < most ? shared : most;
 }
 
+// the columns (a member's query head each) that a block of the prefixes' kernel for heads of up
+// to d takes, in tiles of 16: its registers' share, and the size of the pieces that it leaves
+#define PAGED_SHARED_TILES(d, q8) ((d) <= 64 ? 4 : (d) <= 128 || ((d) == 256 && !(q8)) ? 2 : 1)
+
 // the row of q and y of a sequence whose rows of the step are [first, end): the
 // last of them, or -1 where it has none or its last is not among the `rows`
 IHIP_HD int32_t paged_row(int32_t first, int32_t end, int32_t rows)
