@@ -586,7 +586,10 @@ int ihip_prompt_cache_stats(ihip_prompt_cache* pc, int64_t* requests, int64_t* h
 
 /* 8-bit pages (ihip_pages.dtype alone, not an element type of tensors): the values
  * of a head of a token are int8 codes times one single scale, 1 / 127 of the head's
- * largest magnitude; 0.52 of a half's bytes for heads of 128 */
+ * largest magnitude; 0.52 of a half's bytes for heads of 128. Attention adds them up as
+ * values in single, but for what weights lose beside the largest value scale of their
+ * sequence and KV head, 2^-39 of that one each: as much as single's roundings where
+ * scales are 2^15 apart */
 #define IHIP_Q8_HEAD 64
 
 /* the pool of one layer. A slot is page * page_size + token: the values of a

@@ -208,7 +208,8 @@ struct AttnShape {
   static constexpr int OS = D + 4;                     // a head's row in o_s
   // weights enter the product times this: into the halves' normal range. The two parts
   // hold 22 bits of those down to 2^-18 of the largest; smaller ones are off by 2^-40 of
-  // the largest at most
+  // the largest at most. (8-bit pages: of weights times their values' scales, off by 2^-39
+  // of the largest scale that the wave has met, whatever that one's weight)
   static constexpr float PS = T == 1 || T == 3 ? 32768.f : 1.f;
 
   // the first of the FL values that lane group g has of factor f: 8-bit keys come in loads
