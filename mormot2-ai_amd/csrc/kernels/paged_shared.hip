@@ -6,12 +6,15 @@
 
 using namespace ihip;
 
-// Columns (a member's query head each) of a block: 16 CT. As many as leave two blocks a CU
-// their registers: heads of 128 two tiles (32 chats behind 4096 tokens 26 us; four tiles
-// and one block a CU 33, four that spill 53), of 64 four (128 sequences behind 30011
-// 240 us; two and three blocks a CU 245, two and four 310), of 256 in 8-bit pages one (three
-// prompts of 9001 68 us; two and one block 95 where one took 80). Others of 256 have two and
-// one block (halves 97 us; one and two that spill 135 where two took 111).
+// Columns (a member's query head each) of a block: 16 CT. As many as the loop over keys holds
+// in the registers of two blocks a CU: heads of 128 two tiles (32 chats behind 4096 tokens 26
+// us; four tiles and one block a CU 33, four and two blocks 53), of 64 four (128 sequences
+// behind 30011 240 us; two and three blocks a CU 245, two and four 310), of 256 in 8-bit
+// pages one (three prompts of 9001 68 us; two and one block 95 where one took 80). Others of
+// 256 have two and one block (halves 97 us; one and two blocks 135 where two took 111). What
+// lives from an item's start to its end does not fit beside that loop: the compiler spills up to 61
+// registers (halves of 128 34, 8-bit heads of 256 26, and 67 of paged_own's; none of 512),
+// which are stored and loaded once an item. Sizes between these have up to 11 loads a step.
 template <int T, int D>
 constexpr int shared_ct = PAGED_SHARED_TILES(D, T == 3);
 template <int T, int D>

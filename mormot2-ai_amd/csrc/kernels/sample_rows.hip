@@ -570,6 +570,10 @@ extern "C" __global__ __launch_bounds__(256) void sample_rows_finish(SampleRowsA
   float least = (float)lo;
   if ((double)least > lo) least = key_logit(row_key(least) - 1);
   if (!(least > -3.4028235e38f)) least = -3.4028235e38f;  // (infinities and NaN are no candidates)
+  // (Rows with top-k have no bins by the grid. Where their octaves do not hold k tokens - large k,
+  // or a low temperature, at which few tokens lie within 2^-32 of their part's best - one
+  // block walks the row several times: 16 rows of 151936 at temperature 0.1 with top-k 40
+  // 765 us, 21 at 0.8.)
   if (state == ROW_MANY && !by_k) {
     if (t == 0) {
       slot = atomicAdd(a.heavy, 1);
